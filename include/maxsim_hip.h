@@ -396,6 +396,87 @@ int msim_binary_cascade_topk_async(msim_binary_docs* h, const float* d_query, in
                                    int64_t query_tokens, int64_t k, int64_t candidates,
                                    float* d_scores, int64_t* d_indices, void* stream);
 
+/* ===================================================================== */
+/* 4-bit key/value cache of a reader model (no counterpart in the         */
+/* reference, which ends at the passages' scores).                       */
+/* ===================================================================== */
+/* Keys and values are kept in the corpus' row format: per token and head one
+ * single precision scale s = max|x| / 7 (1 for a row of zeros) and codes
+ * clip(rint(x / s), -7, 7) in two's complement nibbles, even dim low.  A row
+ * that holds an infinity or a NaN is kept as the scale NaN.  Rows live in the
+ * pages of a pool that the caller allocates; a sequence is a row of a page
+ * table and a length.  Everything is in device memory, every call only enqueues.
+ *
+ * rows of a call: packed; rows [offsets[b], offsets[b + 1]) are the last ones
+ * of sequence b, whose lengths[b] counts them already.  offsets NULL: one row
+ * per sequence.  Lengths are cut to the table, rows to the row count; a page
+ * number outside the pool is a hole: not written, read back as zeros, taking
+ * no attention. */
+typedef struct msim_kv4_pool {
+  uint8_t* k_codes;  /* [num_pages, kv_heads, page_size, dim / 2], 16-byte aligned */
+  float* k_scales;   /* [num_pages, kv_heads, page_size], 16-byte aligned */
+  uint8_t* v_codes;
+  float* v_scales;
+  int64_t num_pages;
+  int32_t kv_heads;
+  int32_t page_size; /* a power of two, 16 to 65536 */
+  int32_t dim;       /* 64, 96, 128, 192 or 256 */
+} msim_kv4_pool;
+
+/* Types of rows, queries, outputs and inputs. */
+#define MSIM_F32 0
+#define MSIM_F16 1
+#define MSIM_BF16 2
+
+/* Keys and values [rows, kv_heads, dim] (strides in elements, dims dense)
+ * quantised into the cache.  Rows that share a slot leave one of them. */
+int msim_kv4_append_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                          const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                          const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_row_stride, int64_t v_head_stride, int type, void* stream);
+/* The same rows read back: code * scale, rounded once to `type`. */
+int msim_kv4_read_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                        const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows, void* k,
+                        int64_t k_row_stride, int64_t k_head_stride, void* v, int64_t v_row_stride,
+                        int64_t v_head_stride, int type, void* stream);
+/* Bytes of device workspace that msim_kv4_attend_async needs for these sizes. */
+int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
+                              int64_t heads, uint64_t* bytes);
+/* Attention of queries [rows, heads, dim] over the cache: head h reads key/value
+ * head h / (heads / kv_heads).  A row at position p = length - rows + i sees keys
+ * j < length with, if causal, j <= p; j > p - window (window 0: all); mask[row, j]
+ * != 0 (mask NULL: all; keys past mask_width are hidden).  out = softmax(scale
+ * q.k) v in the queries' type; lse f32 [rows, heads] (NULL: not wanted) the
+ * logarithm of the softmax's sum.  A row that sees nothing: zeros, -infinity.
+ * The workspace (16-byte aligned) is used until the call's work is done. */
+int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                          const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                          const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads, int type,
+                          double scale, int causal, int64_t window, const uint8_t* mask,
+                          int64_t mask_row_stride, int64_t mask_width, void* out, int64_t out_row_stride,
+                          int64_t out_head_stride, float* lse, void* workspace, uint64_t workspace_bytes,
+                          void* stream);
+
+/* ===================================================================== */
+/* Products with a matrix in 4 bits and group scales (no counterpart in   */
+/* the reference): y = x W^T (+ bias), w[n, k] = code[n, k] * scale[n,    */
+/* k / group].                                                            */
+/* ===================================================================== */
+/* Bytes of the matrix as the product reads it. */
+int msim_linear4_layout_bytes(int64_t n, int64_t k, int64_t group, uint64_t* codes_bytes, uint64_t* scales_bytes);
+/* Lays a matrix out, once: codes u8 [n, k / 2] (two's complement nibbles, even
+ * column low, 4-byte aligned), scales bfloat16 [n, k / group]; group 32, 64 or
+ * 128, k a multiple of it.  Device pointers; only enqueues. */
+int msim_linear4_layout_async(const uint8_t* codes, const uint16_t* scales, int64_t n, int64_t k, int64_t group,
+                              uint8_t* out_codes, uint16_t* out_scales, void* stream);
+/* x [rows, k] (row stride in elements) times the matrix's rows, sums in single
+ * precision, rounded once to `type` into out [rows, n].  bias f32 [n] or NULL.
+ * Meant for few rows (it reads the matrix once per 32 of them); an infinity in x
+ * may come out as a NaN. */
+int msim_linear4_async(const uint8_t* codes, const uint16_t* scales, int64_t n, int64_t k, int64_t group,
+                       const float* bias, const void* x, int64_t rows, int64_t x_row_stride, int type, void* out,
+                       int64_t out_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

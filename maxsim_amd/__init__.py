@@ -31,7 +31,8 @@ from maxsim_amd.experimental import (
     pack_int4_symmetric_device,
     topk_int4_maxsim,
 )
-
+from maxsim_amd.kvcache import Int4KVCache
+from maxsim_amd.linear4 import Int4Linear, pack_int4_groups
 from maxsim_amd.sdk import MODE_PRESETS, Corpus, CorpusMemoryReport, Index, Reranker, SearchResult
 
 __all__ = [
@@ -52,12 +53,15 @@ __all__ = [
     "prefix_topk",
     "residual_int4_to_device",
     "residual_score",
+    "Int4KVCache",
+    "Int4Linear",
     "Int4PackedDocs",
     "PackedDocs",
     "int4_maxsim",
     "int4_maxsim_int8q",
     "int4_to_device",
     "maxsim",
+    "pack_int4_groups",
     "pack_int4_symmetric",
     "pack_int4_symmetric_device",
     "pack_query_signs",

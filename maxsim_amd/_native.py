@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libmaxsim_hip.so")
 MSIM_OK, MSIM_EINVAL, MSIM_ERUNTIME, MSIM_ENOTSUP = 0, 1, 2, 3
 
 c_i64 = ctypes.c_int64
+c_u64 = ctypes.c_uint64
 c_int = ctypes.c_int
 c_dbl = ctypes.c_double
 c_vp = ctypes.c_void_p
@@ -93,6 +94,18 @@ SIGNATURES: dict[str, list] = {
     "msim_binary_binres_topk": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp],
     "msim_binary_cascade_topk": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp],
     "msim_binary_cascade_topk_async": [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp],
+    # 4-bit key/value cache
+    "msim_kv4_append_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+                              c_int, c_vp],
+    "msim_kv4_read_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+                            c_int, c_vp],
+    "msim_kv4_attend_workspace": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp],
+    "msim_kv4_attend_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_dbl,
+                              c_int, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_u64, c_vp],
+    # products with a 4-bit matrix
+    "msim_linear4_layout_bytes": [c_i64, c_i64, c_i64, c_vp, c_vp],
+    "msim_linear4_layout_async": [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp],
+    "msim_linear4_async": [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_i64, c_vp],
 }
 
 _RESTYPES = {"msim_last_error": ctypes.c_char_p, "msim_get_fused_wait_ticks": c_i64}
@@ -126,6 +139,19 @@ class BinaryProps(ctypes.Structure):
         ("token_scale_vector_size", ctypes.c_uint64),
         ("resident_bytes", ctypes.c_uint64),
         ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class Kv4Pool(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", c_vp),
+        ("k_scales", c_vp),
+        ("v_codes", c_vp),
+        ("v_scales", c_vp),
+        ("num_pages", c_i64),
+        ("kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
     ]
 
 

@@ -1,0 +1,59 @@
+// codes4.hpp -- 4-bit codes and single precision values as operands of
+// v_mfma_f32_16x16x32_f16 / _bf16.
+#pragma once
+
+#include "common.hpp"
+
+namespace msim {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v4f mfma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// A pair of codes under a constant exponent, bits 3..6 of both halves: 24 + code
+// in bfloat16 and 136 + code in f16 (the sign bit turned).
+__device__ __forceinline__ uint32_t pair_bf16_24(uint32_t w) { return (w & 0x00780078u) ^ 0x41C041C0u; }
+__device__ __forceinline__ uint32_t pair_f16(uint32_t w) {
+  const v2h base = {(_Float16)136.0f, (_Float16)136.0f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & 0x00780078u) ^ 0x58405840u) - base);
+}
+// The codes themselves in bfloat16: single precision differences, all exact.
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
+  const uint32_t r = pair_bf16_24(w);
+  const float lo = __uint_as_float(r << 16) - 24.0f, hi = __uint_as_float(r & 0xFFFF0000u) - 24.0f;
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// Three bfloat16 parts (in the upper halves) that sum to x exactly: the upper
+// eight bits of the significand, the next eight, the rest.  An infinity or a
+// NaN is its first part alone.
+__device__ __forceinline__ void split3(uint32_t x, uint32_t (&part)[3]) {
+  const bool special = (x & 0x7F800000u) == 0x7F800000u;
+  const uint32_t a = x & 0xFFFF0000u;
+  const float r1 = special ? 0.0f : __uint_as_float(x) - __uint_as_float(a);
+  const uint32_t b = __float_as_uint(r1) & 0xFFFF0000u;
+  part[0] = special && (x & 0x007FFFFFu) ? 0x7FC00000u : a;
+  part[1] = b;
+  part[2] = __float_as_uint(r1 - __uint_as_float(b));
+}
+
+// Eight single precision values as three operands.
+__device__ __forceinline__ void split3(const uint32_t (&x)[8], v8b (&out)[3]) {
+  v4u parts[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo[3], hi[3];
+    split3(x[2 * i], lo);
+    split3(x[2 * i + 1], hi);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) parts[k][i] = __builtin_amdgcn_perm(hi[k], lo[k], 0x07060302u);
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(v8b, parts[k]);
+}
+
+}  // namespace msim

@@ -1,0 +1,230 @@
+// kv4_rows.hip -- key and value rows into the 4-bit cache, and back.
+//
+//   append:  s = f32(max|x|) / f32(7) (0 -> 1), c = clip(rint(x / s), -7, 7)
+//            as the corpus packer does, the quotient rounded to single precision
+//            before rint; a row that holds an infinity or a NaN gets the scale
+//            NaN (it reads back as NaN, and so does attention that reaches it)
+//   read:    c * s, rounded once to the type asked for
+//
+// Byte work, bound by HBM: dim * (2 or 4) bytes in and dim / 2 + 4 out per row
+// and head, or the reverse.
+#include "kv4.hpp"
+
+namespace msim {
+
+namespace {
+
+template <Kv4Type T>
+struct Elem;
+template <>
+struct Elem<kKv4F32> {
+  typedef float type;
+};
+template <>
+struct Elem<kKv4F16> {
+  typedef _Float16 type;
+};
+template <>
+struct Elem<kKv4BF16> {
+  typedef __bf16 type;
+};
+
+// Eight elements as single precision bits.
+template <Kv4Type T>
+__device__ __forceinline__ void load8(const void* p, bool wide, uint32_t (&x)[8]) {
+  if constexpr (T == kKv4F32) {
+    const uint32_t* u = static_cast<const uint32_t*>(p);
+    if (wide) {
+      const v4u a = reinterpret_cast<const v4u*>(u)[0], b = reinterpret_cast<const v4u*>(u)[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = u[i];
+    }
+  } else {
+    const uint16_t* u = static_cast<const uint16_t*>(p);
+    uint32_t w[4];
+    if (wide) {
+      const v4u a = *reinterpret_cast<const v4u*>(u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = a[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+      x[i] = T == kKv4BF16 ? (uint32_t)h << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, h));
+    }
+  }
+}
+
+// Eight single precision values stored in type T, each rounded once.
+template <Kv4Type T>
+__device__ __forceinline__ void store8(void* p, bool wide, const float (&x)[8]) {
+  typedef typename Elem<T>::type E;
+  E e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = (E)x[i];
+  if (wide) {
+    constexpr int kWords = sizeof(E) * 8 / 16;
+    v4u w[kWords];
+    __builtin_memcpy(w, e, sizeof e);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<v4u*>(p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) static_cast<E*>(p)[i] = e[i];
+  }
+}
+
+// Lanes that share a row (8 elements each), a power of two.
+constexpr int row_lanes(int dim) { return dim <= 64 ? 8 : (dim <= 128 ? 16 : 32); }
+
+template <int N>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+#pragma unroll
+  for (int i = 1; i < N; i *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, i));
+  return v;
+}
+
+// Slot of row `row` (each group of lanes has its own row; all 64 lanes call).
+__device__ __forceinline__ bool row_slot(const Kv4Pool& pool, const Kv4Batch& batch, int row, Kv4Slot& slot) {
+  const int first = wave_uniform(row);
+  int b = -1;
+  if (batch.offsets == nullptr) {
+    b = row < min(batch.batch, batch.rows) ? row : -1;
+  } else if (first < batch.rows) {
+    b = kv4_find_sequence(batch, first);
+    // Most waves lie inside one sequence; the others search on, lane by lane.
+    if (b >= 0 && row >= kv4_first_row(batch, b + 1)) b = kv4_find_sequence_from(batch, row, b);
+    if (b < 0 && row != first) b = kv4_find_sequence_from(batch, row, 0);
+  }
+  return row < batch.rows && b >= 0 && kv4_slot(pool, batch, b, row, slot);
+}
+
+template <Kv4Type T, int kDim>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Pool pool, Kv4Batch batch, Kv4Rows keys, Kv4Rows values,
+                                                         bool wide) {
+  typedef typename Elem<T>::type E;
+  constexpr int kLanes = row_lanes(kDim), kRows = 256 / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int head = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1;
+  const Kv4Rows& src = value ? values : keys;
+  const bool have = row < batch.rows && part * 8 < kDim;
+  uint32_t x[8] = {};
+  if (have)
+    load8<T>(static_cast<const E*>(src.ptr) + row * src.row_stride + head * src.head_stride + part * 8, wide, x);
+  Kv4Slot slot;
+  const bool placed = row_slot(pool, batch, row, slot);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, x[i] & 0x7FFFFFFFu);
+  m = lanes_max<kLanes>(m);
+  // The bits pass through an empty asm, so that this stays an integer test
+  // where the compiler assumes that no value is a NaN.
+  asm volatile("" : "+v"(m));
+  const bool finite = m < 0x7F800000u;
+  float s = finite ? __fdiv_rn(__uint_as_float(m), 7.0f) : 1.0f;
+  if (s == 0.0f) s = 1.0f;
+  int c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = rintf(__fdiv_rn(__uint_as_float(x[i]), s));
+    c[i] = finite ? (int)fminf(fmaxf(r, -7.0f), 7.0f) : 0;
+  }
+  if (!placed || !have) return;
+  const int64_t at = kv4_pool_row(pool, slot.page, head, slot.slot);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= (uint32_t)(c[i] & 15) << (4 * i);
+  *reinterpret_cast<uint32_t*>(pool.codes[value] + at * (kDim / 2) + part * 4) = w;
+  if (part == 0) reinterpret_cast<uint32_t*>(pool.scales[value])[at] = finite ? __float_as_uint(s) : 0x7FC00000u;
+}
+
+template <Kv4Type T, int kDim>
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Pool pool, Kv4Batch batch, Kv4Rows keys, Kv4Rows values,
+                                                       bool wide) {
+  typedef typename Elem<T>::type E;
+  constexpr int kLanes = row_lanes(kDim), kRows = 256 / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int head = blockIdx.y >> 1;
+  const bool value = blockIdx.y & 1;
+  const Kv4Rows& dst = value ? values : keys;
+  Kv4Slot slot;
+  const bool placed = row_slot(pool, batch, row, slot);
+  if (row >= batch.rows || part * 8 >= kDim) return;
+  uint32_t w = 0;
+  float s = 0.0f;
+  if (placed) {
+    const int64_t at = kv4_pool_row(pool, slot.page, head, slot.slot);
+    w = *reinterpret_cast<const uint32_t*>(pool.codes[value] + at * (kDim / 2) + part * 4);
+    s = pool.scales[value][at];
+  }
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)((int)(w << (28 - 4 * i)) >> 28) * s;
+  store8<T>(static_cast<E*>(dst.ptr) + row * dst.row_stride + head * dst.head_stride + part * 8, wide, x);
+}
+
+// 16-byte accesses: every row of every head starts on 16 bytes.
+bool rows_aligned(const Kv4Rows& r, int size) {
+  return reinterpret_cast<uintptr_t>(r.ptr) % 16 == 0 && r.row_stride * size % 16 == 0 && r.head_stride * size % 16 == 0;
+}
+
+template <Kv4Type T, int kDim>
+hipError_t launch_rows(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], bool append,
+                       hipStream_t stream) {
+  constexpr int kRows = 256 / row_lanes(kDim);
+  const int size = T == kKv4F32 ? 4 : 2;
+  const bool wide = rows_aligned(rows[0], size) && rows_aligned(rows[1], size);
+  const dim3 grid((unsigned)((batch.rows + kRows - 1) / kRows), (unsigned)pool.kv_heads * 2);
+  if (append)
+    kv4_append_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], wide);
+  else
+    kv4_read_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], wide);
+  return hipGetLastError();
+}
+
+template <Kv4Type T>
+hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], bool append,
+                       hipStream_t stream) {
+  switch (pool.dim) {
+    case 64: return launch_rows<T, 64>(pool, batch, rows, append, stream);
+    case 96: return launch_rows<T, 96>(pool, batch, rows, append, stream);
+    case 128: return launch_rows<T, 128>(pool, batch, rows, append, stream);
+    case 192: return launch_rows<T, 192>(pool, batch, rows, append, stream);
+    case 256: return launch_rows<T, 256>(pool, batch, rows, append, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], Kv4Type type, bool append,
+                  hipStream_t stream) {
+  if (batch.rows <= 0) return hipSuccess;
+  switch (type) {
+    case kKv4F32: return launch_type<kKv4F32>(pool, batch, rows, append, stream);
+    case kKv4F16: return launch_type<kKv4F16>(pool, batch, rows, append, stream);
+    case kKv4BF16: return launch_type<kKv4BF16>(pool, batch, rows, append, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_kv4_append(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], Kv4Type type,
+                             hipStream_t stream) {
+  return launch(pool, batch, rows, type, true, stream);
+}
+
+hipError_t launch_kv4_read(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], Kv4Type type,
+                           hipStream_t stream) {
+  return launch(pool, batch, rows, type, false, stream);
+}
+
+}  // namespace msim

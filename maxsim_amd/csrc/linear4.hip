@@ -1,0 +1,310 @@
+// linear4.hip -- y = x W^T for few rows x and a matrix W in 4 bits:
+//
+//   y_mn = sum over groups G of s_nG (sum_{k in G} x_mk c_nk)  (+ bias_n)
+//
+// On v_mfma_f32_16x16x32: A is 16 rows of W times 32 columns, B the same
+// columns of up to 16 rows of x, so that a lane's accumulators are four rows
+// of W (its scales) by one row of x.  A group's sum is a chain of group / 32
+// MFMAs; its scales multiply the sum, in single precision, and nothing else is
+// dequantised.
+//
+// Codes in the registers of the MFMA.  A word holds eight columns of a row as
+// nibbles, turned left by three bits: bits 3..6 of a half, under a constant
+// exponent, make 16 + (code ^ 8) = 24 + code in bfloat16 (7 mantissa bits) and
+// 136 + code in f16 (10 bits), by one bitwise operation per pair.
+//   bfloat16 x: the 24 stays; the chain starts from -24 sum(x), which one more
+//     MFMA gives (every row of its A is -24), so the sum is of the codes again.
+//     The products are exact and the offset costs 24 / |c| times the rounding
+//     of single precision sums, 2^-19 or so against bfloat16's 2^-9.
+//   f16 x: 136 is subtracted (exactly) before the product.
+//   f32 x: three bfloat16 parts that sum to x exactly, codes made exact.
+//
+// Bytes bound it: n k / 2 and the scales, for any number of rows that fits a
+// pass (32).  Waves of a workgroup take the 128-column tiles of the same rows of W in
+// turn and join in LDS in a fixed order.
+#include "codes4.hpp"
+#include "linear4.hpp"
+
+namespace msim {
+
+namespace {
+
+// One thread per word of the laid-out codes.
+__global__ __launch_bounds__(256) void linear4_layout_kernel(const uint8_t* __restrict__ codes,
+                                                             const uint16_t* __restrict__ scales, int64_t n,
+                                                             int64_t k, int group, uint32_t* __restrict__ out_codes,
+                                                             uint16_t* __restrict__ out_scales) {
+  const int64_t tiles_k = (k + 127) / 128, words = linear4_tiles(n, k) * 256;
+  const int per_tile = 128 / group;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t tile = i / 256;
+    const int lane = (int)(i % 256) / 4, c = (int)(i % 4);
+    const int64_t row = tile / tiles_k * 16 + lane % 16, col = tile % tiles_k * 128 + 32 * c + 8 * (lane / 16);
+    uint32_t w = 0;
+    if (row < n && col < k) {
+      const uint32_t src = *reinterpret_cast<const uint32_t*>(codes + row * (k / 2) + col / 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w |= ((src >> (4 * j)) & 15u) << (4 * (j / 2) + 16 * (j & 1));
+    }
+    out_codes[i] = w << 3 | w >> 29;
+    const int g = (int)(i % 256);
+    if (g < 16 * per_tile) {  // [4][per_tile][4 rows]
+      const int64_t srow = tile / tiles_k * 16 + g / (4 * per_tile) * 4 + g % 4;
+      const int64_t at = tile % tiles_k * per_tile + g / 4 % per_tile;
+      out_scales[tile * 16 * per_tile + g] = srow < n && at < k / group ? scales[srow * (k / group) + at] : 0;
+    }
+  }
+}
+
+template <Kv4Type T>
+struct Operand {
+  typedef v8b type;
+  static constexpr int kParts = 1;
+};
+template <>
+struct Operand<kKv4F16> {
+  typedef v8h type;
+  static constexpr int kParts = 1;
+};
+template <>
+struct Operand<kKv4F32> {
+  typedef v8b type;
+  static constexpr int kParts = 3;
+};
+
+template <Kv4Type T>
+__device__ __forceinline__ typename Operand<T>::type decode(uint32_t w) {
+  const uint32_t p[4] = {w, w >> 4, w >> 8, __builtin_amdgcn_alignbit(w, w, 12)};
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = T == kKv4F16 ? pair_f16(p[i]) : (T == kKv4BF16 ? pair_bf16_24(p[i]) : pair_bf16(p[i]));
+  return __builtin_bit_cast(typename Operand<T>::type, r);
+}
+
+// Eight elements of a row of x as they lie in memory (p NULL: zeros).
+template <int kWords>
+__device__ __forceinline__ void load_x(const void* p, bool wide, uint32_t (&x)[kWords]) {
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) x[i] = 0;
+  if (p == nullptr) return;
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) {
+      const v4u a = static_cast<const v4u*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = a[j];
+    }
+  } else if constexpr (kWords == 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<const uint32_t*>(p)[i];
+  } else {
+    const uint16_t* src = static_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = src[2 * i] | (uint32_t)src[2 * i + 1] << 16;
+  }
+}
+
+// The same as MFMA operands.
+template <Kv4Type T, int kWords>
+__device__ __forceinline__ void operands(const uint32_t (&u)[kWords],
+                                         typename Operand<T>::type (&x)[Operand<T>::kParts]) {
+  if constexpr (T == kKv4F32) {
+    split3(u, x);
+  } else {
+    x[0] = __builtin_bit_cast(typename Operand<T>::type, (v4u){u[0], u[1], u[2], u[3]});
+  }
+}
+
+template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
+struct LinearTile {
+  v4u codes[kRowTiles];
+  uint32_t scales[kRowTiles][kGroups * 2];  // [group][4 rows], bfloat16
+  uint32_t x[4][kCols][T == kKv4F32 ? 8 : 4];
+};
+
+template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
+__global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const void* __restrict__ x, int64_t rows,
+                                                       int64_t x_row_stride, bool wide, void* __restrict__ out,
+                                                       int64_t out_row_stride) {
+  typedef LinearTile<T, kGroups, kCols, kRowTiles> Tile;
+  constexpr int kParts = Operand<T>::kParts;
+  constexpr int kSize = T == kKv4F32 ? 4 : 2;
+  extern __shared__ float s_acc[];
+  const int lane = lane_id(), col = lane % 16, g = lane / 16;
+  const int wave = wave_uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
+  const int tiles_k = (w.k + 127) / 128, tiles_n = (w.n + 15) / 16;
+  const int n0 = blockIdx.x * kRowTiles;
+  const int64_t m0 = (int64_t)blockIdx.y * 16 * kCols;
+
+  auto load = [&](int kt, Tile& t) {
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r) {
+      const int64_t tile = (int64_t)min(n0 + r, tiles_n - 1) * tiles_k + kt;
+      t.codes[r] = reinterpret_cast<const v4u*>(w.codes)[tile * kWave + lane];
+      const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + (tile * 4 + g) * kGroups * 2;
+#pragma unroll
+      for (int i = 0; i < kGroups * 2; ++i) t.scales[r][i] = s[i];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = kt * 128 + 32 * c + 8 * g;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        const int64_t m = m0 + 16 * j + col;
+        const bool have = m < rows && k < w.k;
+        load_x(have ? static_cast<const char*>(x) + (m * x_row_stride + k) * kSize : nullptr, wide, t.x[c][j]);
+      }
+    }
+  };
+
+  v4f acc[kRowTiles][kCols];
+#pragma unroll
+  for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) acc[r][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+
+  int kt = wave;
+  Tile tile;
+  if (kt < tiles_k) load(kt, tile);
+  for (; kt < tiles_k; kt += waves) {
+    Tile next;
+    if (kt + waves < tiles_k) load(kt + waves, next);
+    typename Operand<T>::type b[4][kCols][kParts];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) operands<T>(tile.x[c][j], b[c][j]);
+    v4f start[kGroups][kCols];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        start[i][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (T == kKv4BF16) {
+          const v4u offset = {0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u};  // -24
+#pragma unroll
+          for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c)
+            start[i][j] = mfma(__builtin_bit_cast(v8b, offset), b[c][j][0], start[i][j]);
+        }
+      }
+    v4f sum[kRowTiles][kGroups][kCols];
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) sum[r][i][j] = start[i][j];
+#pragma unroll
+        for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c) {
+          const typename Operand<T>::type a = decode<T>(tile.codes[r][c]);
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) sum[r][i][j] = mfma(a, b[c][j][p], sum[r][i][j]);
+        }
+      }
+    mfma_results_fence();
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t s2 = tile.scales[r][i * 2 + e / 2];
+          const float s = __uint_as_float(e & 1 ? s2 & 0xFFFF0000u : s2 << 16);
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) acc[r][j][e] = __builtin_fmaf(s, sum[r][i][j][e], acc[r][j][e]);
+        }
+    tile = next;
+  }
+
+  // [wave][row tile][column tile][element][lane]
+  constexpr int kPerWave = kRowTiles * kCols * 4 * kWave;
+#pragma unroll
+  for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s_acc[wave * kPerWave + ((r * kCols + j) * 4 + e) * kWave + lane] = acc[r][j][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kPerWave; i += blockDim.x) {
+    const int n_in = i % (16 * kRowTiles), m_in = i / (16 * kRowTiles);
+    const int r = n_in / 16, e = n_in % 4, l = n_in % 16 / 4 * 16 + m_in % 16, j = m_in / 16;
+    const int n = n0 * 16 + n_in;
+    const int64_t m = m0 + m_in;
+    if (n >= w.n || m >= rows) continue;
+    float y = 0.0f;
+    for (int v = 0; v < waves; ++v) y += s_acc[v * kPerWave + ((r * kCols + j) * 4 + e) * kWave + l];
+    if (w.bias != nullptr) y += w.bias[n];
+    const int64_t at = m * out_row_stride + n;
+    if constexpr (T == kKv4F32) static_cast<float*>(out)[at] = y;
+    if constexpr (T == kKv4F16) static_cast<_Float16*>(out)[at] = (_Float16)y;
+    if constexpr (T == kKv4BF16) static_cast<__bf16*>(out)[at] = (__bf16)y;
+  }
+}
+
+template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
+hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
+                        int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  const int size = T == kKv4F32 ? 4 : 2;
+  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_row_stride * size % 16 == 0;
+  const int64_t gx = ((w.n + 15) / 16 + kRowTiles - 1) / kRowTiles, gy = (rows + 16 * kCols - 1) / (16 * kCols);
+  if (gy > 65535) return hipErrorInvalidValue;
+  // Enough waves for the CUs' latency, within the tiles there are and the LDS
+  // that joins them.
+  const int tiles_k = (w.k + 127) / 128;
+  int waves = 4;
+  while (waves < 8 && waves * 2 <= tiles_k && waves * 2 * kRowTiles * kCols <= 32 && gx * gy * waves < num_cus * 8)
+    waves *= 2;
+  const size_t lds = sizeof(float) * waves * kRowTiles * kCols * 4 * kWave;
+  linear4_kernel<T, kGroups, kCols, kRowTiles><<<dim3((unsigned)gx, (unsigned)gy), dim3(waves * kWave), lds, stream>>>(
+      w, x, rows, x_row_stride, wide, out, out_row_stride);
+  return hipGetLastError();
+}
+
+template <Kv4Type T, int kGroups>
+hipError_t launch_group(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
+                        int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  if (rows <= 4) return launch_shape<T, kGroups, 1, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  if (rows <= 16) return launch_shape<T, kGroups, 1, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  // Two column tiles of single precision parts leave registers for one row tile.
+  constexpr int kRowTiles = T == kKv4F32 ? 1 : 2;
+  return launch_shape<T, kGroups, 2, kRowTiles>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+}
+
+template <Kv4Type T>
+hipError_t launch_type(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
+                       int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  switch (w.group) {
+    case 32: return launch_group<T, 4>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+    case 64: return launch_group<T, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+    case 128: return launch_group<T, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_linear4_layout(const uint8_t* codes, const uint16_t* scales, int64_t n, int64_t k, int group,
+                                 uint8_t* out_codes, uint16_t* out_scales, hipStream_t stream) {
+  const int64_t words = linear4_tiles(n, k) * 256;
+  const int64_t blocks = std::min<int64_t>((words + 255) / 256, 65536);
+  if (blocks <= 0) return hipSuccess;
+  linear4_layout_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
+      codes, scales, n, k, group, reinterpret_cast<uint32_t*>(out_codes), out_scales);
+  return hipGetLastError();
+}
+
+hipError_t launch_linear4(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, Kv4Type type,
+                          void* out, int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  if (rows <= 0) return hipSuccess;
+  switch (type) {
+    case kKv4F32: return launch_type<kKv4F32>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+    case kKv4F16: return launch_type<kKv4F16>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+    case kKv4BF16: return launch_type<kKv4BF16>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace msim
