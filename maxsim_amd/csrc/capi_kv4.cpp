@@ -64,9 +64,10 @@ void check_rows(const void* p, Kv4Type type, const char* what) {
   if (!aligned(p, type == kKv4F32 ? 4 : 2)) throw InvalidArgument(std::string(what) + " must be aligned to its type");
 }
 
-void check_heads(const Kv4Pool& pool, int64_t heads) {
+void check_heads(const Kv4Pool& pool, const Kv4Batch& batch, int64_t heads) {
   if (heads < 1 || heads % pool.kv_heads != 0) throw InvalidArgument("heads must be a multiple of kv_heads");
-  if (heads > 16384) throw NotSupported("at most 16384 heads");
+  if (heads > 16384 || ((int64_t)batch.rows + batch.batch) * heads >= int64_t{1} << 30)
+    throw NotSupported("at most 16384 heads, and less than 2^30 of (rows + batch) * heads");
 }
 
 int rows_call(const msim_kv4_pool* pool, const int32_t* table, const int32_t* lengths, const int32_t* offsets,
@@ -110,7 +111,7 @@ extern "C" int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batc
     const Kv4Pool p = check_pool(pool);
     static const int32_t present = 0;  // only the sizes count here
     const Kv4Batch b = check_batch(p, &present, &present, &present, batch, max_pages, rows);
-    check_heads(p, heads);
+    check_heads(p, b, heads);
     *bytes = kv4_attend_workspace(p, b, (int)heads, device_cu_count());
   });
 }
@@ -126,7 +127,7 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     const Kv4Pool p = check_pool(pool);
     const Kv4Batch b = check_batch(p, page_table, lengths, offsets, batch, max_pages, rows);
     const Kv4Type t = check_type(type);
-    check_heads(p, heads);
+    check_heads(p, b, heads);
     if (!std::isfinite(scale)) throw InvalidArgument("scale must be finite");
     if (window < 0) throw InvalidArgument("window must not be negative");
     if (mask != nullptr && mask_width < 0) throw InvalidArgument("mask width must not be negative");
@@ -147,6 +148,9 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     a.mask = mask;
     a.mask_row_stride = mask_row_stride;
     a.mask_width = mask_width;
+    const int64_t size = t == kKv4F32 ? 4 : 2;
+    a.q_wide = aligned(q, 16) && q_row_stride * size % 16 == 0 && q_head_stride * size % 16 == 0;
+    a.out_wide = aligned(out, 4 * size) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0;
     a.heads = (int32_t)heads;
     a.causal = causal != 0;
     a.window = window == 0 || window > INT_MAX ? INT_MAX : (int32_t)window;

@@ -82,6 +82,16 @@ __device__ __forceinline__ void lds_load_b32(v4i rsrc, uint32_t byte_offset, uin
       : "memory");
 }
 
+// The same from a 64-bit address of each lane's own, 4 bytes per lane.
+__device__ __forceinline__ void lds_load_b32_global(const void* address, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, off\n\ts_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds), "v"(address)
+      : "memory");
+}
+
 // The same with a wave-uniform byte offset (soffset) added to every lane's
 // voffset.  The buffer range check covers voffset only: the caller keeps
 // soffset + voffset inside the buffer.

@@ -45,14 +45,14 @@ struct Kv4Rows {  // rows of keys or values in a program's memory
 
 __device__ __forceinline__ int kv4_length(const Kv4Pool& pool, const Kv4Batch& batch, int b) {
   const int64_t most = (int64_t)batch.max_pages << pool.page_shift;
-  const int n = batch.lengths[b];
+  const int n = as_constant(batch.lengths)[b];
   return n < 0 ? 0 : ((int64_t)n > most ? (int)most : n);
 }
 
 // First row of sequence b (b up to batch): never past the row count.
 __device__ __forceinline__ int kv4_first_row(const Kv4Batch& batch, int b) {
   if (batch.offsets == nullptr) return min(b, batch.rows);
-  const int v = batch.offsets[b];
+  const int v = as_constant(batch.offsets)[b];
   return v < 0 ? 0 : min(v, batch.rows);
 }
 
@@ -120,6 +120,7 @@ struct Kv4AttendArgs {
   const uint8_t* mask;  // [rows, mask_width] or nullptr; 0 hides a key
   int64_t mask_row_stride;
   int64_t mask_width;
+  int32_t q_wide, out_wide;  // rows of every head start on 16 bytes (out: on 4 elements)
   int32_t heads;
   int32_t causal;
   int32_t window;  // keys at p - window + 1 .. p; INT32_MAX: all

@@ -41,7 +41,21 @@ namespace {
 
 constexpr int kTileKeys = 32;
 constexpr int kWaves = 4;
-constexpr int kMinChunk = 256;  // keys of a split, at least
+#ifndef MSIM_KV4_STAGES
+#define MSIM_KV4_STAGES 3
+#endif
+
+// Rings of tiles, and in their place the join of the waves.
+constexpr int attend_lds(int dim, int cols) {
+  const int rings = kWaves * (dim <= 128 ? MSIM_KV4_STAGES : 2) * (32 * dim + 256);
+  const int join = 16 * cols * 4 * kWaves * (2 + dim + 4);
+  return rings > join ? rings : join;
+}
+
+// Workgroups of 4 waves that a CU holds by their registers.
+constexpr int waves_per_simd(Kv4Type type, int dim, int cols) {
+  return type == kKv4F32 || dim > 128 || cols > 1 ? (dim > 192 || (type == kKv4F32 && dim * cols > 192) ? 1 : 2) : 3;
+}
 constexpr float kUnset = -FLT_MAX;
 // A row's reference moves when a product passes 2^15 or a probability 2^100, to
 // where the largest are 2^13 and 2^90.
@@ -51,126 +65,124 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 
 // --------------------------------------------------------------- the split
 //
-// A unit of work is (sequence, tile of query rows, chunk of keys, head).  The
-// chunk length follows from the work there is: all (row tile, key) pairs,
-// shared evenly among `target` units.
-struct Split {
-  int chunk;  // keys
-  int seq, first_row, rows, length, low;
-  int tile, part, parts;
-  int slot;  // of the unit's partial result, if parts > 1
-};
+// An item is (sequence, tile of query rows, key/value head), a granule 128 of
+// its keys.  All granules, in the order of items, are dealt out evenly: worker
+// i of n has those from i G / n to (i + 1) G / n, whatever items they belong to.
+// An item that lies within one worker is finished there; of the others each
+// worker leaves a partial result, in its slot 1 if the item begins there, in
+// slot 0 if it came in from the worker before (it has at most one of each).
+//
+// Where no sequence can be longer than kShort keys a granule is kShort: no item
+// is split, and the call is one launch.
+constexpr int kGranule = kWaves * kTileKeys;
+constexpr int kShort = 4 * kGranule;
 
-struct SplitShape {
-  int share;   // query heads per key/value head
-  int tile_rows;
-  int target;  // units, about
-  int slots;
+//
+// Granules, items and rows are counted in 32 bits: the host refuses calls of 2^30
+// rows times heads and doubles the granule where their number could pass 2^31.
+struct Split {
+  uint32_t share;       // query heads per key/value head
+  uint32_t tile_shift;  // log2(query rows of a tile)
+  uint32_t workers;     // at most
+  uint32_t granule_shift;
+  uint32_t least;       // granules of a worker, where that leaves more than one
+  uint32_t one_launch;  // no item is split
 };
 
 struct SeqWork {
-  int first, rows, length, low, tiles;
+  int first, rows, length, low;
+  uint32_t tiles;
+  uint32_t granules;  // of one item
 };
 
 __device__ __forceinline__ SeqWork seq_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                            const SplitShape& shape, int b) {
+                                            const Split& split, int b) {
   SeqWork w;
   w.first = kv4_first_row(batch, b);
   w.rows = max(0, kv4_first_row(batch, b + 1) - w.first);
   w.length = kv4_length(pool, batch, b);
-  const int64_t low = (int64_t)w.length - w.rows - args.window + 1;  // of the first row
-  w.low = low > 0 ? (int)min(low, (int64_t)w.length) / kTileKeys * kTileKeys : 0;
-  w.tiles = (int)(((int64_t)w.rows * shape.share + shape.tile_rows - 1) / shape.tile_rows);
+  // The first key that the first row sees, if it sees the last ones only.
+  const int start = w.length - w.rows;
+  w.low = start >= args.window ? (start - args.window + 1) / kTileKeys * kTileKeys : 0;
+  w.tiles = ((uint32_t)w.rows * split.share + (1u << split.tile_shift) - 1) >> split.tile_shift;
+  w.granules = max(1u, ((uint32_t)(w.length - w.low) + (1u << split.granule_shift) - 1) >> split.granule_shift);
   return w;
 }
 
-__device__ __forceinline__ int parts_of(const SeqWork& w, int chunk) {
-  return max(1, (int)(((int64_t)w.length - w.low + chunk - 1) / chunk));
+// A sequence that is the whole wave's.
+__device__ __forceinline__ SeqWork uniform_seq_work(const Kv4Pool& pool, const Kv4Batch& batch,
+                                                    const Kv4AttendArgs& args, const Split& split, int b) {
+  SeqWork w = seq_work(pool, batch, args, split, b);
+  w.first = wave_uniform(w.first);
+  w.rows = wave_uniform(w.rows);
+  w.length = wave_uniform(w.length);
+  w.low = wave_uniform(w.low);
+  w.tiles = wave_uniform(w.tiles);
+  w.granules = wave_uniform(w.granules);
+  return w;
 }
 
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T* lds) {
-#pragma unroll
-  for (int i = 1; i < kWave; i *= 2) v += __shfl_xor(v, i);
-  if (lane_id() == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  T sum = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) sum += lds[i];
-  __syncthreads();
-  return sum;
+// Inclusive sums over the lanes (DPP row shifts, then the rows' last lanes).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  typedef std::integral_constant<int, 0xF> All;
+  add(std::integral_constant<int, 0x111>{}, All{});
+  add(std::integral_constant<int, 0x112>{}, All{});
+  add(std::integral_constant<int, 0x114>{}, All{});
+  add(std::integral_constant<int, 0x118>{}, All{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+  return v;
 }
 
-// The workgroup's unit: the one numbered `unit`, or (unit < 0) sequence `seq`
-// with the slot of its first partial result.  False past the last unit.
-__device__ __forceinline__ bool find_split(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                           const SplitShape& shape, int64_t unit, int seq, Split& out) {
-  __shared__ int64_t s_sum[kWaves];
-  __shared__ int64_t s_scan[kWaves][2];
-  __shared__ int s_found[2];
-  int64_t pairs = 0;
-  for (int b = threadIdx.x; b < batch.batch; b += blockDim.x) {
-    const SeqWork w = seq_work(pool, batch, args, shape, b);
-    pairs += (int64_t)w.tiles * (w.length - w.low);
+// `total` granules among `workers`: the first `extra` have one more.
+struct Deal {
+  uint32_t total, workers, each, extra;
+  __device__ uint32_t begin(uint32_t i) const { return i * each + min(i, extra); }
+  __device__ uint32_t worker_of(uint32_t granule) const {
+    const uint32_t longer = extra * (each + 1);
+    return min(workers - 1, granule < longer ? granule / (each + 1) : extra + (granule - longer) / each);
   }
-  pairs = block_sum(pairs, s_sum);
-  const int64_t even = (pairs * pool.kv_heads + shape.target - 1) / shape.target;
-  out.chunk = (int)min((int64_t)1 << 30, (max((int64_t)kMinChunk, even) + 127) / 128 * 128);
-  if (threadIdx.x == 0) s_found[0] = -1;
-  int64_t units = 0, slots = 0;  // before this pass's sequences
-  __syncthreads();
-  int64_t at = -1, slot_at = 0;
-  for (int b0 = 0; b0 < batch.batch; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    int64_t mine = 0, mine_slots = 0;
-    if (b < batch.batch) {
-      const SeqWork w = seq_work(pool, batch, args, shape, b);
-      const int parts = parts_of(w, out.chunk);
-      mine = (int64_t)w.tiles * parts;
-      mine_slots = parts > 1 ? mine : 0;
+};
+
+// By a wave together: the deal, and the sequence that holds the first granule
+// of worker `worker` (or, worker < 0, sequence `seq`) with the granules before
+// it.  False if the worker has none.
+__device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
+                                          const Split& split, int worker, int& seq, uint32_t& before, Deal& deal) {
+  const int lane = lane_id();
+  auto granules = [&](int b) -> uint32_t {
+    if (b >= batch.batch) return 0;
+    const SeqWork w = seq_work(pool, batch, args, split, b);
+    return w.tiles * pool.kv_heads * w.granules;
+  };
+  const uint32_t head = granules(lane);
+  uint32_t total = head;
+  for (int b0 = kWave; b0 < batch.batch; b0 += kWave) total += granules(b0 + lane);
+  const uint32_t head_scan = wave_scan(head);
+  deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
+                                    : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
+  deal.workers = min(split.workers, max(1u, deal.total / split.least));
+  deal.each = deal.total / deal.workers;
+  deal.extra = deal.total - deal.each * deal.workers;
+  if (deal.total == 0 || worker >= (int)deal.workers) return false;
+  const uint32_t target = worker >= 0 ? deal.begin(worker) : 0;
+  uint32_t done = 0;
+  for (int b0 = 0; b0 < batch.batch; b0 += kWave) {
+    const uint32_t mine = b0 == 0 ? head : granules(b0 + lane);
+    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine)), first = upto - mine;
+    const uint64_t here = __ballot(worker >= 0 ? first <= target && target < upto : b0 + lane == seq);
+    if (here != 0) {
+      const int at = __builtin_ctzll(here);
+      seq = wave_uniform(b0 + at);
+      before = __builtin_amdgcn_readlane(first, at);
+      return true;
     }
-    int64_t sum = mine, sum_slots = mine_slots;
-#pragma unroll
-    for (int i = 1; i < kWave; i *= 2) {
-      const int64_t u = __shfl_up(sum, i), s = __shfl_up(sum_slots, i);
-      if (lane_id() >= i) sum += u, sum_slots += s;
-    }
-    if (lane_id() == kWave - 1) s_scan[threadIdx.x / kWave][0] = sum, s_scan[threadIdx.x / kWave][1] = sum_slots;
-    __syncthreads();
-    int64_t before = units, before_slots = slots;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const int64_t u = s_scan[i][0], s = s_scan[i][1];
-      if (i < (int)threadIdx.x / kWave) before += u, before_slots += s;
-      units += u, slots += s;
-    }
-    const int64_t first = before + sum - mine;
-    const bool here = b < batch.batch && (unit >= 0 ? first <= unit && unit < first + mine : b == seq);
-    if (here) {
-      s_found[0] = b;
-      s_sum[0] = unit >= 0 ? unit - first : 0;
-      s_sum[1] = before_slots + sum_slots - mine_slots;
-    }
-    __syncthreads();
-    if (s_found[0] >= 0) {
-      at = s_sum[0], slot_at = s_sum[1];
-      break;
-    }
+    done = __builtin_amdgcn_readlane(upto, kWave - 1);
   }
-  const int b = wave_uniform(s_found[0]);
-  if (b < 0) return false;
-  const SeqWork w = seq_work(pool, batch, args, shape, b);
-  out.seq = b;
-  out.first_row = wave_uniform(w.first);
-  out.rows = wave_uniform(w.rows);
-  out.length = wave_uniform(w.length);
-  out.low = wave_uniform(w.low);
-  out.parts = wave_uniform(parts_of(w, out.chunk));
-  const int local = wave_uniform((int)at);
-  out.tile = local / out.parts;
-  out.part = local % out.parts;
-  out.slot = wave_uniform((int)slot_at) + local;
-  return true;
+  return false;
 }
 
 // ------------------------------------------------------------ the main kernel
@@ -183,12 +195,18 @@ struct Shape {
   static constexpr int kTiles = kValueDims;                 // 16-dim tiles of the output
 };
 
+// A tile as it lies in LDS: [keys, values][half][16 rows], then the scales
+// [keys, values][half][16].  Rows of a half are kept in the order 0, 4, 8, 12, 1,
+// 5, ... so that the four rows that a value read of a wave touches are adjacent
+// (no bank conflicts).
 template <int kDim>
-struct Tile {
-  uint32_t key[2][kDim / 32];                                  // [half][word]
-  uint32_t value[2][4][Shape<kDim>::kValueDims > 8 ? 2 : 1];   // [half][key][word]
-  v4f key_scale[2], value_scale[2];
-  bool hole[2];
+struct TileLds {
+  static constexpr int kHalf = 8 * kDim;
+  static constexpr int kScales = 4 * kHalf;
+  static constexpr int kBytes = kScales + 256;
+  static constexpr int kHalfLoads = (kHalf + 1023) / 1024;
+  static constexpr int kLoads = 4 * kHalfLoads + 1;  // of a wave, per tile
+  static constexpr int kStages = kDim <= 128 ? MSIM_KV4_STAGES : 2;
 };
 
 // Eight codes of a word as bfloat16, in the order of decode_word.
@@ -211,11 +229,35 @@ __device__ __forceinline__ v8h decode_word(uint32_t w) {
 // The order of a word's codes in decode_word's result.
 __device__ __forceinline__ constexpr int word_order(int i) { return (i & 1) * 4 + i / 2; }
 
+// Eight elements of a query from element i on (16-byte loads if `wide`).
 template <Kv4Type T>
-__device__ __forceinline__ float load_query(const void* q, int64_t i) {
-  if constexpr (T == kKv4F32) return static_cast<const float*>(q)[i];
-  if constexpr (T == kKv4F16) return (float)static_cast<const _Float16*>(q)[i];
-  return __uint_as_float((uint32_t) static_cast<const uint16_t*>(q)[i] << 16);
+__device__ __forceinline__ void load8(const void* q, int64_t i, bool wide, float (&x)[8]) {
+  if constexpr (T == kKv4F32) {
+    const float* p = static_cast<const float*>(q) + i;
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const v4f v = reinterpret_cast<const v4f*>(p)[k];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * k + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = p[j];
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(q) + i;
+    uint16_t h[8];
+    if (wide) {
+      __builtin_memcpy(h, __builtin_assume_aligned(p, 16), 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = T == kKv4BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
+  }
 }
 
 template <Kv4Type T>
@@ -225,38 +267,63 @@ __device__ __forceinline__ void store_out(void* out, int64_t i, float x) {
   if constexpr (T == kKv4BF16) static_cast<__bf16*>(out)[i] = (__bf16)x;
 }
 
-template <int kDim>
-__device__ __forceinline__ void load_tile(const Kv4Pool& pool, const Kv4Batch& batch, int seq, int length, int head,
-                                          int key0, Tile<kDim>& t) {
-  typedef Shape<kDim> S;
-  const int lane = lane_id(), col = lane % 16, g = lane / 16;
+// Four elements of an output row (one store if `wide`).
+template <Kv4Type T>
+__device__ __forceinline__ void store4(void* out, int64_t i, bool wide, v4f x) {
+  if (!wide) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) store_out<T>(out, i + k, x[k]);
+  } else if constexpr (T == kKv4F32) {
+    *reinterpret_cast<v4f*>(static_cast<float*>(out) + i) = x;
+  } else {
+    typedef typename std::conditional<T == kKv4F16, _Float16, __bf16>::type E;
+    typedef E v4e __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4e*>(static_cast<E*>(out) + i) = (v4e){(E)x[0], (E)x[1], (E)x[2], (E)x[3]};
+  }
+}
+
+// Page numbers of a tile's halves (pages hold 16 rows or a multiple, so a half
+// lies in one page); -1 past the sequence's end.
+struct TilePages {
+  int page[2];
+};
+__device__ __forceinline__ TilePages tile_pages(const Kv4Pool& pool, const Kv4Batch& batch, int seq, int length, int key0) {
+  TilePages p;
+  const auto* table = as_constant(batch.table) + (int64_t)seq * batch.max_pages;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    // Pages hold 16 rows or a multiple, so a half lies in one page.
     const int key = key0 + 16 * h;
-    int page = key < length ? as_constant(batch.table)[(int64_t)seq * batch.max_pages + (key >> pool.page_shift)] : -1;
-    t.hole[h] = (uint32_t)page >= (uint32_t)pool.num_pages;
-    if (t.hole[h]) page = 0;
-    const int64_t at = kv4_pool_row(pool, page, head, key & ((1 << pool.page_shift) - 1));
-    const uint8_t* keys = pool.codes[0] + at * (kDim / 2);
-    const uint8_t* values = pool.codes[1] + at * (kDim / 2);
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(keys + col * (kDim / 2) + g * (kDim / 8));
+    p.page[h] = key < length ? table[key >> pool.page_shift] : -1;
+  }
+  return p;
+}
+
+// Starts a tile's way to LDS (kLoads loads); holes come from page 0.
+template <int kDim>
+__device__ __forceinline__ void load_tile(const Kv4Pool& pool, const TilePages& pages, int head, int key0,
+                                          uint32_t lds) {
+  typedef TileLds<kDim> L;
+  constexpr int kChunks = kDim / 32;  // of 16 bytes in a row
+  const int lane = lane_id();
+  int64_t at[2];
 #pragma unroll
-    for (int i = 0; i < S::kKeyWords; ++i) t.key[h][i] = kw[i];
-    const int vl = S::kValueLanes == 16 ? col : min(col, S::kValueLanes - 1);
+  for (int h = 0; h < 2; ++h) {
+    const int page = (uint32_t)pages.page[h] < (uint32_t)pool.num_pages ? pages.page[h] : 0;
+    at[h] = kv4_pool_row(pool, page, head, (key0 + 16 * h) & ((1 << pool.page_shift) - 1));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint8_t* row = values + (4 * g + r) * (kDim / 2) + vl * (S::kValueDims / 2);
-      if constexpr (S::kValueDims == 4) {
-        t.value[h][r][0] = *reinterpret_cast<const uint16_t*>(row);
-      } else {
+    for (int side = 0; side < 2; ++side) {
+      const v4i rsrc = make_rsrc_words(pool.codes[side] + at[h] * (kDim / 2), L::kHalf);
 #pragma unroll
-        for (int i = 0; i < S::kValueDims / 8; ++i) t.value[h][r][i] = reinterpret_cast<const uint32_t*>(row)[i];
+      for (int i = 0; i < L::kHalfLoads; ++i) {
+        const int chunk = i * kWave + lane, place = chunk / kChunks;
+        const int row = place % 4 * 4 + place / 4;
+        if (L::kHalf % 1024 == 0 || chunk < L::kHalf / 16)
+          lds_load_b128(rsrc, row * (kDim / 2) + chunk % kChunks * 16, lds + (side * 2 + h) * L::kHalf + i * 1024);
       }
     }
-    t.key_scale[h] = *reinterpret_cast<const v4f*>(pool.scales[0] + at + 4 * g);
-    t.value_scale[h] = *reinterpret_cast<const v4f*>(pool.scales[1] + at + 4 * g);
   }
+  const float* scales = lane & 32 ? pool.scales[1] : pool.scales[0];
+  lds_load_b32_global(scales + (lane & 16 ? at[1] : at[0]) + lane % 16, lds + L::kScales);
 }
 
 __device__ __forceinline__ float across_groups_max(float v) {
@@ -268,37 +335,19 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// kCols 16-row column tiles of queries per workgroup; its waves take the key
-// tiles in turn.
+// Granules from .. upto of an item.  kCols 16-row column tiles of queries per
+// workgroup; its waves take the key tiles in turn.
 template <Kv4Type T, int kDim, int kCols>
-__global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
-                                                                   SplitShape shape, float* __restrict__ partial) {
+__device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
+                                            const Split& split, float* __restrict__ partial, const SeqWork& u,
+                                            int seq, uint32_t tile, int head, uint32_t from, uint32_t upto) {
   typedef Shape<kDim> S;
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
   constexpr int kProbParts = T == kKv4F32 ? 3 : 1;  // of a probability
   typedef typename std::conditional<T == kKv4F32, v8b, v8h>::type Prob;
   constexpr int kRows = 16 * kCols;
-  extern __shared__ char s_raw[];
+  __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols)];
   const int lane = lane_id(), col = lane % 16, g = lane / 16, wave = wave_uniform(threadIdx.x / kWave);
-  const int head = blockIdx.x % pool.kv_heads;
-  Split u;
-  if (!find_split(pool, batch, args, shape, blockIdx.x / pool.kv_heads, 0, u)) {
-    // Past the last unit, as the last workgroup always is: rows of no sequence
-    // come out as rows that see nothing.
-    if (blockIdx.x == gridDim.x - 1 && batch.offsets != nullptr) {
-      const int first = kv4_first_row(batch, 0), last = kv4_first_row(batch, batch.batch);
-      for (int row = 0; row < batch.rows; ++row) {
-        if (row >= first && row < last) row = last;
-        if (row >= batch.rows) break;
-        for (int i = threadIdx.x; i < args.heads * kDim; i += blockDim.x)
-          store_out<T>(args.out, row * args.out_row_stride + i / kDim * args.out_head_stride + i % kDim, 0.0f);
-        for (int h = threadIdx.x; h < args.heads && args.lse != nullptr; h += blockDim.x)
-          args.lse[(int64_t)row * args.heads + h] = kNegInf;
-      }
-    }
-    return;
-  }
-
   // Query rows of this tile: row r is new token r / share, head r % share.
   v8h q[kCols][kParts][S::kKeyWords];
   float factor[kCols];       // of a product with the codes, towards log2 scores
@@ -307,21 +356,24 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
   int all_low = 0, all_high = INT_MAX, any_low = INT_MAX, any_high = 0;
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
-    const int64_t r = (int64_t)u.tile * kRows + 16 * c + col;
-    const int token = (int)(r / shape.share), sub = (int)(r % shape.share);
+    const uint32_t r = tile * kRows + 16 * c + col;
+    const int token = (int)(r / split.share), sub = (int)(r - token * split.share);
     const bool have = token < u.rows;
-    const int64_t base = have ? (int64_t)(u.first_row + token) * args.q_row_stride +
-                                    (int64_t)(head * shape.share + sub) * args.q_head_stride
+    const int64_t base = have ? (int64_t)(u.first + token) * args.q_row_stride +
+                                    (int64_t)(head * split.share + sub) * args.q_head_stride
                               : 0;
     float x[S::kKeyWords][8];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < S::kKeyWords; ++i)
+    for (int i = 0; i < S::kKeyWords; ++i) {
+      float y[8];
+      load8<T>(args.q, have ? base + g * (kDim / 4) + i * 8 : 0, args.q_wide != 0, y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        x[i][j] = have ? load_query<T>(args.q, base + g * (kDim / 4) + i * 8 + word_order(j)) : 0.0f;
+        x[i][j] = have ? y[word_order(j)] : 0.0f;
         top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
       }
+    }
     top = max(top, (uint32_t)__shfl_xor((int)top, 16));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
     const int shift = 141 - (int)(top >> 23);  // the largest to [2^14, 2^15)
@@ -336,13 +388,12 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
       }
     factor[c] = ldexpf(args.scale_log2, -shift);
     const int pos = u.length - u.rows + token;
-    const int64_t low = (int64_t)pos - args.window + 1;
-    see_low[c] = low > 0 ? (int)low : 0;
+    see_low[c] = pos >= args.window ? pos - args.window + 1 : 0;
     see_high[c] = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
     mask[c] = nullptr;
     if (args.mask != nullptr) {
       see_high[c] = (int)min((int64_t)see_high[c], args.mask_width);
-      mask[c] = args.mask + (have ? (int64_t)(u.first_row + token) * args.mask_row_stride : 0);
+      mask[c] = args.mask + (have ? (int64_t)(u.first + token) * args.mask_row_stride : 0);
     }
     if (!have) {  // a row of padding: nothing depends on what it sees
       see_low[c] = 0;
@@ -358,10 +409,9 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
   all_high = wave_reduce(all_high, [](int a, int b) { return min(a, b); });
   any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
   any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
-  // Keys of this unit: its chunk, cut to what some row sees.
-  const int64_t chunk_low = u.low + (int64_t)u.part * u.chunk;
-  int begin = (int)max(chunk_low, (int64_t)min(any_low, u.length) / kTileKeys * kTileKeys);
-  const int end = (int)min(chunk_low + u.chunk, (int64_t)any_high);
+  // This worker's keys of the item, cut to what some row sees.
+  const int begin = max(u.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
+  const int end = (int)min((int64_t)u.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
 
   float ref[kCols], sum[kCols];
   v4f o[kCols][S::kTiles];
@@ -373,41 +423,90 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
     for (int t = 0; t < S::kTiles; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  int key0 = begin + wave * kTileKeys;
-  Tile<kDim> tile;
-  if (key0 < end) load_tile<kDim>(pool, batch, u.seq, u.length, head, key0, tile);
-  for (; key0 < end; key0 += kWaves * kTileKeys) {
-    Tile<kDim> next;
-    if (key0 + kWaves * kTileKeys < end)
-      load_tile<kDim>(pool, batch, u.seq, u.length, head, key0 + kWaves * kTileKeys, next);
+  // A ring of tiles per wave: kStages - 1 of them on their way while one is
+  // worked on.
+  typedef TileLds<kDim> L;
+  constexpr int kStep = kWaves * kTileKeys, kAhead = L::kStages - 1;
+  const int key_first = begin + wave * kTileKeys;
+  const int tiles = end > key_first ? (end - key_first + kStep - 1) / kStep : 0;
+  const char* ring = s_raw + wave * L::kStages * L::kBytes;
+  const uint32_t ring_lds = lds_address(ring);
+  bool hole[L::kStages][2];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + i * kStep);
+    if (i < tiles) load_tile<kDim>(pool, pages, head, key_first + i * kStep, ring_lds + i * L::kBytes);
+    hole[i][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
+    hole[i][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
+  }
+  TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + kAhead * kStep);
+  int slot = 0, fill = kAhead * L::kBytes;  // offsets in the ring
+  for (int n = 0; n < tiles; ++n) {
+    const int key0 = key_first + n * kStep;
+    hole[kAhead][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
+    hole[kAhead][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
+    if (n + kAhead < tiles) {
+      load_tile<kDim>(pool, pages, head, key0 + kAhead * kStep, ring_lds + fill);
+      vm_wait_lds<kAhead * L::kLoads>();
+    } else {
+      vm_wait_lds<0>();
+    }
+    // The page numbers of the tile after that.
+    pages = tile_pages(pool, batch, seq, u.length, key0 + (kAhead + 1) * kStep);
+    const char* now = ring + slot;
+    slot = slot + L::kBytes == L::kStages * L::kBytes ? 0 : slot + L::kBytes;
+    fill = fill + L::kBytes == L::kStages * L::kBytes ? 0 : fill + L::kBytes;
 
     // Scores of the tile.
     v4f s[kCols][2];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) s[c][0] = s[c][1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      uint32_t words[S::kKeyWords];
+      const int place = col % 4 * 4 + col / 4;
+      const uint32_t* src =
+          reinterpret_cast<const uint32_t*>(now + h * L::kHalf + place * (kDim / 2) + g * (kDim / 8));
+      if constexpr (S::kKeyWords % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < S::kKeyWords / 4; ++i) {
+          const v4u w = reinterpret_cast<const v4u*>(src)[i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) words[4 * i + j] = w[j];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::kKeyWords; ++i) words[i] = src[i];
+      }
 #pragma unroll
       for (int i = 0; i < S::kKeyWords; ++i) {
-        const v8h a = decode_word(tile.key[h][i]);
+        const v8h a = decode_word(words[i]);
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
           for (int p = 0; p < kParts; ++p)
             s[c][h] = mfma(a, q[c][p][i], s[c][h]);
       }
+    }
+    v4f key_scale[2], value_scale[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v4f* scales = reinterpret_cast<const v4f*>(now + L::kScales + h * 64);
+      key_scale[h] = scales[g];
+      value_scale[h] = scales[8 + g];
+    }
     mfma_results_fence();
 
-    const bool whole = key0 >= all_low && key0 + kTileKeys <= all_high && args.mask == nullptr && !tile.hole[0] &&
-                       !tile.hole[1];
+    const bool whole = key0 >= all_low && key0 + kTileKeys <= all_high && args.mask == nullptr && !hole[0][0] &&
+                       !hole[0][1];
     Prob probs[kCols][kProbParts];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       float x[8], vs[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = s[c][i / 4][i % 4] * (tile.key_scale[i / 4][i % 4] * factor[c]);
-        vs[i] = tile.value_scale[i / 4][i % 4];
+        x[i] = s[c][i / 4][i % 4] * (key_scale[i / 4][i % 4] * factor[c]);
+        vs[i] = value_scale[i / 4][i % 4];
       }
       if (!whole) {
         // A hidden key takes no part in the maxima, and its probability and
@@ -415,7 +514,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = key0 + 16 * (i / 4) + 4 * g + i % 4;
-          bool see = key >= see_low[c] && key < see_high[c] && !tile.hole[i / 4];
+          bool see = key >= see_low[c] && key < see_high[c] && !hole[0][i / 4];
           if (args.mask != nullptr && see) see = mask[c][key] != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
@@ -452,9 +551,15 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
 #pragma unroll
     for (int k = 0; k < (S::kValueDims + 7) / 8; ++k) {
       uint32_t low[4], high[4];
+      const int vl = S::kValueLanes == 16 ? col : min(col, S::kValueLanes - 1);
+      auto value = [&](int h, int r) -> uint32_t {
+        const char* src = now + (2 + h) * L::kHalf + (4 * r + g) * (kDim / 2) + vl * (S::kValueDims / 2) + 4 * k;
+        if constexpr (S::kValueDims == 4) return *reinterpret_cast<const uint16_t*>(src);
+        return *reinterpret_cast<const uint32_t*>(src);
+      };
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const uint32_t a = tile.value[p / 2][2 * (p % 2)][k], b = tile.value[p / 2][2 * (p % 2) + 1][k];
+        const uint32_t a = value(p / 2, 2 * (p % 2)), b = value(p / 2, 2 * (p % 2) + 1);
         low[p] = __builtin_amdgcn_perm(b, a, 0x05040100u);
         high[p] = __builtin_amdgcn_perm(b, a, 0x07060302u);
       }
@@ -486,131 +591,175 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_attend_kernel(Kv4Pool pool,
         }
       }
     }
-    tile = next;
+    // All reads of the slot are behind this point: the next turn fills it.
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) asm volatile("" : "+v"(o[c][t]));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) hole[i][0] = hole[i + 1][0], hole[i][1] = hole[i + 1][1];
   }
   mfma_results_fence();
 
-  // The waves' results joined in a fixed order: the upper half hands over to
-  // the lower one until wave 0 holds the sum.
-  float* s_ref = reinterpret_cast<float*>(s_raw);           // [waves][cols][16]
-  float* s_sum = s_ref + kWaves * kRows;                    // [waves][cols][16]
-  v4f* s_o = reinterpret_cast<v4f*>(s_sum + kWaves * kRows);  // [waves / 2][cols][tiles][64]
+  // The waves' results joined in their order, in LDS.
+  float* s_ref = reinterpret_cast<float*>(s_raw);  // [waves][rows]
+  float* s_sum = s_ref + kWaves * kRows;           // [waves][rows]
+  float* s_o = s_sum + kWaves * kRows;             // [waves][rows][dim + 4]
+  constexpr int kPitch = kDim + 4;                 // spreads the rows over the banks
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) sum[c] = across_groups_sum(sum[c]);
+  __syncthreads();  // the rings have been read
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
-    sum[c] = across_groups_sum(sum[c]);
-    if (g == 0) s_ref[wave * kRows + 16 * c + col] = ref[c];
+    const int r = wave * kRows + 16 * c + col;
+    if (g == 0) s_ref[r] = ref[c], s_sum[r] = sum[c];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * g + i < S::kValueLanes) {
+        v4f* dst = reinterpret_cast<v4f*>(s_o + r * kPitch + (4 * g + i) * S::kValueDims);
+#pragma unroll
+        for (int t = 0; t < S::kTiles / 4; ++t)
+          dst[t] = (v4f){o[c][4 * t][i], o[c][4 * t + 1][i], o[c][4 * t + 2][i], o[c][4 * t + 3][i]};
+      }
   }
   __syncthreads();
+  const bool whole_item = from == 0 && upto == u.granules;
+  constexpr int kPerRow = kDim / 4;
+  for (int i = threadIdx.x; i < kRows * kPerRow; i += kWaves * kWave) {
+    const int local = i / kPerRow, d = i % kPerRow * 4;
+    const uint32_t r = tile * kRows + local;
+    const int token = (int)(r / split.share), sub = (int)(r - token * split.share);
+    if (token >= u.rows) continue;
+    float all = s_ref[local];
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    float all = s_ref[16 * c + col];
+    for (int w = 1; w < kWaves; ++w) all = fmaxf(all, s_ref[w * kRows + local]);
+    float total = 0.0f;
+    v4f sum4 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) all = fmaxf(all, s_ref[w * kRows + 16 * c + col]);
-    const float alpha = exp2_hw(ref[c] - all);
-    ref[c] = all;
-    sum[c] *= alpha;
-    if (g == 0) s_sum[wave * kRows + 16 * c + col] = sum[c];
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) o[c][t] *= alpha;
-  }
-#pragma unroll
-  for (int n = kWaves / 2; n >= 1; n /= 2) {
-    if (wave >= n && wave < 2 * n) {
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) s_o[(((wave - n) * kCols + c) * S::kTiles + t) * kWave + lane] = o[c][t];
+    for (int w = 0; w < kWaves; ++w) {
+      const float alpha = exp2_hw(s_ref[w * kRows + local] - all);
+      total += s_sum[w * kRows + local] * alpha;
+      sum4 += *reinterpret_cast<const v4f*>(s_o + (w * kRows + local) * kPitch + d) * alpha;
     }
-    __syncthreads();
-    if (wave < n) {
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int t = 0; t < S::kTiles; ++t) o[c][t] += s_o[((wave * kCols + c) * S::kTiles + t) * kWave + lane];
-    }
-    __syncthreads();
-  }
-  if (wave != 0) return;
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    const int64_t r = (int64_t)u.tile * kRows + 16 * c + col;
-    const int token = (int)(r / shape.share), sub = (int)(r % shape.share);
-    float total = s_sum[16 * c + col];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) total += s_sum[w * kRows + 16 * c + col];
-    if (u.parts > 1) {
-      const int64_t slot = ((int64_t)u.slot * pool.kv_heads + head);
-      if (slot >= shape.slots) continue;
-      float* dst = partial + slot * kRows * (kDim + 2) + (16 * c + col) * (kDim + 2);
-      if (g == 0) {
-        dst[kDim] = ref[c];
-        dst[kDim + 1] = total;
+    if (!whole_item) {
+      // [rows][dim], then [rows][reference, sum]
+      float* dst = partial + ((int64_t)blockIdx.x * 2 + (from == 0)) * kRows * (kDim + 2);
+      *reinterpret_cast<v4f*>(dst + local * kDim + d) = sum4;
+      if (d == 0) {
+        dst[kRows * kDim + 2 * local] = all;
+        dst[kRows * kDim + 2 * local + 1] = total;
       }
-#pragma unroll
-      for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (4 * g + i < S::kValueLanes) dst[(4 * g + i) * S::kValueDims + t] = o[c][t][i];
       continue;
     }
-    if (token >= u.rows) continue;
-    const int qh = head * shape.share + sub;
-    const int64_t row = u.first_row + token;
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    if (args.lse != nullptr && g == 0)
-      args.lse[row * args.heads + qh] = total == 0.0f ? kNegInf : (ref[c] + __log2f(total)) * 0.69314718055994531f;
-    const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * g + i < S::kValueLanes)
-          store_out<T>(args.out, base + (4 * g + i) * S::kValueDims + t, o[c][t][i] * inv);
+    const int qh = head * split.share + sub;
+    const int64_t row = u.first + token;
+    if (args.lse != nullptr && d == 0)
+      args.lse[row * args.heads + qh] = total == 0.0f ? kNegInf : (all + __log2f(total)) * 0.69314718055994531f;
+    sum4 *= total == 0.0f ? 0.0f : 1.0f / total;
+    store4<T>(args.out, row * args.out_row_stride + (int64_t)qh * args.out_head_stride + d, args.out_wide != 0, sum4);
   }
 }
 
-// One workgroup per (row of the call, head): joins the parts of a split row.
+// Worker blockIdx.x's granules, item by item.
+template <Kv4Type T, int kDim, int kCols>
+__global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
+                                                                   Split split, float* __restrict__ partial) {
+  Deal deal;
+  int seq = 0;
+  uint32_t before = 0;
+  if (!find_work(pool, batch, args, split, blockIdx.x, seq, before, deal)) {
+    // The last workgroup has none: rows of no sequence come out as rows that
+    // see nothing.
+    if (blockIdx.x == gridDim.x - 1 && batch.offsets != nullptr) {
+      const int first = kv4_first_row(batch, 0), last = kv4_first_row(batch, batch.batch);
+      for (int row = 0; row < batch.rows; ++row) {
+        if (row >= first && row < last) row = last;
+        if (row >= batch.rows) break;
+        for (int i = threadIdx.x; i < args.heads * kDim; i += blockDim.x)
+          store_out<T>(args.out, row * args.out_row_stride + i / kDim * args.out_head_stride + i % kDim, 0.0f);
+        for (int h = threadIdx.x; h < args.heads && args.lse != nullptr; h += blockDim.x)
+          args.lse[(int64_t)row * args.heads + h] = kNegInf;
+      }
+    }
+    return;
+  }
+  uint32_t granule = deal.begin(blockIdx.x);
+  const uint32_t last_granule = deal.begin(blockIdx.x + 1);
+  SeqWork u = uniform_seq_work(pool, batch, args, split, seq);
+  while (granule < last_granule) {
+    while (granule - before >= u.tiles * pool.kv_heads * u.granules) {
+      before += u.tiles * pool.kv_heads * u.granules;
+      if (++seq >= batch.batch) return;  // offsets out of order
+      u = uniform_seq_work(pool, batch, args, split, seq);
+    }
+    const uint32_t item = (granule - before) / u.granules;
+    const uint32_t item_at = before + item * u.granules;  // its first granule
+    const uint32_t from = granule - item_at, upto = min(u.granules, last_granule - item_at);
+    const uint32_t tile = item / (uint32_t)pool.kv_heads;
+    attend_item<T, kDim, kCols>(pool, batch, args, split, partial, u, seq, tile, item - tile * pool.kv_heads, from,
+                                upto);
+    granule = item_at + upto;
+    __syncthreads();
+  }
+}
+
+// One workgroup per (row of the call, head): joins the parts of a split item.
 template <Kv4Type T, int kDim>
 __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
-                                                                 SplitShape shape, const float* __restrict__ partial) {
-  const int row = blockIdx.x;
-  const int seq = kv4_find_sequence(batch, row);
-  Split u;
-  if (seq < 0 || !find_split(pool, batch, args, shape, -1, seq, u)) return;
-  if (u.parts <= 1) return;
-  const int token = row - u.first_row;
-  for (int qh = blockIdx.y * kWaves + threadIdx.x / kWave; qh < args.heads; qh += gridDim.y * kWaves) {
-    const int head = qh / shape.share;
-    const int64_t r = (int64_t)token * shape.share + qh % shape.share;
-    const int64_t slot0 = u.slot + r / shape.tile_rows * u.parts;
-    const float* src = partial + r % shape.tile_rows * (kDim + 2);
-    const int64_t stride = (int64_t)shape.tile_rows * (kDim + 2);
-    float all = kUnset;
-    for (int p = lane_id(); p < u.parts; p += kWave) {
-      const int64_t slot = (slot0 + p) * pool.kv_heads + head;
-      if (slot < shape.slots) all = fmaxf(all, src[slot * stride + kDim]);
-    }
-    all = wave_reduce(all, [](float a, float b) { return fmaxf(a, b); });
-    float total = 0.0f, o[(kDim + 63) / 64] = {};
-    for (int p = 0; p < u.parts; ++p) {
-      const int64_t slot = (slot0 + p) * pool.kv_heads + head;
-      if (slot >= shape.slots) break;
-      const float* part = src + slot * stride;
-      const float alpha = exp2_hw(part[kDim] - all);
-      total += part[kDim + 1] * alpha;
+                                                                 Split split, const float* __restrict__ partial) {
+  constexpr int kRegs = (kDim + 63) / 64;
+  __shared__ float s_part[kWaves][kDim + 2];
+  const int row = blockIdx.x, qh = blockIdx.y, wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
+  int seq = kv4_find_sequence(batch, row);
+  Deal deal;
+  uint32_t before = 0;
+  if (seq < 0 || !find_work(pool, batch, args, split, -1, seq, before, deal)) return;
+  const SeqWork u = uniform_seq_work(pool, batch, args, split, seq);
+  const uint32_t head = qh / split.share, rows = 1u << split.tile_shift;
+  const uint32_t r = (uint32_t)(row - u.first) * split.share + (qh - head * split.share), local = r & (rows - 1);
+  const uint32_t item_at = before + ((r >> split.tile_shift) * pool.kv_heads + head) * u.granules;
+  const uint32_t first = deal.worker_of(item_at), last = deal.worker_of(item_at + u.granules - 1);
+  if (first == last) return;
+  // Each wave joins every kWaves-th part, then the waves' sums are joined.
+  float all = kUnset, total = 0.0f, o[kRegs] = {};
+  for (uint32_t i = first + wave; i <= last; i += kWaves) {
+    const float* slot = partial + ((int64_t)i * 2 + (i == first)) * rows * (kDim + 2);
+    const float* part = slot + local * kDim;
+    const float ref = slot[rows * kDim + 2 * local], more = slot[rows * kDim + 2 * local + 1], now = fmaxf(all, ref);
+    const float old = exp2_hw(all - now), alpha = exp2_hw(ref - now);
+    all = now;
+    total = total * old + more * alpha;
 #pragma unroll
-      for (int i = 0; i < (kDim + 63) / 64; ++i)
-        if (i * 64 + lane_id() < kDim) o[i] += part[i * 64 + lane_id()] * alpha;
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    if (args.lse != nullptr && lane_id() == 0)
-      args.lse[(int64_t)row * args.heads + qh] =
-          total == 0.0f ? kNegInf : (all + __log2f(total)) * 0.69314718055994531f;
-    const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
-#pragma unroll
-    for (int i = 0; i < (kDim + 63) / 64; ++i)
-      if (i * 64 + lane_id() < kDim) store_out<T>(args.out, base + i * 64 + lane_id(), o[i] * inv);
+    for (int k = 0; k < kRegs; ++k)
+      if (k * 64 + lane < kDim) o[k] = o[k] * old + part[k * 64 + lane] * alpha;
   }
+#pragma unroll
+  for (int k = 0; k < kRegs; ++k)
+    if (k * 64 + lane < kDim) s_part[wave][k * 64 + lane] = o[k];
+  if (lane == 0) s_part[wave][kDim] = all, s_part[wave][kDim + 1] = total;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_part[w][kDim]);
+  total = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kRegs; ++k) o[k] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float alpha = exp2_hw(s_part[w][kDim] - all);
+    total += s_part[w][kDim + 1] * alpha;
+#pragma unroll
+    for (int k = 0; k < kRegs; ++k)
+      if (k * 64 + lane < kDim) o[k] += s_part[w][k * 64 + lane] * alpha;
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if (args.lse != nullptr && lane == 0)
+    args.lse[(int64_t)row * args.heads + qh] =
+        total == 0.0f ? kNegInf : (all + __log2f(total)) * 0.69314718055994531f;
+  const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
+#pragma unroll
+  for (int k = 0; k < kRegs; ++k)
+    if (k * 64 + lane < kDim) store_out<T>(args.out, base + k * 64 + lane, o[k] * inv);
 }
 
 // Column tiles per workgroup: as many as a sequence's rows fill on average (one
@@ -620,55 +769,50 @@ int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
 }
 
-SplitShape split_shape(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
-  SplitShape s;
+Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, int num_cus) {
+  Split s;
+  const int columns = columns_for(pool, batch, heads);
   s.share = heads / pool.kv_heads;
-  s.tile_rows = 16 * columns_for(pool, batch, heads);
-  s.target = 4 * num_cus;
-  // A split sequence has more than one chunk, so its last one is less than
-  // half of what it adds: units of split sequences number less than twice the
-  // target.
-  s.slots = 2 * s.target + pool.kv_heads;
+  s.tile_shift = columns == 2 ? 5 : 4;
+  const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
+  s.one_launch = longest <= kShort;
+  s.granule_shift = __builtin_ctz(s.one_launch ? kShort : kGranule);
+  const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
+  while (items * ((longest >> s.granule_shift) + 1) >= (int64_t)1 << 31) ++s.granule_shift;
+  s.least = s.one_launch ? 1 : 4;
+  s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
   return s;
 }
 
 template <Kv4Type T, int kDim, int kCols>
-hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                         const SplitShape& shape, float* partial, hipStream_t stream) {
-  const int64_t tiles = ((int64_t)batch.rows * shape.share) / shape.tile_rows + batch.batch;
-  const int64_t grid = tiles * pool.kv_heads + shape.target + pool.kv_heads;
-  if (grid > (1 << 24)) return hipErrorInvalidValue;
-  constexpr int kRows = 16 * kCols;
-  const size_t lds = sizeof(float) * (2 * kWaves * kRows + (kWaves / 2) * kRows * 16 * Shape<kDim>::kTiles);
-  kv4_attend_kernel<T, kDim, kCols><<<dim3((unsigned)grid), dim3(kWaves * kWave), lds, stream>>>(pool, batch, args,
-                                                                                               shape, partial);
+hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
+                         float* partial, hipStream_t stream) {
+  kv4_attend_kernel<T, kDim, kCols><<<dim3((unsigned)split.workers + 1), dim3(kWaves * kWave), 0, stream>>>(
+      pool, batch, args, split, partial);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  // No sequence is split if none can be longer than the least chunk.
-  if (((int64_t)batch.max_pages << pool.page_shift) > kMinChunk) {
-    const int by = std::min(8, (args.heads + kWaves - 1) / kWaves);
-    kv4_join_kernel<T, kDim><<<dim3((unsigned)batch.rows, (unsigned)by), dim3(kWaves * kWave), 0, stream>>>(
-        pool, batch, args, shape, partial);
-  }
+  if (!split.one_launch)
+    kv4_join_kernel<T, kDim><<<dim3((unsigned)batch.rows, (unsigned)args.heads), dim3(kWaves * kWave), 0, stream>>>(
+        pool, batch, args, split, partial);
   return hipGetLastError();
 }
 
 template <Kv4Type T, int kDim>
-hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const SplitShape& shape,
+hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                       float* partial, hipStream_t stream) {
   if constexpr (kDim <= 128)
-    if (shape.tile_rows == 32) return launch_attend<T, kDim, 2>(pool, batch, args, shape, partial, stream);
-  return launch_attend<T, kDim, 1>(pool, batch, args, shape, partial, stream);
+    if (split.tile_shift == 5) return launch_attend<T, kDim, 2>(pool, batch, args, split, partial, stream);
+  return launch_attend<T, kDim, 1>(pool, batch, args, split, partial, stream);
 }
 
 template <Kv4Type T>
-hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const SplitShape& shape,
+hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                        float* partial, hipStream_t stream) {
   switch (pool.dim) {
-    case 64: return launch_dim<T, 64>(pool, batch, args, shape, partial, stream);
-    case 96: return launch_dim<T, 96>(pool, batch, args, shape, partial, stream);
-    case 128: return launch_dim<T, 128>(pool, batch, args, shape, partial, stream);
-    case 192: return launch_dim<T, 192>(pool, batch, args, shape, partial, stream);
-    case 256: return launch_dim<T, 256>(pool, batch, args, shape, partial, stream);
+    case 64: return launch_dim<T, 64>(pool, batch, args, split, partial, stream);
+    case 96: return launch_dim<T, 96>(pool, batch, args, split, partial, stream);
+    case 128: return launch_dim<T, 128>(pool, batch, args, split, partial, stream);
+    case 192: return launch_dim<T, 192>(pool, batch, args, split, partial, stream);
+    case 256: return launch_dim<T, 256>(pool, batch, args, split, partial, stream);
   }
   return hipErrorInvalidValue;
 }
@@ -676,19 +820,19 @@ hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
 }  // namespace
 
 size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
-  const SplitShape s = split_shape(pool, batch, heads, num_cus);
-  return (size_t)s.slots * s.tile_rows * (pool.dim + 2) * sizeof(float);
+  const Split s = split_for(pool, batch, heads, kKv4BF16, num_cus);  // the type with the most workers
+  return ((size_t)s.workers * 2 << s.tile_shift) * (pool.dim + 2) * sizeof(float);
 }
 
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              void* workspace, int num_cus, hipStream_t stream) {
   if (batch.rows <= 0) return hipSuccess;
-  const SplitShape shape = split_shape(pool, batch, args.heads, num_cus);
+  const Split split = split_for(pool, batch, args.heads, type, num_cus);
   float* partial = static_cast<float*>(workspace);
   switch (type) {
-    case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, shape, partial, stream);
-    case kKv4F16: return launch_type<kKv4F16>(pool, batch, args, shape, partial, stream);
-    case kKv4BF16: return launch_type<kKv4BF16>(pool, batch, args, shape, partial, stream);
+    case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, stream);
+    case kKv4F16: return launch_type<kKv4F16>(pool, batch, args, split, partial, stream);
+    case kKv4BF16: return launch_type<kKv4BF16>(pool, batch, args, split, partial, stream);
   }
   return hipErrorInvalidValue;
 }
