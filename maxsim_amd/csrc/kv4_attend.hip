@@ -30,24 +30,19 @@
 // Bytes bound it: dim + 8 per key and head against 4 dim operations per query
 // row.  The keys of a sequence are split among workgroups when there are few
 // query rows; each leaves its unnormalised sum and a second launch joins them.
-#include <cfloat>
-
-#include "codes4.hpp"
-#include "kv4.hpp"
+#include "kv4_split.hpp"
 
 namespace msim {
 
 namespace {
 
-constexpr int kTileKeys = 32;
+constexpr int kTileKeys = kKeyAlign;
 constexpr int kWaves = 4;
-#ifndef MSIM_KV4_STAGES
-#define MSIM_KV4_STAGES 3
-#endif
+constexpr int kStages = 2;  // of a wave's ring: three or four, with as many or fewer waves, gained nothing
 
 // Rings of tiles, and in their place the join of the waves.
 constexpr int attend_lds(int dim, int cols) {
-  const int rings = kWaves * (dim <= 128 ? MSIM_KV4_STAGES : 2) * (32 * dim + 256);
+  const int rings = kWaves * kStages * (32 * dim + 256);
   const int join = 16 * cols * 4 * kWaves * (2 + dim + 4);
   return rings > join ? rings : join;
 }
@@ -56,135 +51,6 @@ constexpr int attend_lds(int dim, int cols) {
 constexpr int waves_per_simd(Kv4Type type, int dim, int cols) {
   return type == kKv4F32 || dim > 128 || cols > 1 ? (dim > 192 || (type == kKv4F32 && dim * cols > 192) ? 1 : 2) : 3;
 }
-constexpr float kUnset = -FLT_MAX;
-// A row's reference moves when a product passes 2^15 or a probability 2^100, to
-// where the largest are 2^13 and 2^90.
-constexpr float kProductLimit = 15.0f, kProductGoal = 13.0f, kProbLimit = 100.0f, kProbGoal = 90.0f;
-
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// --------------------------------------------------------------- the split
-//
-// An item is (sequence, tile of query rows, key/value head), a granule 128 of
-// its keys.  All granules, in the order of items, are dealt out evenly: worker
-// i of n has those from i G / n to (i + 1) G / n, whatever items they belong to.
-// An item that lies within one worker is finished there; of the others each
-// worker leaves a partial result, in its slot 1 if the item begins there, in
-// slot 0 if it came in from the worker before (it has at most one of each).
-//
-// Where no sequence can be longer than kShort keys a granule is kShort: no item
-// is split, and the call is one launch.
-constexpr int kGranule = kWaves * kTileKeys;
-constexpr int kShort = 4 * kGranule;
-
-//
-// Granules, items and rows are counted in 32 bits: the host refuses calls of 2^30
-// rows times heads and doubles the granule where their number could pass 2^31.
-struct Split {
-  uint32_t share;       // query heads per key/value head
-  uint32_t tile_shift;  // log2(query rows of a tile)
-  uint32_t workers;     // at most
-  uint32_t granule_shift;
-  uint32_t least;       // granules of a worker, where that leaves more than one
-  uint32_t one_launch;  // no item is split
-};
-
-struct SeqWork {
-  int first, rows, length, low;
-  uint32_t tiles;
-  uint32_t granules;  // of one item
-};
-
-__device__ __forceinline__ SeqWork seq_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                            const Split& split, int b) {
-  SeqWork w;
-  w.first = kv4_first_row(batch, b);
-  w.rows = max(0, kv4_first_row(batch, b + 1) - w.first);
-  w.length = kv4_length(pool, batch, b);
-  // The first key that the first row sees, if it sees the last ones only.
-  const int start = w.length - w.rows;
-  w.low = start >= args.window ? (start - args.window + 1) / kTileKeys * kTileKeys : 0;
-  w.tiles = ((uint32_t)w.rows * split.share + (1u << split.tile_shift) - 1) >> split.tile_shift;
-  w.granules = max(1u, ((uint32_t)(w.length - w.low) + (1u << split.granule_shift) - 1) >> split.granule_shift);
-  return w;
-}
-
-// A sequence that is the whole wave's.
-__device__ __forceinline__ SeqWork uniform_seq_work(const Kv4Pool& pool, const Kv4Batch& batch,
-                                                    const Kv4AttendArgs& args, const Split& split, int b) {
-  SeqWork w = seq_work(pool, batch, args, split, b);
-  w.first = wave_uniform(w.first);
-  w.rows = wave_uniform(w.rows);
-  w.length = wave_uniform(w.length);
-  w.low = wave_uniform(w.low);
-  w.tiles = wave_uniform(w.tiles);
-  w.granules = wave_uniform(w.granules);
-  return w;
-}
-
-// Inclusive sums over the lanes (DPP row shifts, then the rows' last lanes).
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  auto add = [&](auto ctrl, auto rows) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-  };
-  typedef std::integral_constant<int, 0xF> All;
-  add(std::integral_constant<int, 0x111>{}, All{});
-  add(std::integral_constant<int, 0x112>{}, All{});
-  add(std::integral_constant<int, 0x114>{}, All{});
-  add(std::integral_constant<int, 0x118>{}, All{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
-  return v;
-}
-
-// `total` granules among `workers`: the first `extra` have one more.
-struct Deal {
-  uint32_t total, workers, each, extra;
-  __device__ uint32_t begin(uint32_t i) const { return i * each + min(i, extra); }
-  __device__ uint32_t worker_of(uint32_t granule) const {
-    const uint32_t longer = extra * (each + 1);
-    return min(workers - 1, granule < longer ? granule / (each + 1) : extra + (granule - longer) / each);
-  }
-};
-
-// By a wave together: the deal, and the sequence that holds the first granule
-// of worker `worker` (or, worker < 0, sequence `seq`) with the granules before
-// it.  False if the worker has none.
-__device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                          const Split& split, int worker, int& seq, uint32_t& before, Deal& deal) {
-  const int lane = lane_id();
-  auto granules = [&](int b) -> uint32_t {
-    if (b >= batch.batch) return 0;
-    const SeqWork w = seq_work(pool, batch, args, split, b);
-    return w.tiles * pool.kv_heads * w.granules;
-  };
-  const uint32_t head = granules(lane);
-  uint32_t total = head;
-  for (int b0 = kWave; b0 < batch.batch; b0 += kWave) total += granules(b0 + lane);
-  const uint32_t head_scan = wave_scan(head);
-  deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
-                                    : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
-  deal.workers = min(split.workers, max(1u, deal.total / split.least));
-  deal.each = deal.total / deal.workers;
-  deal.extra = deal.total - deal.each * deal.workers;
-  if (deal.total == 0 || worker >= (int)deal.workers) return false;
-  const uint32_t target = worker >= 0 ? deal.begin(worker) : 0;
-  uint32_t done = 0;
-  for (int b0 = 0; b0 < batch.batch; b0 += kWave) {
-    const uint32_t mine = b0 == 0 ? head : granules(b0 + lane);
-    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine)), first = upto - mine;
-    const uint64_t here = __ballot(worker >= 0 ? first <= target && target < upto : b0 + lane == seq);
-    if (here != 0) {
-      const int at = __builtin_ctzll(here);
-      seq = wave_uniform(b0 + at);
-      before = __builtin_amdgcn_readlane(first, at);
-      return true;
-    }
-    done = __builtin_amdgcn_readlane(upto, kWave - 1);
-  }
-  return false;
-}
-
 // ------------------------------------------------------------ the main kernel
 
 template <int kDim>
@@ -206,81 +72,7 @@ struct TileLds {
   static constexpr int kBytes = kScales + 256;
   static constexpr int kHalfLoads = (kHalf + 1023) / 1024;
   static constexpr int kLoads = 4 * kHalfLoads + 1;  // of a wave, per tile
-  static constexpr int kStages = kDim <= 128 ? MSIM_KV4_STAGES : 2;
 };
-
-// Eight codes of a word as bfloat16, in the order of decode_word.
-__device__ __forceinline__ v8b decode_word_bf16(uint32_t w) {
-  return __builtin_bit_cast(v8b, (v4u){pair_bf16(w << 3), pair_bf16(w >> 1), pair_bf16(w >> 5), pair_bf16(w >> 9)});
-}
-
-// Eight codes of a word as f16: pairs (code i, code i + 4).
-__device__ __forceinline__ v8h decode_word(uint32_t w) {
-  const v2h base = {(_Float16)1032.0f, (_Float16)1032.0f};
-  const v2h high = {(_Float16)72.0f, (_Float16)72.0f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  const uint32_t w8 = w >> 8;
-  const v2h a = __builtin_bit_cast(v2h, (w & 0x000F000Fu) ^ 0x64086408u) - base;
-  const v2h b = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & 0x00F000F0u) ^ 0x64806480u), sixteenth, -high);
-  const v2h c = __builtin_bit_cast(v2h, (w8 & 0x000F000Fu) ^ 0x64086408u) - base;
-  const v2h d = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w8 & 0x00F000F0u) ^ 0x64806480u), sixteenth, -high);
-  return (v8h){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// The order of a word's codes in decode_word's result.
-__device__ __forceinline__ constexpr int word_order(int i) { return (i & 1) * 4 + i / 2; }
-
-// Eight elements of a query from element i on (16-byte loads if `wide`).
-template <Kv4Type T>
-__device__ __forceinline__ void load8(const void* q, int64_t i, bool wide, float (&x)[8]) {
-  if constexpr (T == kKv4F32) {
-    const float* p = static_cast<const float*>(q) + i;
-    if (wide) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const v4f v = reinterpret_cast<const v4f*>(p)[k];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * k + j] = v[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = p[j];
-    }
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(q) + i;
-    uint16_t h[8];
-    if (wide) {
-      __builtin_memcpy(h, __builtin_assume_aligned(p, 16), 16);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = p[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[j] = T == kKv4BF16 ? __uint_as_float((uint32_t)h[j] << 16) : (float)__builtin_bit_cast(_Float16, h[j]);
-  }
-}
-
-template <Kv4Type T>
-__device__ __forceinline__ void store_out(void* out, int64_t i, float x) {
-  if constexpr (T == kKv4F32) static_cast<float*>(out)[i] = x;
-  if constexpr (T == kKv4F16) static_cast<_Float16*>(out)[i] = (_Float16)x;
-  if constexpr (T == kKv4BF16) static_cast<__bf16*>(out)[i] = (__bf16)x;
-}
-
-// Four elements of an output row (one store if `wide`).
-template <Kv4Type T>
-__device__ __forceinline__ void store4(void* out, int64_t i, bool wide, v4f x) {
-  if (!wide) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) store_out<T>(out, i + k, x[k]);
-  } else if constexpr (T == kKv4F32) {
-    *reinterpret_cast<v4f*>(static_cast<float*>(out) + i) = x;
-  } else {
-    typedef typename std::conditional<T == kKv4F16, _Float16, __bf16>::type E;
-    typedef E v4e __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<v4e*>(static_cast<E*>(out) + i) = (v4e){(E)x[0], (E)x[1], (E)x[2], (E)x[3]};
-  }
-}
 
 // Page numbers of a tile's halves (pages hold 16 rows or a multiple, so a half
 // lies in one page); -1 past the sequence's end.
@@ -339,8 +131,8 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 // workgroup; its waves take the key tiles in turn.
 template <Kv4Type T, int kDim, int kCols>
 __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                            const Split& split, float* __restrict__ partial, const SeqWork& u,
-                                            int seq, uint32_t tile, int head, uint32_t from, uint32_t upto) {
+                                            const Split& split, float* __restrict__ partial, const Cursor& at,
+                                            uint32_t from, uint32_t upto) {
   typedef Shape<kDim> S;
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
   constexpr int kProbParts = T == kKv4F32 ? 3 : 1;  // of a probability
@@ -348,6 +140,10 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   constexpr int kRows = 16 * kCols;
   __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols)];
   const int lane = lane_id(), col = lane % 16, g = lane / 16, wave = wave_uniform(threadIdx.x / kWave);
+  const SeqWork& u = at.work;
+  const uint32_t tile = at.tile;
+  const int seq = at.seq, head = at.head;
+
   // Query rows of this tile: row r is new token r / share, head r % share.
   v8h q[kCols][kParts][S::kKeyWords];
   float factor[kCols];       // of a product with the codes, towards log2 scores
@@ -376,7 +172,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     }
     top = max(top, (uint32_t)__shfl_xor((int)top, 16));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    const int shift = 141 - (int)(top >> 23);  // the largest to [2^14, 2^15)
+    const int shift = query_shift(top);
 #pragma unroll
     for (int i = 0; i < S::kKeyWords; ++i)
 #pragma unroll
@@ -410,8 +206,8 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
   any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
   // This worker's keys of the item, cut to what some row sees.
-  const int begin = max(u.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
-  const int end = (int)min((int64_t)u.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
+  const int begin = max(at.range.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
+  const int end = (int)min((int64_t)at.range.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
 
   float ref[kCols], sum[kCols];
   v4f o[kCols][S::kTiles];
@@ -426,12 +222,12 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   // A ring of tiles per wave: kStages - 1 of them on their way while one is
   // worked on.
   typedef TileLds<kDim> L;
-  constexpr int kStep = kWaves * kTileKeys, kAhead = L::kStages - 1;
+  constexpr int kStep = kWaves * kTileKeys, kAhead = kStages - 1;
   const int key_first = begin + wave * kTileKeys;
   const int tiles = end > key_first ? (end - key_first + kStep - 1) / kStep : 0;
-  const char* ring = s_raw + wave * L::kStages * L::kBytes;
+  const char* ring = s_raw + wave * kStages * L::kBytes;
   const uint32_t ring_lds = lds_address(ring);
-  bool hole[L::kStages][2];
+  bool hole[kStages][2];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + i * kStep);
@@ -454,8 +250,8 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     // The page numbers of the tile after that.
     pages = tile_pages(pool, batch, seq, u.length, key0 + (kAhead + 1) * kStep);
     const char* now = ring + slot;
-    slot = slot + L::kBytes == L::kStages * L::kBytes ? 0 : slot + L::kBytes;
-    fill = fill + L::kBytes == L::kStages * L::kBytes ? 0 : fill + L::kBytes;
+    slot = slot + L::kBytes == kStages * L::kBytes ? 0 : slot + L::kBytes;
+    fill = fill + L::kBytes == kStages * L::kBytes ? 0 : fill + L::kBytes;
 
     // Scores of the tile.
     v4f s[kCols][2];
@@ -623,7 +419,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       }
   }
   __syncthreads();
-  const bool whole_item = from == 0 && upto == u.granules;
+  const bool whole_item = from == 0 && upto == at.range.granules;
   constexpr int kPerRow = kDim / 4;
   for (int i = threadIdx.x; i < kRows * kPerRow; i += kWaves * kWave) {
     const int local = i / kPerRow, d = i % kPerRow * 4;
@@ -642,8 +438,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       sum4 += *reinterpret_cast<const v4f*>(s_o + (w * kRows + local) * kPitch + d) * alpha;
     }
     if (!whole_item) {
-      // [rows][dim], then [rows][reference, sum]
-      float* dst = partial + ((int64_t)blockIdx.x * 2 + (from == 0)) * kRows * (kDim + 2);
+      float* dst = partial_slot(partial, split, kDim, blockIdx.x, from == 0);
       *reinterpret_cast<v4f*>(dst + local * kDim + d) = sum4;
       if (d == 0) {
         dst[kRows * kDim + 2 * local] = all;
@@ -654,7 +449,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     const int qh = head * split.share + sub;
     const int64_t row = u.first + token;
     if (args.lse != nullptr && d == 0)
-      args.lse[row * args.heads + qh] = total == 0.0f ? kNegInf : (all + __log2f(total)) * 0.69314718055994531f;
+      args.lse[row * args.heads + qh] = log_sum(all, total);
     sum4 *= total == 0.0f ? 0.0f : 1.0f / total;
     store4<T>(args.out, row * args.out_row_stride + (int64_t)qh * args.out_head_stride + d, args.out_wide != 0, sum4);
   }
@@ -665,101 +460,106 @@ template <Kv4Type T, int kDim, int kCols>
 __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
                                                                    Split split, float* __restrict__ partial) {
   Deal deal;
-  int seq = 0;
-  uint32_t before = 0;
-  if (!find_work(pool, batch, args, split, blockIdx.x, seq, before, deal)) {
-    // The last workgroup has none: rows of no sequence come out as rows that
-    // see nothing.
-    if (blockIdx.x == gridDim.x - 1 && batch.offsets != nullptr) {
-      const int first = kv4_first_row(batch, 0), last = kv4_first_row(batch, batch.batch);
-      for (int row = 0; row < batch.rows; ++row) {
-        if (row >= first && row < last) row = last;
-        if (row >= batch.rows) break;
-        for (int i = threadIdx.x; i < args.heads * kDim; i += blockDim.x)
-          store_out<T>(args.out, row * args.out_row_stride + i / kDim * args.out_head_stride + i % kDim, 0.0f);
-        for (int h = threadIdx.x; h < args.heads && args.lse != nullptr; h += blockDim.x)
-          args.lse[(int64_t)row * args.heads + h] = kNegInf;
-      }
-    }
+  Cursor at;
+  if (!find_work(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
+    if (blockIdx.x == gridDim.x - 1) loose_rows<T>(pool, batch, args);  // this workgroup never has work
+    note_unfinished(partial, split, kDim, at, 0);
     return;
   }
   uint32_t granule = deal.begin(blockIdx.x);
-  const uint32_t last_granule = deal.begin(blockIdx.x + 1);
-  SeqWork u = uniform_seq_work(pool, batch, args, split, seq);
-  while (granule < last_granule) {
-    while (granule - before >= u.tiles * pool.kv_heads * u.granules) {
-      before += u.tiles * pool.kv_heads * u.granules;
-      if (++seq >= batch.batch) return;  // offsets out of order
-      u = uniform_seq_work(pool, batch, args, split, seq);
-    }
-    const uint32_t item = (granule - before) / u.granules;
-    const uint32_t item_at = before + item * u.granules;  // its first granule
-    const uint32_t from = granule - item_at, upto = min(u.granules, last_granule - item_at);
-    const uint32_t tile = item / (uint32_t)pool.kv_heads;
-    attend_item<T, kDim, kCols>(pool, batch, args, split, partial, u, seq, tile, item - tile * pool.kv_heads, from,
-                                upto);
-    granule = item_at + upto;
+  const uint32_t last = deal.begin(blockIdx.x + 1);
+  at.enter(pool, batch, args, split);
+  int parts = 0;
+  while (granule < last && at.seek(pool, batch, args, split, granule)) {
+    const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
+    attend_item<T, kDim, kCols>(pool, batch, args, split, partial, at, from, upto);
+    granule = at.item_at + upto;
+    if (from == 0 && upto < at.range.granules)
+      parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
     __syncthreads();
   }
+  note_unfinished(partial, split, kDim, at, parts);
 }
 
-// One workgroup per (row of the call, head): joins the parts of a split item.
+// Joins the parts of split items: workgroup (i, y) has rows y, y + gridDim.y, ...
+// of the item that worker i left unfinished.
 template <Kv4Type T, int kDim>
-__global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
-                                                                 Split split, const float* __restrict__ partial) {
+__global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split,
+                                                                 float* __restrict__ partial) {
   constexpr int kRegs = (kDim + 63) / 64;
-  __shared__ float s_part[kWaves][kDim + 2];
-  const int row = blockIdx.x, qh = blockIdx.y, wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
-  int seq = kv4_find_sequence(batch, row);
-  Deal deal;
-  uint32_t before = 0;
-  if (seq < 0 || !find_work(pool, batch, args, split, -1, seq, before, deal)) return;
-  const SeqWork u = uniform_seq_work(pool, batch, args, split, seq);
-  const uint32_t head = qh / split.share, rows = 1u << split.tile_shift;
-  const uint32_t r = (uint32_t)(row - u.first) * split.share + (qh - head * split.share), local = r & (rows - 1);
-  const uint32_t item_at = before + ((r >> split.tile_shift) * pool.kv_heads + head) * u.granules;
-  const uint32_t first = deal.worker_of(item_at), last = deal.worker_of(item_at + u.granules - 1);
-  if (first == last) return;
-  // Each wave joins every kWaves-th part, then the waves' sums are joined.
-  float all = kUnset, total = 0.0f, o[kRegs] = {};
-  for (uint32_t i = first + wave; i <= last; i += kWaves) {
-    const float* slot = partial + ((int64_t)i * 2 + (i == first)) * rows * (kDim + 2);
-    const float* part = slot + local * kDim;
-    const float ref = slot[rows * kDim + 2 * local], more = slot[rows * kDim + 2 * local + 1], now = fmaxf(all, ref);
-    const float old = exp2_hw(all - now), alpha = exp2_hw(ref - now);
-    all = now;
-    total = total * old + more * alpha;
+  __shared__ float s_part[kWaves][kDim + 1];
+  const int wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
+  const uint32_t first = blockIdx.x;
+  const Unfinished item = reinterpret_cast<const Unfinished*>(partial + partial_floats(split, kDim))[first];
+  const int parts = min(item.parts, (int)(split.workers - first));
+  const uint32_t rows = 1u << split.tile_shift;
+  for (uint32_t local = blockIdx.y; parts > 0 && local < rows; local += gridDim.y) {
+    const uint32_t r = (item.tile << split.tile_shift) + local;
+    const int token = (int)(r / split.share), qh = item.head * split.share + (int)(r - token * split.share);
+    if (token >= item.rows) return;
+    // Lanes weigh 64 parts at a time; each wave adds up every kWaves-th of them,
+    // then the waves' sums are joined.
+    float all = kUnset, total = 0.0f, o[kRegs] = {};
+    for (int p0 = 0; p0 < parts; p0 += kWave) {
+      const int count = min(kWave, parts - p0);
+      auto slot = [&](int p) -> const float* {
+        return partial_slot(partial, split, kDim, first + p0 + p, p0 + p == 0);
+      };
+      const bool have = lane < count;
+      const float* mine = slot(have ? lane : 0) + rows * kDim + 2 * local;
+      const float ref = have ? mine[0] : kUnset, share = have ? mine[1] : 0.0f;
+      // All loads of the wave's parts go out before the weights are known.
+      float part[kWave / kWaves][kRegs];
+#pragma unroll
+      for (int i = 0; i < kWave / kWaves; ++i) {
+        const int p = i * kWaves + wave;
+        if (p >= count) break;
+        const float* src = slot(p) + local * kDim;
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k) part[i][k] = src[min(k * 64 + lane, kDim - 1)];
+      }
+      const float now = fmaxf(all, wave_reduce(ref, [](float a, float b) { return fmaxf(a, b); }));
+      const float old = exp2_hw(all - now), alpha = exp2_hw(ref - now);
+      all = now;
+      const float weighed = lane % kWaves == wave ? share * alpha : 0.0f;
+      total = total * old + wave_reduce(weighed, [](float a, float b) { return a + b; });
+#pragma unroll
+      for (int k = 0; k < kRegs; ++k) o[k] *= old;
+#pragma unroll
+      for (int i = 0; i < kWave / kWaves; ++i) {
+        const int p = i * kWaves + wave;
+        if (p >= count) break;
+        const float a = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alpha), p));
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k) o[k] = __builtin_fmaf(part[i][k], a, o[k]);
+      }
+    }
 #pragma unroll
     for (int k = 0; k < kRegs; ++k)
-      if (k * 64 + lane < kDim) o[k] = o[k] * old + part[k * 64 + lane] * alpha;
+      if (k * 64 + lane < kDim) s_part[wave][k * 64 + lane] = o[k];
+    if (lane == 0) s_part[wave][kDim] = total;
+    __syncthreads();
+    if (wave == 0) {
+      total = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kRegs; ++k) o[k] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        total += s_part[w][kDim];
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k)
+          if (k * 64 + lane < kDim) o[k] += s_part[w][k * 64 + lane];
+      }
+      const int64_t row = item.first + token;
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      if (args.lse != nullptr && lane == 0) args.lse[row * args.heads + qh] = log_sum(all, total);
+      const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
+#pragma unroll
+      for (int k = 0; k < kRegs; ++k)
+        if (k * 64 + lane < kDim) store_out<T>(args.out, base + k * 64 + lane, o[k] * inv);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int k = 0; k < kRegs; ++k)
-    if (k * 64 + lane < kDim) s_part[wave][k * 64 + lane] = o[k];
-  if (lane == 0) s_part[wave][kDim] = all, s_part[wave][kDim + 1] = total;
-  __syncthreads();
-  if (wave != 0) return;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_part[w][kDim]);
-  total = 0.0f;
-#pragma unroll
-  for (int k = 0; k < kRegs; ++k) o[k] = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float alpha = exp2_hw(s_part[w][kDim] - all);
-    total += s_part[w][kDim + 1] * alpha;
-#pragma unroll
-    for (int k = 0; k < kRegs; ++k)
-      if (k * 64 + lane < kDim) o[k] += s_part[w][k * 64 + lane] * alpha;
-  }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  if (args.lse != nullptr && lane == 0)
-    args.lse[(int64_t)row * args.heads + qh] =
-        total == 0.0f ? kNegInf : (all + __log2f(total)) * 0.69314718055994531f;
-  const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
-#pragma unroll
-  for (int k = 0; k < kRegs; ++k)
-    if (k * 64 + lane < kDim) store_out<T>(args.out, base + k * 64 + lane, o[k] * inv);
 }
 
 // Column tiles per workgroup: as many as a sequence's rows fill on average (one
@@ -771,37 +571,56 @@ int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
 
 Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, int num_cus) {
   Split s;
-  const int columns = columns_for(pool, batch, heads);
   s.share = heads / pool.kv_heads;
-  s.tile_shift = columns == 2 ? 5 : 4;
+  if (kv4_prompt_takes(pool, batch, heads, type)) {
+    s = kv4_prompt_split(num_cus);
+  } else {
+    const int columns = columns_for(pool, batch, heads);
+    s.tile_shift = columns == 2 ? 5 : 4;
+    s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
+    s.least = 4;
+  }
+  s.share = heads / pool.kv_heads;
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
   s.one_launch = longest <= kShort;
+  if (s.one_launch) s.least = 1;
   s.granule_shift = __builtin_ctz(s.one_launch ? kShort : kGranule);
   const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
   while (items * ((longest >> s.granule_shift) + 1) >= (int64_t)1 << 31) ++s.granule_shift;
-  s.least = s.one_launch ? 1 : 4;
-  s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
   return s;
+}
+
+template <Kv4Type T, int kDim>
+hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial,
+                       hipStream_t stream) {
+  // One row of a tile per workgroup, or a share of them; without offsets a tile
+  // has as many rows as heads share a key/value head.
+  const uint32_t rows = std::min(1u << split.tile_shift, batch.offsets == nullptr ? split.share : UINT32_MAX);
+  kv4_join_kernel<T, kDim><<<dim3(split.workers, std::min(32u, rows)), dim3(kWaves * kWave), 0, stream>>>(args, split,
+                                                                                                      partial);
+  return hipGetLastError();
 }
 
 template <Kv4Type T, int kDim, int kCols>
 hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                          float* partial, hipStream_t stream) {
-  kv4_attend_kernel<T, kDim, kCols><<<dim3((unsigned)split.workers + 1), dim3(kWaves * kWave), 0, stream>>>(
-      pool, batch, args, split, partial);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (!split.one_launch)
-    kv4_join_kernel<T, kDim><<<dim3((unsigned)batch.rows, (unsigned)args.heads), dim3(kWaves * kWave), 0, stream>>>(
-        pool, batch, args, split, partial);
+  kv4_attend_kernel<T, kDim, kCols><<<dim3(split.workers + 1), dim3(kWaves * kWave), 0, stream>>>(pool, batch, args,
+                                                                                                split, partial);
   return hipGetLastError();
 }
 
 template <Kv4Type T, int kDim>
 hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                       float* partial, hipStream_t stream) {
-  if constexpr (kDim <= 128)
-    if (split.tile_shift == 5) return launch_attend<T, kDim, 2>(pool, batch, args, split, partial, stream);
-  return launch_attend<T, kDim, 1>(pool, batch, args, split, partial, stream);
+  hipError_t e = hipErrorInvalidValue;
+  if (kv4_prompt_takes(pool, batch, args.heads, T))
+    e = launch_kv4_prompt(pool, batch, args, T, split, partial, stream);
+  else if (kDim > 128 || split.tile_shift == 4)
+    e = launch_attend<T, kDim, 1>(pool, batch, args, split, partial, stream);
+  else if constexpr (kDim <= 128)
+    e = launch_attend<T, kDim, 2>(pool, batch, args, split, partial, stream);
+  if (e != hipSuccess || split.one_launch) return e;
+  return launch_join<T, kDim>(batch, args, split, partial, stream);
 }
 
 template <Kv4Type T>
@@ -820,8 +639,12 @@ hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
 }  // namespace
 
 size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
-  const Split s = split_for(pool, batch, heads, kKv4BF16, num_cus);  // the type with the most workers
-  return ((size_t)s.workers * 2 << s.tile_shift) * (pool.dim + 2) * sizeof(float);
+  size_t bytes = 0;
+  for (Kv4Type type : {kKv4F32, kKv4BF16}) {  // f16 splits as bfloat16
+    const Split s = split_for(pool, batch, heads, type, num_cus);
+    bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * sizeof(Unfinished));
+  }
+  return bytes;
 }
 
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
