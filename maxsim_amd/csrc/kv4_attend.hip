@@ -493,12 +493,17 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
   const Unfinished item = reinterpret_cast<const Unfinished*>(partial + partial_floats(split, kDim))[first];
   const int parts = min(item.parts, (int)(split.workers - first));
   const uint32_t rows = 1u << split.tile_shift;
-  for (uint32_t local = blockIdx.y; parts > 0 && local < rows; local += gridDim.y) {
+  // Up to kDirect parts a wave joins a row by itself; of more, each wave adds up
+  // every kWaves-th part and the waves' sums are joined.
+  constexpr int kDirect = kWave / kWaves;
+  const bool direct = parts <= kDirect;
+  const int start = direct ? 0 : wave, stride = direct ? 1 : kWaves;
+  const uint32_t row_step = gridDim.y * (direct ? kWaves : 1);
+  for (uint32_t local = direct ? blockIdx.y * kWaves + wave : blockIdx.y; parts > 0 && local < rows;
+       local += row_step) {
     const uint32_t r = (item.tile << split.tile_shift) + local;
     const int token = (int)(r / split.share), qh = item.head * split.share + (int)(r - token * split.share);
     if (token >= item.rows) return;
-    // Lanes weigh 64 parts at a time; each wave adds up every kWaves-th of them,
-    // then the waves' sums are joined.
     float all = kUnset, total = 0.0f, o[kRegs] = {};
     for (int p0 = 0; p0 < parts; p0 += kWave) {
       const int count = min(kWave, parts - p0);
@@ -509,10 +514,10 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
       const float* mine = slot(have ? lane : 0) + rows * kDim + 2 * local;
       const float ref = have ? mine[0] : kUnset, share = have ? mine[1] : 0.0f;
       // All loads of the wave's parts go out before the weights are known.
-      float part[kWave / kWaves][kRegs];
+      float part[kDirect][kRegs];
 #pragma unroll
-      for (int i = 0; i < kWave / kWaves; ++i) {
-        const int p = i * kWaves + wave;
+      for (int i = 0; i < kDirect; ++i) {
+        const int p = i * stride + start;
         if (p >= count) break;
         const float* src = slot(p) + local * kDim;
 #pragma unroll
@@ -521,25 +526,25 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
       const float now = fmaxf(all, wave_reduce(ref, [](float a, float b) { return fmaxf(a, b); }));
       const float old = exp2_hw(all - now), alpha = exp2_hw(ref - now);
       all = now;
-      const float weighed = lane % kWaves == wave ? share * alpha : 0.0f;
+      const float weighed = direct || lane % kWaves == wave ? share * alpha : 0.0f;
       total = total * old + wave_reduce(weighed, [](float a, float b) { return a + b; });
 #pragma unroll
       for (int k = 0; k < kRegs; ++k) o[k] *= old;
 #pragma unroll
-      for (int i = 0; i < kWave / kWaves; ++i) {
-        const int p = i * kWaves + wave;
+      for (int i = 0; i < kDirect; ++i) {
+        const int p = i * stride + start;
         if (p >= count) break;
         const float a = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alpha), p));
 #pragma unroll
         for (int k = 0; k < kRegs; ++k) o[k] = __builtin_fmaf(part[i][k], a, o[k]);
       }
     }
+    if (!direct) {
 #pragma unroll
-    for (int k = 0; k < kRegs; ++k)
-      if (k * 64 + lane < kDim) s_part[wave][k * 64 + lane] = o[k];
-    if (lane == 0) s_part[wave][kDim] = total;
-    __syncthreads();
-    if (wave == 0) {
+      for (int k = 0; k < kRegs; ++k)
+        if (k * 64 + lane < kDim) s_part[wave][k * 64 + lane] = o[k];
+      if (lane == 0) s_part[wave][kDim] = total;
+      __syncthreads();
       total = 0.0f;
 #pragma unroll
       for (int k = 0; k < kRegs; ++k) o[k] = 0.0f;
@@ -547,9 +552,11 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
       for (int w = 0; w < kWaves; ++w) {
         total += s_part[w][kDim];
 #pragma unroll
-        for (int k = 0; k < kRegs; ++k)
-          if (k * 64 + lane < kDim) o[k] += s_part[w][k * 64 + lane];
+        for (int k = 0; k < kRegs; ++k) o[k] += s_part[w][min(k * 64 + lane, kDim - 1)];
       }
+      __syncthreads();
+    }
+    if (direct || wave == 0) {
       const int64_t row = item.first + token;
       const float inv = total == 0.0f ? 0.0f : 1.0f / total;
       if (args.lse != nullptr && lane == 0) args.lse[row * args.heads + qh] = log_sum(all, total);
@@ -558,7 +565,6 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
       for (int k = 0; k < kRegs; ++k)
         if (k * 64 + lane < kDim) store_out<T>(args.out, base + k * 64 + lane, o[k] * inv);
     }
-    __syncthreads();
   }
 }
 

@@ -128,6 +128,13 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
 
 __device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
+__device__ __forceinline__ float max16(const float (&x)[16]) {
+  float m = max3_op(x[0], x[1], x[2]);
+#pragma unroll
+  for (int i = 3; i < 15; i += 4) m = max5_op(m, x[i], x[i + 1], x[i + 2], x[i + 3]);
+  return fmaxf(m, x[15]);
+}
+
 template <Kv4Type T, int kDim>
 __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                             const Split& split, float* __restrict__ partial, const Cursor& at,
@@ -229,24 +236,33 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
       page = page_of(pool, batch, at.seq, u.length, key + kKeys);
     }
     const float* scales = reinterpret_cast<const float*>(now + B::kScales);
+    const v8h* keys = reinterpret_cast<const v8h*>(now) + lane;
+    const v8h* values = reinterpret_cast<const v8h*>(now + B::kKeyBytes) + lane;
+    // The 32-key steps that this wave's rows see something of.
+    const int step0 = max(0, any_low - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
 #pragma unroll 1
-    for (int st = 0; st < kKeys / 32; ++st) {
+    for (int st = step0; st < step1; ++st) {
       const int first = key0 + 32 * st;
-      if (first >= any_high || first + 32 <= any_low) continue;
-      v16f s = (v16f)(0.0f);
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i)
-        s = mfma32(reinterpret_cast<const v8h*>(now)[(st * kChunks + i) * 64 + lane], q[i], s);
-      mfma_results_fence();
-      float x[16], vs[16];
-      float top = kNegInf, most = 0.0f;
+      v4f k4[4], v4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const v4f k4 = *reinterpret_cast<const v4f*>(scales + 32 * st + 8 * i + 4 * g);
-        const v4f v4 = *reinterpret_cast<const v4f*>(scales + kKeys + 32 * st + 8 * i + 4 * g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * i + j] = s[4 * i + j] * k4[j], vs[4 * i + j] = v4[j];
+        k4[i] = *reinterpret_cast<const v4f*>(scales + 32 * st + 8 * i + 4 * g);
+        v4[i] = *reinterpret_cast<const v4f*>(scales + kKeys + 32 * st + 8 * i + 4 * g);
       }
+      v16f s = (v16f)(0.0f);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) s = mfma32(keys[(st * kChunks + i) * kWave], q[i], s);
+      // The step's values are read beside the products.
+      __builtin_amdgcn_sched_barrier(0);
+      v8h va[2][kTiles];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) va[c][t] = values[((2 * st + c) * kTiles + t) * kWave];
+      mfma_results_fence();
+      float x[16], vs[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = s[i] * k4[i / 4][i % 4], vs[i] = v4[i / 4][i % 4];
       if (!(first >= all_low && first + 32 <= all_high && args.mask == nullptr && first + 32 <= u.length) ||
           __ballot(scales[2 * kKeys + 32 * st + col] != 0.0f) != 0) {
         // A hidden key takes no part in the maxima, and its probability and
@@ -260,10 +276,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           vs[i] = see ? vs[i] : 0.0f;
         }
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]), most = fmaxf(most, vs[i]);
-      top *= factor;
-      const float product = top + __builtin_amdgcn_logf(most);
+      const float top = max16(x) * factor, product = top + __builtin_amdgcn_logf(max16(vs));
       if (__ballot(product > ref + kProductLimit || top > ref + kProbLimit) != 0) {
         const float next = fmaxf(ref, fmaxf(other_half_max(product) - kProductGoal, other_half_max(top) - kProbGoal));
         const float alpha = exp2_hw(ref - next);
@@ -273,19 +286,18 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
         for (int t = 0; t < kTiles; ++t) o[t] *= alpha;
       }
       v8h probs[2];
+      float more = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = exp2_hw(__builtin_fmaf(x[i], factor, -ref));
-        sum += p;
+        (i & 1 ? more : sum) += p;
         probs[i / 8][i % 8] = (_Float16)(p * vs[i]);
       }
+      sum += more;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const v8h a = reinterpret_cast<const v8h*>(now + B::kKeyBytes)[((2 * st + c) * kTiles + t) * 64 + lane];
-          o[t] = mfma32(a, probs[c], o[t]);
-        }
+        for (int t = 0; t < kTiles; ++t) o[t] = mfma32(va[c][t], probs[c], o[t]);
     }
     char* swap = now;
     now = other;

@@ -83,10 +83,21 @@ __device__ __forceinline__ void store8(void* p, bool wide, const float (&x)[8]) 
 // Lanes that share a row (8 elements each), a power of two.
 constexpr int row_lanes(int dim) { return dim <= 64 ? 8 : (dim <= 128 ? 16 : 32); }
 
+// Maximum over the N lanes of a row, by DPP within 16 lanes.
 template <int N>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-#pragma unroll
-  for (int i = 1; i < N; i *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, i));
+  auto step = [&](auto ctrl) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  step(std::integral_constant<int, 0xB1>{});  // quad_perm [1,0,3,2]
+  step(std::integral_constant<int, 0x4E>{});  // quad_perm [2,3,0,1]
+  if constexpr (N == 8) {
+    step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  } else {
+    step(std::integral_constant<int, 0x124>{});  // row_ror:4
+    step(std::integral_constant<int, 0x128>{});  // row_ror:8
+  }
+  if constexpr (N == 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
   return v;
 }
 
@@ -105,71 +116,129 @@ __device__ __forceinline__ bool row_slot(const Kv4Pool& pool, const Kv4Batch& ba
   return row < batch.rows && b >= 0 && kv4_slot(pool, batch, b, row, slot);
 }
 
+// Codes of a lane's eight elements, element i in nibble i.  x * (1 / s) plus 1.5 *
+// 2^23 leaves the code's two's complement nibble in the sum's last bits; where a
+// product lies so near the middle between two codes that the correctly rounded
+// quotient may round the other way, or s has no normal reciprocal, the wave
+// divides.  (Products differ from quotients by less than 2^-20; near the middle is
+// 2^-18.)  |x / s| rounds to 7 at most unless s is subnormal.
+__device__ __forceinline__ uint32_t codes8(const uint32_t (&x)[8], float s) {
+  constexpr float kMagic = 12582912.0f;
+  const float inv = __builtin_amdgcn_rcpf(s);
+  uint32_t w = 0;
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = __uint_as_float(x[i]);
+    const float t = __builtin_fmaf(v, inv, kMagic), r = t - kMagic;
+    off = fmaxf(off, fabsf(__builtin_fmaf(v, inv, -r)));
+    w |= (__float_as_uint(t) & 15u) << (4 * i);
+  }
+  if (__ballot(off > 0.5f - 0x1p-18f || s < 0x1p-125f) != 0) {
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float r = rintf(__fdiv_rn(__uint_as_float(x[i]), s));
+      w |= ((uint32_t)(int)fminf(fmaxf(r, -7.0f), 7.0f) & 15u) << (4 * i);
+    }
+  }
+  return w;
+}
+
+// A workgroup has 256 / row_lanes rows, of keys (blockIdx.y 0) or values, and
+// `heads` of their heads, kBatch at a time: the rows' slots are looked up once,
+// and what it touches of the program's memory is contiguous.
+constexpr int kBatch = 4;
+constexpr int64_t kEnoughGroups = 2048;
+
 template <Kv4Type T, int kDim>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Pool pool, Kv4Batch batch, Kv4Rows keys, Kv4Rows values,
-                                                         bool wide) {
+                                                         int heads, bool wide) {
   typedef typename Elem<T>::type E;
   constexpr int kLanes = row_lanes(kDim), kRows = 256 / kLanes;
   const int part = threadIdx.x % kLanes;
   const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
-  const int head = blockIdx.y >> 1;
-  const bool value = blockIdx.y & 1;
-  const Kv4Rows& src = value ? values : keys;
+  const int first = blockIdx.z * heads, last = min(pool.kv_heads, first + heads);
+  const Kv4Rows& src = blockIdx.y ? values : keys;
   const bool have = row < batch.rows && part * 8 < kDim;
-  uint32_t x[8] = {};
-  if (have)
-    load8<T>(static_cast<const E*>(src.ptr) + row * src.row_stride + head * src.head_stride + part * 8, wide, x);
+  const E* from = static_cast<const E*>(src.ptr) + (have ? row * src.row_stride + part * 8 : 0);
+  uint32_t x[kBatch][8];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    if (have && first + i < last) load8<T>(from + (first + i) * src.head_stride, wide, x[i]);
   Kv4Slot slot;
   const bool placed = row_slot(pool, batch, row, slot);
-  uint32_t m = 0;
+  for (int h0 = first; h0 < last; h0 += kBatch) {
+    uint32_t y[kBatch][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, x[i] & 0x7FFFFFFFu);
-  m = lanes_max<kLanes>(m);
-  // The bits pass through an empty asm, so that this stays an integer test
-  // where the compiler assumes that no value is a NaN.
-  asm volatile("" : "+v"(m));
-  const bool finite = m < 0x7F800000u;
-  float s = finite ? __fdiv_rn(__uint_as_float(m), 7.0f) : 1.0f;
-  if (s == 0.0f) s = 1.0f;
-  int c[8];
+    for (int i = 0; i < kBatch; ++i) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float r = rintf(__fdiv_rn(__uint_as_float(x[i]), s));
-    c[i] = finite ? (int)fminf(fmaxf(r, -7.0f), 7.0f) : 0;
+      for (int j = 0; j < 8; ++j) y[i][j] = have && h0 + i < last ? x[i][j] : 0;
+      if (have && h0 + kBatch + i < last) load8<T>(from + (h0 + kBatch + i) * src.head_stride, wide, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (h0 + i >= last) break;
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, y[i][j] & 0x7FFFFFFFu);
+      m = lanes_max<kLanes>(m);
+      // The bits pass through an empty asm, so that this stays an integer test
+      // where the compiler assumes that no value is a NaN.
+      asm volatile("" : "+v"(m));
+      const bool finite = m < 0x7F800000u;
+      float s = finite ? __fdiv_rn(__uint_as_float(m), 7.0f) : 1.0f;
+      if (s == 0.0f) s = 1.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[i][j] = finite ? y[i][j] : 0;
+      const uint32_t w = codes8(y[i], s);
+      if (!placed || !have) continue;
+      const int64_t at = kv4_pool_row(pool, slot.page, h0 + i, slot.slot);
+      *reinterpret_cast<uint32_t*>((blockIdx.y ? pool.codes[1] : pool.codes[0]) + at * (kDim / 2) + part * 4) = w;
+      if (part == 0)
+        reinterpret_cast<uint32_t*>(blockIdx.y ? pool.scales[1] : pool.scales[0])[at] =
+            finite ? __float_as_uint(s) : 0x7FC00000u;
+    }
   }
-  if (!placed || !have) return;
-  const int64_t at = kv4_pool_row(pool, slot.page, head, slot.slot);
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w |= (uint32_t)(c[i] & 15) << (4 * i);
-  *reinterpret_cast<uint32_t*>(pool.codes[value] + at * (kDim / 2) + part * 4) = w;
-  if (part == 0) reinterpret_cast<uint32_t*>(pool.scales[value])[at] = finite ? __float_as_uint(s) : 0x7FC00000u;
 }
 
 template <Kv4Type T, int kDim>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Pool pool, Kv4Batch batch, Kv4Rows keys, Kv4Rows values,
-                                                       bool wide) {
+                                                       int heads, bool wide) {
   typedef typename Elem<T>::type E;
   constexpr int kLanes = row_lanes(kDim), kRows = 256 / kLanes;
   const int part = threadIdx.x % kLanes;
   const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
-  const int head = blockIdx.y >> 1;
-  const bool value = blockIdx.y & 1;
-  const Kv4Rows& dst = value ? values : keys;
+  const int first = blockIdx.z * heads, last = min(pool.kv_heads, first + heads);
+  const Kv4Rows& dst = blockIdx.y ? values : keys;
   Kv4Slot slot;
   const bool placed = row_slot(pool, batch, row, slot);
   if (row >= batch.rows || part * 8 >= kDim) return;
-  uint32_t w = 0;
-  float s = 0.0f;
-  if (placed) {
-    const int64_t at = kv4_pool_row(pool, slot.page, head, slot.slot);
-    w = *reinterpret_cast<const uint32_t*>(pool.codes[value] + at * (kDim / 2) + part * 4);
-    s = pool.scales[value][at];
-  }
-  float x[8];
+  const uint8_t* codes = blockIdx.y ? pool.codes[1] : pool.codes[0];
+  const float* scales = blockIdx.y ? pool.scales[1] : pool.scales[0];
+  E* to = static_cast<E*>(dst.ptr) + row * dst.row_stride + part * 8;
+  for (int h0 = first; h0 < last; h0 += kBatch) {
+    uint32_t w[kBatch];
+    float s[kBatch];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)((int)(w << (28 - 4 * i)) >> 28) * s;
-  store8<T>(static_cast<E*>(dst.ptr) + row * dst.row_stride + head * dst.head_stride + part * 8, wide, x);
+    for (int i = 0; i < kBatch; ++i) {
+      w[i] = 0;
+      s[i] = 0.0f;
+      if (placed && h0 + i < last) {
+        const int64_t at = kv4_pool_row(pool, slot.page, h0 + i, slot.slot);
+        w[i] = *reinterpret_cast<const uint32_t*>(codes + at * (kDim / 2) + part * 4);
+        s[i] = scales[at];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (h0 + i >= last) break;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (float)((int)(w[i] << (28 - 4 * j)) >> 28) * s[i];
+      store8<T>(to + (h0 + i) * dst.head_stride, wide, x);
+    }
+  }
 }
 
 // 16-byte accesses: every row of every head starts on 16 bytes.
@@ -183,11 +252,15 @@ hipError_t launch_rows(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows
   constexpr int kRows = 256 / row_lanes(kDim);
   const int size = T == kKv4F32 ? 4 : 2;
   const bool wide = rows_aligned(rows[0], size) && rows_aligned(rows[1], size);
-  const dim3 grid((unsigned)((batch.rows + kRows - 1) / kRows), (unsigned)pool.kv_heads * 2);
+  // All heads in one workgroup, or as few as give every CU some workgroups.
+  const int64_t tiles = (batch.rows + kRows - 1) / kRows;
+  int heads = pool.kv_heads;
+  while (heads > 1 && tiles * 2 * ((pool.kv_heads + heads - 1) / heads) < kEnoughGroups) heads = (heads + 1) / 2;
+  const dim3 grid((unsigned)tiles, 2, (unsigned)((pool.kv_heads + heads - 1) / heads));
   if (append)
-    kv4_append_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], wide);
+    kv4_append_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], heads, wide);
   else
-    kv4_read_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], wide);
+    kv4_read_kernel<T, kDim><<<grid, dim3(256), 0, stream>>>(pool, batch, rows[0], rows[1], heads, wide);
   return hipGetLastError();
 }
 
