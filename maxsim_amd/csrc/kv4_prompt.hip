@@ -128,13 +128,6 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
 
 __device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
-__device__ __forceinline__ float max16(const float (&x)[16]) {
-  float m = max3_op(x[0], x[1], x[2]);
-#pragma unroll
-  for (int i = 3; i < 15; i += 4) m = max5_op(m, x[i], x[i + 1], x[i + 2], x[i + 3]);
-  return fmaxf(m, x[15]);
-}
-
 template <Kv4Type T, int kDim>
 __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                             const Split& split, float* __restrict__ partial, const Cursor& at,
@@ -276,7 +269,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           vs[i] = see ? vs[i] : 0.0f;
         }
       }
-      const float top = max16(x) * factor, product = top + __builtin_amdgcn_logf(max16(vs));
+      const float top = max_of(x) * factor, product = top + __builtin_amdgcn_logf(max_of(vs));
       if (__ballot(product > ref + kProductLimit || top > ref + kProbLimit) != 0) {
         const float next = fmaxf(ref, fmaxf(other_half_max(product) - kProductGoal, other_half_max(top) - kProbGoal));
         const float alpha = exp2_hw(ref - next);

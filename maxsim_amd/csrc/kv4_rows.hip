@@ -29,37 +29,62 @@ struct Elem<kKv4BF16> {
   typedef __bf16 type;
 };
 
-// Eight elements as single precision bits.
+// Eight elements as they lie in memory.
 template <Kv4Type T>
-__device__ __forceinline__ void load8(const void* p, bool wide, uint32_t (&x)[8]) {
-  if constexpr (T == kKv4F32) {
-    const uint32_t* u = static_cast<const uint32_t*>(p);
+struct Raw {
+  static constexpr int kWords = T == kKv4F32 ? 8 : 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const void* p, bool wide) {
     if (wide) {
-      const v4u a = reinterpret_cast<const v4u*>(u)[0], b = reinterpret_cast<const v4u*>(u)[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+      for (int i = 0; i < kWords / 4; ++i) {
+        const v4u a = static_cast<const v4u*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = a[j];
+      }
+    } else if constexpr (T == kKv4F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = static_cast<const uint32_t*>(p)[i];
     } else {
+      const uint16_t* h = static_cast<const uint16_t*>(p);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = u[i];
-    }
-  } else {
-    const uint16_t* u = static_cast<const uint16_t*>(p);
-    uint32_t w[4];
-    if (wide) {
-      const v4u a = *reinterpret_cast<const v4u*>(u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = a[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-      x[i] = T == kKv4BF16 ? (uint32_t)h << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, h));
+      for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
     }
   }
-}
+  // Element i in single precision.
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (T == kKv4F32) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (T == kKv4BF16) {
+      return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    } else {
+      return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    }
+  }
+  // Bits of the largest magnitude, in the element's own format (ordered as
+  // integers, infinities and NaNs on top).
+  __device__ __forceinline__ uint32_t peak() const {
+    if constexpr (T == kKv4F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    } else {
+      typedef uint16_t v2s __attribute__((ext_vector_type(2)));
+      v2s m = __builtin_bit_cast(v2s, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2s, w[i] & 0x7FFF7FFFu));
+      return max((uint32_t)m.x, (uint32_t)m.y);
+    }
+  }
+  static constexpr uint32_t kInfinity = T == kKv4F32 ? 0x7F800000u : (T == kKv4BF16 ? 0x7F80u : 0x7C00u);
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    if constexpr (T == kKv4F32) return __uint_as_float(bits);
+    if constexpr (T == kKv4BF16) return __uint_as_float(bits << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  }
+};
 
 // Eight single precision values stored in type T, each rounded once.
 template <Kv4Type T>
@@ -122,27 +147,30 @@ __device__ __forceinline__ bool row_slot(const Kv4Pool& pool, const Kv4Batch& ba
 // quotient may round the other way, or s has no normal reciprocal, the wave
 // divides.  (Products differ from quotients by less than 2^-20; near the middle is
 // 2^-18.)  |x / s| rounds to 7 at most unless s is subnormal.
-__device__ __forceinline__ uint32_t codes8(const uint32_t (&x)[8], float s) {
+template <Kv4Type T>
+__device__ __forceinline__ uint32_t codes8(const Raw<T>& x, float s) {
   constexpr float kMagic = 12582912.0f;
   const float inv = __builtin_amdgcn_rcpf(s);
-  uint32_t w = 0;
+  uint32_t t[8];
   float off = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float v = __uint_as_float(x[i]);
-    const float t = __builtin_fmaf(v, inv, kMagic), r = t - kMagic;
-    off = fmaxf(off, fabsf(__builtin_fmaf(v, inv, -r)));
-    w |= (__float_as_uint(t) & 15u) << (4 * i);
+    const float v = x[i], sum = __builtin_fmaf(v, inv, kMagic);
+    off = fmaxf(off, fabsf(__builtin_fmaf(v, inv, -(sum - kMagic))));
+    t[i] = __float_as_uint(sum);
   }
   if (__ballot(off > 0.5f - 0x1p-18f || s < 0x1p-125f) != 0) {
-    w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float r = rintf(__fdiv_rn(__uint_as_float(x[i]), s));
-      w |= ((uint32_t)(int)fminf(fmaxf(r, -7.0f), 7.0f) & 15u) << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i)
+      t[i] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.0f), 7.0f);
   }
-  return w;
+  // Last bytes of the even and of the odd ones, then their nibbles.
+  auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) -> uint32_t {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u),
+                                 0x05040100u);
+  };
+  const uint32_t even = bytes(t[0], t[2], t[4], t[6]), odd = bytes(t[1], t[3], t[5], t[7]);
+  return (even & 0x0F0F0F0Fu) | (odd << 4 & 0xF0F0F0F0u);
 }
 
 // A workgroup has 256 / row_lanes rows, of keys (blockIdx.y 0) or values, and
@@ -162,43 +190,37 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Pool pool, Kv4Batch 
   const Kv4Rows& src = blockIdx.y ? values : keys;
   const bool have = row < batch.rows && part * 8 < kDim;
   const E* from = static_cast<const E*>(src.ptr) + (have ? row * src.row_stride + part * 8 : 0);
-  uint32_t x[kBatch][8];
+  Raw<T> x[kBatch] = {}, next[kBatch] = {};
 #pragma unroll
   for (int i = 0; i < kBatch; ++i)
-    if (have && first + i < last) load8<T>(from + (first + i) * src.head_stride, wide, x[i]);
+    if (have && first + i < last) x[i].load(from + (first + i) * src.head_stride, wide);
   Kv4Slot slot;
   const bool placed = row_slot(pool, batch, row, slot);
+  uint8_t* codes = blockIdx.y ? pool.codes[1] : pool.codes[0];
+  float* scales = blockIdx.y ? pool.scales[1] : pool.scales[0];
   for (int h0 = first; h0 < last; h0 += kBatch) {
-    uint32_t y[kBatch][8];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[i][j] = have && h0 + i < last ? x[i][j] : 0;
-      if (have && h0 + kBatch + i < last) load8<T>(from + (h0 + kBatch + i) * src.head_stride, wide, x[i]);
-    }
+    for (int i = 0; i < kBatch; ++i)
+      if (have && h0 + kBatch + i < last) next[i].load(from + (h0 + kBatch + i) * src.head_stride, wide);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (h0 + i >= last) break;
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, y[i][j] & 0x7FFFFFFFu);
-      m = lanes_max<kLanes>(m);
+      uint32_t m = lanes_max<kLanes>(x[i].peak());
       // The bits pass through an empty asm, so that this stays an integer test
       // where the compiler assumes that no value is a NaN.
       asm volatile("" : "+v"(m));
-      const bool finite = m < 0x7F800000u;
-      float s = finite ? __fdiv_rn(__uint_as_float(m), 7.0f) : 1.0f;
+      const bool finite = m < Raw<T>::kInfinity;
+      float s = finite ? __fdiv_rn(Raw<T>::value(m), 7.0f) : 1.0f;
       if (s == 0.0f) s = 1.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[i][j] = finite ? y[i][j] : 0;
-      const uint32_t w = codes8(y[i], s);
-      if (!placed || !have) continue;
-      const int64_t at = kv4_pool_row(pool, slot.page, h0 + i, slot.slot);
-      *reinterpret_cast<uint32_t*>((blockIdx.y ? pool.codes[1] : pool.codes[0]) + at * (kDim / 2) + part * 4) = w;
-      if (part == 0)
-        reinterpret_cast<uint32_t*>(blockIdx.y ? pool.scales[1] : pool.scales[0])[at] =
-            finite ? __float_as_uint(s) : 0x7FC00000u;
+      const uint32_t w = codes8<T>(x[i], s);
+      if (placed && have) {
+        const int64_t at = kv4_pool_row(pool, slot.page, h0 + i, slot.slot);
+        *reinterpret_cast<uint32_t*>(codes + at * (kDim / 2) + part * 4) = finite ? w : 0;
+        if (part == 0) reinterpret_cast<uint32_t*>(scales)[at] = finite ? __float_as_uint(s) : 0x7FC00000u;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) x[i] = next[i];
   }
 }
 

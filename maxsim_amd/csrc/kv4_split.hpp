@@ -205,6 +205,16 @@ __device__ __forceinline__ v8h decode_word(uint32_t w) {
   return (v8h){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// The same with 72 added to every code: no subtraction, 64 + (code ^ 8) from bits
+// 4..7 of a half.
+__device__ __forceinline__ v8h decode_word_72(uint32_t w) {
+  const uint32_t p[4] = {w << 4, w, w >> 4, w >> 8};
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (p[i] & 0x00F000F0u) ^ 0x54805480u;
+  return __builtin_bit_cast(v8h, r);
+}
+
 // The order of a word's codes in decode_word's result.
 __device__ __forceinline__ constexpr int word_order(int i) { return (i & 1) * 4 + i / 2; }
 
@@ -264,6 +274,15 @@ __device__ __forceinline__ void store4(void* out, int64_t i, bool wide, v4f x) {
 // Multiplies a query row to f16's range: the exponent to add (its largest entry
 // in [2^14, 2^15)) from the bits of that entry.
 __device__ __forceinline__ int query_shift(uint32_t top) { return 141 - (int)(top >> 23); }
+
+// The maximum of 8 or 16 values, three operands at a time.
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+  float m = max3_op(x[0], x[1], x[2]);
+#pragma unroll
+  for (int i = 3; i + 4 <= N; i += 4) m = max5_op(m, x[i], x[i + 1], x[i + 2], x[i + 3]);
+  return fmaxf(m, x[N - 1]);
+}
 
 // A row of the output, and of lse, by the last sums.
 __device__ __forceinline__ float log_sum(float ref, float total) {
