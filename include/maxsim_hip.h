@@ -439,7 +439,8 @@ int msim_kv4_read_async(const msim_kv4_pool* pool, const int32_t* page_table, co
                         const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows, void* k,
                         int64_t k_row_stride, int64_t k_head_stride, void* v, int64_t v_row_stride,
                         int64_t v_head_stride, int type, void* stream);
-/* Bytes of device workspace that msim_kv4_attend_async needs for these sizes. */
+/* Bytes of device workspace that msim_kv4_attend_async needs for these sizes (0:
+ * none, NULL will do). */
 int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
                               int64_t heads, uint64_t* bytes);
 /* Attention of queries [rows, heads, dim] over the cache: head h reads key/value

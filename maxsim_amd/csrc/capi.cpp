@@ -77,9 +77,16 @@ void validate_positive_scales(const float* v, int64_t n, const char* msg) {
 int device_cu_count() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return 256;
+  // A device's count does not change: asked for once per thread and device.
+  static thread_local std::vector<int> counts;
+  if (dev < (int)counts.size() && counts[dev] > 0) return counts[dev];
   int cus = 0;
   if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     return 256;
+  if (dev >= 0) {
+    if (dev >= (int)counts.size()) counts.resize(dev + 1, 0);
+    counts[dev] = cus;
+  }
   return cus;
 }
 

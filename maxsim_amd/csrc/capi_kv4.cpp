@@ -135,7 +135,8 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     check_rows(q, t, "q");
     check_rows(out, t, "out");
     const int cus = device_cu_count();
-    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < kv4_attend_workspace(p, b, (int)heads, cus))
+    const size_t need = kv4_attend_workspace(p, b, (int)heads, cus);
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need))
       throw InvalidArgument("workspace is smaller than msim_kv4_attend_workspace asks for, or not 16-byte aligned");
     Kv4AttendArgs a{};
     a.q = q;

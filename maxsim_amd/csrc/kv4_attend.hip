@@ -657,6 +657,7 @@ size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int head
   size_t bytes = 0;
   for (Kv4Type type : {kKv4F32, kKv4BF16}) {  // f16 splits as bfloat16
     const Split s = split_for(pool, batch, heads, type, num_cus);
+    if (s.one_launch) continue;
     bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * sizeof(Unfinished));
   }
   return bytes;

@@ -33,18 +33,14 @@ from maxsim_amd import _native
 HEAD_DIMS = (64, 96, 128, 192, 256)
 
 
-def _types():
-    import torch
-
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
-_TYPES: dict = {}
+_TYPES: dict = {}  # torch dtype -> type number of the C ABI, once torch is there
 
 
 def _type_of(dtype) -> int:
     if not _TYPES:
-        _TYPES.update(_types())
+        import torch
+
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError("dtype must be float32, float16 or bfloat16")
@@ -62,27 +58,19 @@ def _cuda_device(device):
     return device
 
 
-class _on_device:
-    """Makes a device current around a launch, where it is not."""
-
-    def __init__(self, device):
-        import torch
-
-        self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
-def _raw_stream(device) -> int:
+def _launch(device, call, *args) -> None:
+    """Calls the C ABI with the current stream of `device` as the last argument,
+    that device being current."""
     import torch
 
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _native.check(status)
 
 
 class Int4KVCache:
@@ -109,6 +97,8 @@ class Int4KVCache:
             raise ValueError("page_size must be a power of two from 16 to 65536")
         self.device = _cuda_device(device)
         self._lib = _native.load()
+        self._tensor, self._int32 = torch.Tensor, torch.int32
+        self._workspaces = {}  # bytes of attend's workspace by its sizes
         shape = (num_pages, kv_heads, page_size)
         self._k_codes, self._v_codes = (torch.zeros((*shape, head_dim // 2), dtype=torch.uint8, device=self.device)
                                         for _ in range(2))
@@ -146,15 +136,8 @@ class Int4KVCache:
     def _batch(self, page_table, lengths, offsets, rows):
         """(table, lengths, offsets, batch, max_pages, rows) for the C ABI; the
         int32 tensors must be dense."""
-        import torch
-
-        for name, t, ndim in (("page_table", page_table, 2), ("lengths", lengths, 1), ("offsets", offsets, 1)):
-            if t is None and name == "offsets":
-                continue
-            if not torch.is_tensor(t) or t.dtype != torch.int32 or t.ndim != ndim or t.device != self.device:
-                raise ValueError(f"{name} must be an int32 tensor of {ndim} dimension{'s' * (ndim > 1)} on {self.device}")
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
+        self._index("page_table", page_table, 2)
+        self._index("lengths", lengths, 1)
         batch, max_pages = page_table.shape
         if lengths.shape[0] != batch:
             raise ValueError("lengths must have shape [batch]")
@@ -162,15 +145,20 @@ class Int4KVCache:
             if rows != batch:
                 raise ValueError("without offsets there must be one row per sequence")
             return page_table.data_ptr(), lengths.data_ptr(), None, batch, max_pages, rows
+        self._index("offsets", offsets, 1)
         if offsets.shape[0] != batch + 1:
             raise ValueError("offsets must have shape [batch + 1]")
         return page_table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), batch, max_pages, rows
 
+    def _index(self, name, t, ndim) -> None:
+        if not isinstance(t, self._tensor) or t.dtype != self._int32 or t.ndim != ndim or t.device != self.device:
+            raise ValueError(f"{name} must be an int32 tensor of {ndim} dimension{'s' * (ndim > 1)} on {self.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
     def _rows(self, name, t, heads=None):
         """Checks rows [rows, heads, head_dim]: any strides, dims dense."""
-        import torch
-
-        if not torch.is_tensor(t) or t.ndim != 3 or t.shape[2] != self.head_dim or \
+        if not isinstance(t, self._tensor) or t.ndim != 3 or t.shape[2] != self.head_dim or \
                 (heads is not None and t.shape[1] != heads):
             raise ValueError(f"{name} must be a tensor of shape [rows, {heads or 'heads'}, {self.head_dim}]")
         if t.device != self.device:
@@ -189,10 +177,8 @@ class Int4KVCache:
         if self._rows("v", v, self.kv_heads) != kind or v.shape[0] != k.shape[0]:
             raise ValueError("k and v must have the same shape and dtype")
         batch = self._batch(page_table, lengths, offsets, k.shape[0])
-        with _on_device(self.device):
-            _native.check(self._lib.msim_kv4_append_async(
-                self._pool_ptr, *batch, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                kind, _raw_stream(self.device)))
+        _launch(self.device, self._lib.msim_kv4_append_async, self._pool_ptr, *batch, k.data_ptr(), *k.stride()[:2],
+                v.data_ptr(), *v.stride()[:2], kind)
 
     def read(self, page_table, lengths, offsets=None, *, rows=None, dtype=None, out=None):
         """The rows (keys, values) [rows, kv_heads, head_dim] read back, each
@@ -224,10 +210,8 @@ class Int4KVCache:
             k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
                     for _ in range(2))
         batch = self._batch(page_table, lengths, offsets, k.shape[0])
-        with _on_device(self.device):
-            _native.check(self._lib.msim_kv4_read_async(
-                self._pool_ptr, *batch, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                kind, _raw_stream(self.device)))
+        _launch(self.device, self._lib.msim_kv4_read_async, self._pool_ptr, *batch, k.data_ptr(), *k.stride()[:2],
+                v.data_ptr(), *v.stride()[:2], kind)
         return k, v
 
     def attend(self, q, page_table, lengths, offsets=None, *, scale=None, causal=True, window=None, mask=None,
@@ -266,17 +250,22 @@ class Int4KVCache:
             # An empty mask has no memory: it hides every key all the same.
             mask_args = (mask.data_ptr() or self._k_scales.data_ptr(), mask.stride(0), mask.shape[1])
         if out is None:
-            out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif self._rows("out", out, heads) != kind or out.shape[0] != rows:
             raise ValueError("out must have q's shape and dtype")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        with _on_device(self.device):
-            need = ctypes.c_uint64(0)
-            _native.check(self._lib.msim_kv4_attend_workspace(self._pool_ptr, batch[3], batch[4], rows, heads,
-                                                              ctypes.byref(need)))
-            work = torch.empty(max(16, need.value), dtype=torch.uint8, device=self.device)
-            _native.check(self._lib.msim_kv4_attend_async(
-                self._pool_ptr, *batch, q.data_ptr(), q.stride(0), q.stride(1), heads, kind, scale, int(bool(causal)),
-                0 if window is None else int(window), *mask_args, out.data_ptr(), out.stride(0), out.stride(1),
-                None if lse is None else lse.data_ptr(), work.data_ptr(), work.numel(), _raw_stream(self.device)))
+        sizes = (batch[3], batch[4], rows, heads)
+        need = self._workspaces.get(sizes)
+        if need is None:
+            size = ctypes.c_uint64(0)
+            with torch.cuda.device(self.device):
+                _native.check(self._lib.msim_kv4_attend_workspace(self._pool_ptr, *sizes, ctypes.byref(size)))
+            if len(self._workspaces) >= 256:
+                self._workspaces.clear()
+            need = self._workspaces[sizes] = size.value
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _launch(self.device, self._lib.msim_kv4_attend_async, self._pool_ptr, *batch, q.data_ptr(), *q.stride()[:2],
+                heads, kind, scale, 1 if causal else 0, 0 if window is None else int(window), *mask_args,
+                out.data_ptr(), *out.stride()[:2], None if lse is None else lse.data_ptr(),
+                None if work is None else work.data_ptr(), need)
         return (out, lse) if return_lse else out

@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 
 from maxsim_amd import _native
-from maxsim_amd.kvcache import _on_device, _raw_stream, _type_of
+from maxsim_amd.kvcache import _launch, _type_of
 
 GROUP_SIZES = (32, 64, 128)
 
@@ -68,10 +68,10 @@ class Int4Linear:
         self._codes = torch.empty(sizes[0].value, dtype=torch.uint8, device=self.device)
         self._scales = torch.empty(sizes[1].value // 2, dtype=torch.bfloat16, device=self.device)
         codes, scales = codes.contiguous(), scales.contiguous()
-        with _on_device(self.device):
-            _native.check(self._lib.msim_linear4_layout_async(
-                codes.data_ptr(), scales.data_ptr(), n, k, group, self._codes.data_ptr(), self._scales.data_ptr(),
-                _raw_stream(self.device)))
+        _launch(self.device, self._lib.msim_linear4_layout_async, codes.data_ptr(), scales.data_ptr(), n, k, group,
+                self._codes.data_ptr(), self._scales.data_ptr())
+        self._matrix = (self._codes.data_ptr(), self._scales.data_ptr(), n, k, group,
+                        None if self.bias is None else self.bias.data_ptr())
 
     @classmethod
     def from_float(cls, weight, group_size: int = 128, bias=None) -> "Int4Linear":
@@ -94,20 +94,14 @@ class Int4Linear:
         if x.device != self.device:
             raise ValueError(f"x must be on {self.device}")
         kind = _type_of(x.dtype)
-        rows = x.detach()
-        if rows.ndim != 2:
-            rows = rows.reshape(-1, self.in_features)
+        rows = x if x.ndim == 2 else x.reshape(-1, self.in_features)
         if rows.stride(1) != 1:
             rows = rows.contiguous()
-        shape = (*x.shape[:-1], self.out_features)
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=self.device)
-        elif not torch.is_tensor(out) or out.shape != shape or out.dtype != x.dtype or out.device != self.device or \
-                not out.is_contiguous():
+            out = x.new_empty((*x.shape[:-1], self.out_features), requires_grad=False)
+        elif not torch.is_tensor(out) or out.shape != (*x.shape[:-1], self.out_features) or out.dtype != x.dtype or \
+                out.device != self.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor of the result's shape, x's dtype and device")
-        with _on_device(self.device):
-            _native.check(self._lib.msim_linear4_async(
-                self._codes.data_ptr(), self._scales.data_ptr(), self.out_features, self.in_features, self.group_size,
-                None if self.bias is None else self.bias.data_ptr(), rows.data_ptr(), rows.shape[0], rows.stride(0),
-                kind, out.data_ptr(), self.out_features, _raw_stream(self.device)))
+        _launch(self.device, self._lib.msim_linear4_async, *self._matrix, rows.data_ptr(), rows.shape[0],
+                rows.stride(0), kind, out.data_ptr(), self.out_features)
         return out

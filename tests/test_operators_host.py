@@ -54,7 +54,7 @@ def test_batch_checks(change, status, text):
 ])
 def test_attend_checks(change, status, text):
     pool = _pool()
-    args = [P, P, None, 3, 2, 3, P, 256, 64, 4, 0, 0.125, 1, 0, None, 0, 0, P, 256, 64, None, P, 1 << 40, None]
+    args = [P, P, None, 3, 40, 3, P, 256, 64, 4, 0, 0.125, 1, 0, None, 0, 0, P, 256, 64, None, P, 1 << 40, None]
     for i, v in change.items():
         args[i] = v
     got = _status("msim_kv4_attend_async", ctypes.addressof(pool), *args)
