@@ -82,12 +82,9 @@ __device__ __forceinline__ typename Operand<T>::type decode(uint32_t w) {
   return __builtin_bit_cast(typename Operand<T>::type, r);
 }
 
-// Eight elements of a row of x as they lie in memory (p NULL: zeros).
+// Eight elements of a row of x as they lie in memory.
 template <int kWords>
 __device__ __forceinline__ void load_x(const void* p, bool wide, uint32_t (&x)[kWords]) {
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) x[i] = 0;
-  if (p == nullptr) return;
   if (wide) {
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i) {
@@ -116,20 +113,14 @@ __device__ __forceinline__ void operands(const uint32_t (&u)[kWords],
   }
 }
 
-template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
-struct LinearTile {
-  v4u codes[kRowTiles];
-  uint32_t scales[kRowTiles][kGroups * 2];  // [group][4 rows], bfloat16
-  uint32_t x[4][kCols][T == kKv4F32 ? 8 : 4];
-};
-
+// kRowTiles tiles of 16 rows of W, kCols of 16 rows of x per workgroup.
 template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
 __global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const void* __restrict__ x, int64_t rows,
-                                                       int64_t x_row_stride, bool wide, void* __restrict__ out,
-                                                       int64_t out_row_stride) {
-  typedef LinearTile<T, kGroups, kCols, kRowTiles> Tile;
+                                                      int64_t x_row_stride, bool wide, void* __restrict__ out,
+                                                      int64_t out_row_stride) {
   constexpr int kParts = Operand<T>::kParts;
   constexpr int kSize = T == kKv4F32 ? 4 : 2;
+  typedef uint32_t XTile[4][kCols][T == kKv4F32 ? 8 : 4];
   extern __shared__ float s_acc[];
   const int lane = lane_id(), col = lane % 16, g = lane / 16;
   const int wave = wave_uniform(threadIdx.x / kWave), waves = blockDim.x / kWave;
@@ -137,24 +128,29 @@ __global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const voi
   const int n0 = blockIdx.x * kRowTiles;
   const int64_t m0 = (int64_t)blockIdx.y * 16 * kCols;
 
-  auto load = [&](int kt, Tile& t) {
+  auto load_w = [&](int kt, v4u (&codes)[kRowTiles], uint32_t (&scales)[kRowTiles][kGroups * 2]) {
 #pragma unroll
     for (int r = 0; r < kRowTiles; ++r) {
       const int64_t tile = (int64_t)min(n0 + r, tiles_n - 1) * tiles_k + kt;
-      t.codes[r] = reinterpret_cast<const v4u*>(w.codes)[tile * kWave + lane];
+      codes[r] = reinterpret_cast<const v4u*>(w.codes)[tile * kWave + lane];
       const uint32_t* s = reinterpret_cast<const uint32_t*>(w.scales) + (tile * 4 + g) * kGroups * 2;
 #pragma unroll
-      for (int i = 0; i < kGroups * 2; ++i) t.scales[r][i] = s[i];
+      for (int i = 0; i < kGroups * 2; ++i) scales[r][i] = s[i];
     }
+  };
+  // Rows past the last are the last one again (their columns of the result are
+  // not written), columns past the last the last ones (their codes and scales are
+  // zeros).
+  const char* xrow[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; ++j)
+    xrow[j] = static_cast<const char*>(x) + (min(m0 + 16 * j + col, rows - 1) * x_row_stride + 8 * g) * kSize;
+  auto load_rows = [&](int kt, XTile& t) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int k = kt * 128 + 32 * c + 8 * g;
+      const int k = min(kt * 128 + 32 * c, w.k - 32);
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int64_t m = m0 + 16 * j + col;
-        const bool have = m < rows && k < w.k;
-        load_x(have ? static_cast<const char*>(x) + (m * x_row_stride + k) * kSize : nullptr, wide, t.x[c][j]);
-      }
+      for (int j = 0; j < kCols; ++j) load_x(xrow[j] + (int64_t)k * kSize, wide, t[c][j]);
     }
   };
 
@@ -164,17 +160,13 @@ __global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const voi
 #pragma unroll
     for (int j = 0; j < kCols; ++j) acc[r][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-  int kt = wave;
-  Tile tile;
-  if (kt < tiles_k) load(kt, tile);
-  for (; kt < tiles_k; kt += waves) {
-    Tile next;
-    if (kt + waves < tiles_k) load(kt + waves, next);
+  auto multiply = [&](const v4u (&codes)[kRowTiles], const uint32_t (&scales)[kRowTiles][kGroups * 2],
+                      const XTile& t) {
     typename Operand<T>::type b[4][kCols][kParts];
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) operands<T>(tile.x[c][j], b[c][j]);
+      for (int j = 0; j < kCols; ++j) operands<T>(t[c][j], b[c][j]);
     v4f start[kGroups][kCols];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
@@ -188,35 +180,64 @@ __global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const voi
             start[i][j] = mfma(__builtin_bit_cast(v8b, offset), b[c][j][0], start[i][j]);
         }
       }
-    v4f sum[kRowTiles][kGroups][kCols];
-#pragma unroll
-    for (int r = 0; r < kRowTiles; ++r)
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) sum[r][i][j] = start[i][j];
-#pragma unroll
-        for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c) {
-          const typename Operand<T>::type a = decode<T>(tile.codes[r][c]);
-#pragma unroll
-          for (int j = 0; j < kCols; ++j)
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) sum[r][i][j] = mfma(a, b[c][j][p], sum[r][i][j]);
-        }
-      }
-    mfma_results_fence();
-#pragma unroll
-    for (int r = 0; r < kRowTiles; ++r)
+    // A row tile's sums meet their scales one row tile later, behind the next
+    // one's decoding and products: MFMA results are not read right after they are
+    // issued.
+    v4f sum[2][kGroups][kCols];
+    auto scale = [&](int r) {
 #pragma unroll
       for (int i = 0; i < kGroups; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t s2 = tile.scales[r][i * 2 + e / 2];
+          const uint32_t s2 = scales[r][i * 2 + e / 2];
           const float s = __uint_as_float(e & 1 ? s2 & 0xFFFF0000u : s2 << 16);
 #pragma unroll
-          for (int j = 0; j < kCols; ++j) acc[r][j][e] = __builtin_fmaf(s, sum[r][i][j][e], acc[r][j][e]);
+          for (int j = 0; j < kCols; ++j) acc[r][j][e] = __builtin_fmaf(s, sum[r % 2][i][j][e], acc[r][j][e]);
         }
-    tile = next;
+    };
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) sum[r % 2][i][j] = start[i][j];
+#pragma unroll
+        for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c) {
+          const typename Operand<T>::type a = decode<T>(codes[r][c]);
+#pragma unroll
+          for (int j = 0; j < kCols; ++j)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) sum[r % 2][i][j] = mfma(a, b[c][j][p], sum[r % 2][i][j]);
+        }
+      }
+      if (r == 0) continue;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) asm volatile("" : "+v"(sum[0][i][j]), "+v"(sum[1][i][j]));
+      scale(r - 1);
+    }
+    mfma_results_fence();
+    scale(kRowTiles - 1);
+  };
+
+  v4u codes[kRowTiles];
+  uint32_t scales[kRowTiles][kGroups * 2];
+  XTile now, next;
+  if (wave < tiles_k) {
+    load_rows(wave, now);
+    load_w(wave, codes, scales);
+  }
+  for (int kt = wave; kt < tiles_k; kt += waves) {
+    if (kt + waves < tiles_k) load_rows(kt + waves, next);
+    multiply(codes, scales, now);
+    if (kt + waves < tiles_k) load_w(kt + waves, codes, scales);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+#pragma unroll
+        for (int i = 0; i < (T == kKv4F32 ? 8 : 4); ++i) now[c][j][i] = next[c][j][i];
   }
 
   // [wave][row tile][column tile][element][lane]
@@ -255,22 +276,50 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
   // that joins them.
   const int tiles_k = (w.k + 127) / 128;
   int waves = 4;
-  while (waves < 8 && waves * 2 <= tiles_k && waves * 2 * kRowTiles * kCols <= 32 && gx * gy * waves < num_cus * 8)
-    waves *= 2;
+  while (waves < 8 && waves * 2 <= tiles_k && gx * gy * waves < num_cus * 8) waves *= 2;
   const size_t lds = sizeof(float) * waves * kRowTiles * kCols * 4 * kWave;
   linear4_kernel<T, kGroups, kCols, kRowTiles><<<dim3((unsigned)gx, (unsigned)gy), dim3(waves * kWave), lds, stream>>>(
       w, x, rows, x_row_stride, wide, out, out_row_stride);
   return hipGetLastError();
 }
 
+// Row tiles that the registers hold without spilling.
+constexpr int most_row_tiles(Kv4Type type, int groups, int cols) {
+  if (groups * cols >= 8 || (type == kKv4F32 && cols > 1)) return 2;
+  return groups * cols >= 4 ? 4 : 7;
+}
+
+template <Kv4Type T, int kGroups, int kCols>
+hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
+                          int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  // Row tiles of a workgroup: the busiest CU has its workgroups' row tiles to do,
+  // and with each workgroup the rows of x, whose loads (16 rows apart) cost as
+  // much as two row tiles; one row costs half of one.
+  const int64_t tiles = (w.n + 15) / 16, columns = (rows + 16 * kCols - 1) / (16 * kCols);
+  auto cost = [&](int row_tiles) -> int64_t {
+    const int64_t groups = (tiles + row_tiles - 1) / row_tiles * columns;
+    return (groups + num_cus - 1) / num_cus * (2 * row_tiles + (rows > 1 ? 4 * kCols : 1));
+  };
+  constexpr int kMost = most_row_tiles(T, kGroups, kCols);
+  int best = 1;
+  for (int row_tiles : {2, 4, 7})
+    if (row_tiles <= kMost && cost(row_tiles) <= cost(best)) best = row_tiles;
+  if constexpr (kMost >= 7)
+    if (best == 7)
+      return launch_shape<T, kGroups, kCols, 7>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  if constexpr (kMost >= 4)
+    if (best == 4)
+      return launch_shape<T, kGroups, kCols, 4>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  if (best == 2)
+    return launch_shape<T, kGroups, kCols, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  return launch_shape<T, kGroups, kCols, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+}
+
 template <Kv4Type T, int kGroups>
 hipError_t launch_group(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
                         int64_t out_row_stride, int num_cus, hipStream_t stream) {
-  if (rows <= 4) return launch_shape<T, kGroups, 1, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
-  if (rows <= 16) return launch_shape<T, kGroups, 1, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
-  // Two column tiles of single precision parts leave registers for one row tile.
-  constexpr int kRowTiles = T == kKv4F32 ? 1 : 2;
-  return launch_shape<T, kGroups, 2, kRowTiles>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  if (rows <= 16) return launch_columns<T, kGroups, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  return launch_columns<T, kGroups, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
 }
 
 template <Kv4Type T>
