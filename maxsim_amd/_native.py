@@ -180,6 +180,29 @@ def load():
     return lib
 
 
+_calls = None
+
+
+def tensor_calls():
+    """The calls on torch tensors (binding/tensor_calls.cpp), over the loaded library."""
+    global _calls
+    if _calls is not None:
+        return _calls
+    import torch  # noqa: F401  (its libraries come first)
+
+    lib = load()
+    try:
+        from maxsim_amd import _tensor_calls
+    except ImportError as exc:
+        raise NativeLibraryMissing(
+            f"{os.path.join(HERE, '_tensor_calls.so')} is not built; run `python -m maxsim_amd.build`") from exc
+    names = ("msim_last_error", "msim_kv4_append_async", "msim_kv4_read_async", "msim_kv4_attend_workspace",
+             "msim_kv4_attend_async", "msim_linear4_async")
+    _tensor_calls.setup(*(ctypes.cast(getattr(lib, name), c_vp).value for name in names))
+    _calls = _tensor_calls
+    return _calls
+
+
 def check(status: int) -> None:
     """Raise the Python exception matching a C ABI status code."""
     if status == MSIM_OK:

@@ -2,13 +2,15 @@
 
 Usage: ``python -m maxsim_amd.build`` (also called by ``__graft_entry__.build``).
 Compiles every source under ``maxsim_amd/csrc`` with hipcc (one process per
-source, in parallel), then links them into the library.
+source, in parallel), then links them into the library; beside it the Python
+module ``maxsim_amd/_tensor_calls.so`` (calls on torch tensors, with g++).
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -42,6 +44,25 @@ FLAGS = [
 ]
 
 
+# The calls on torch tensors: a Python module of its own beside the library.
+BINDING_SRC = os.path.join(HERE, "binding", "tensor_calls.cpp")
+BINDING = os.path.join(HERE, "_tensor_calls.so")
+
+
+def binding_command(out: str) -> list[str]:
+    import torch
+
+    home = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    includes = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
+    # The two definitions choose HIP in its own and in torch's headers.
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+            *(f"-I{path}" for path in includes), BINDING_SRC, "-o", out, f"-L{os.path.join(home, 'lib')}", "-ltorch",
+            "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python"]
+
+
 def sources() -> list[str]:
     names = sorted(os.listdir(CSRC))
     return [os.path.join(CSRC, n) for n in names if n.endswith((".hip", ".cpp"))]
@@ -65,12 +86,14 @@ def build(verbose: bool = False) -> str:
             print(f"compiling {len(srcs)} sources with {jobs} jobs: " + " ".join(cmds[0][:-4]), flush=True)
         rates_tmp = RATES_LIB + ".tmp"
         cmds.append([hipcc, *FLAGS, RATES_SRC, "-o", rates_tmp])
+        binding_tmp = BINDING + ".tmp"
+        cmds.append(binding_command(binding_tmp))
         with ThreadPoolExecutor(max_workers=jobs) as pool:
             results = list(pool.map(_run, cmds))
         messages: list[str] = []
-        for src, (rc, lines) in zip(srcs + [RATES_SRC], results):
+        for src, (rc, lines) in zip(srcs + [RATES_SRC, BINDING_SRC], results):
             if rc != 0:
-                raise RuntimeError(f"hipcc failed on {os.path.basename(src)}:\n" + "\n".join(lines))
+                raise RuntimeError(f"compiler failed on {os.path.basename(src)}:\n" + "\n".join(lines))
             messages.extend(lines)
         tmp = LIB + ".tmp"
         rc, lines = _run([hipcc, *FLAGS, *objs, "-o", tmp])
@@ -81,6 +104,7 @@ def build(verbose: bool = False) -> str:
         print("\n".join(messages))
     os.replace(tmp, LIB)
     os.replace(rates_tmp, RATES_LIB)
+    os.replace(binding_tmp, BINDING)
     return LIB
 
 

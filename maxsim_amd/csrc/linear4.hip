@@ -113,9 +113,14 @@ __device__ __forceinline__ void operands(const uint32_t (&u)[kWords],
   }
 }
 
+// Waves of a workgroup, by their registers.
+constexpr int most_waves(Kv4Type type, int groups, int cols, int row_tiles) {
+  return type != kKv4F32 && cols == 1 && groups * row_tiles <= 4 ? 16 : 8;
+}
+
 // kRowTiles tiles of 16 rows of W, kCols of 16 rows of x per workgroup.
 template <Kv4Type T, int kGroups, int kCols, int kRowTiles>
-__global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const void* __restrict__ x, int64_t rows,
+__global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) void linear4_kernel(Linear4Matrix w, const void* __restrict__ x, int64_t rows,
                                                       int64_t x_row_stride, bool wide, void* __restrict__ out,
                                                       int64_t out_row_stride) {
   constexpr int kParts = Operand<T>::kParts;
@@ -221,23 +226,33 @@ __global__ __launch_bounds__(512) void linear4_kernel(Linear4Matrix w, const voi
     scale(kRowTiles - 1);
   };
 
-  v4u codes[kRowTiles];
-  uint32_t scales[kRowTiles][kGroups * 2];
-  XTile now, next;
+  // The next tile of x is on its way during a tile's products, and the next tiles
+  // of W too where the registers hold them.
+  constexpr bool kBoth = kRowTiles <= 4 && kGroups * kCols * kRowTiles <= 8 && (T != kKv4F32 || kCols == 1);
+  constexpr bool kRowsAhead = T != kKv4F32 || kCols == 1;
+  v4u codes[kBoth ? 2 : 1][kRowTiles];
+  uint32_t scales[kBoth ? 2 : 1][kRowTiles][kGroups * 2];
+  XTile xs[2];
   if (wave < tiles_k) {
-    load_rows(wave, now);
-    load_w(wave, codes, scales);
+    if constexpr (kRowsAhead) load_rows(wave, xs[0]);
+    load_w(wave, codes[0], scales[0]);
   }
-  for (int kt = wave; kt < tiles_k; kt += waves) {
-    if (kt + waves < tiles_k) load_rows(kt + waves, next);
-    multiply(codes, scales, now);
-    if (kt + waves < tiles_k) load_w(kt + waves, codes, scales);
+  for (int k0 = wave; k0 < tiles_k; k0 += 2 * waves) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int j = 0; j < kCols; ++j)
-#pragma unroll
-        for (int i = 0; i < (T == kKv4F32 ? 8 : 4); ++i) now[c][j][i] = next[c][j][i];
+    for (int d = 0; d < 2; ++d) {
+      const int kt = k0 + d * waves;
+      if (kt >= tiles_k) break;
+      const bool more = kt + waves < tiles_k;
+      if constexpr (!kRowsAhead) load_rows(kt, xs[d]);
+      if (kRowsAhead && more) load_rows(kt + waves, xs[1 - d]);
+      if constexpr (kBoth) {
+        if (more) load_w(kt + waves, codes[1 - d], scales[1 - d]);
+        multiply(codes[d], scales[d], xs[d]);
+      } else {
+        multiply(codes[0], scales[0], xs[d]);
+        if (more) load_w(kt + waves, codes[0], scales[0]);
+      }
+    }
   }
 
   // [wave][row tile][column tile][element][lane]
@@ -276,7 +291,8 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
   // that joins them.
   const int tiles_k = (w.k + 127) / 128;
   int waves = 4;
-  while (waves < 8 && waves * 2 <= tiles_k && gx * gy * waves < num_cus * 8) waves *= 2;
+  while (waves < most_waves(T, kGroups, kCols, kRowTiles) && waves * 2 <= tiles_k && gx * gy * waves < num_cus * 16)
+    waves *= 2;
   const size_t lds = sizeof(float) * waves * kRowTiles * kCols * 4 * kWave;
   linear4_kernel<T, kGroups, kCols, kRowTiles><<<dim3((unsigned)gx, (unsigned)gy), dim3(waves * kWave), lds, stream>>>(
       w, x, rows, x_row_stride, wide, out, out_row_stride);
@@ -285,8 +301,9 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
 
 // Row tiles that the registers hold without spilling.
 constexpr int most_row_tiles(Kv4Type type, int groups, int cols) {
-  if (groups * cols >= 8 || (type == kKv4F32 && cols > 1)) return 2;
-  return groups * cols >= 4 ? 4 : 7;
+  if (type == kKv4F32 && cols > 1) return 1;
+  if (groups * cols >= 8) return 2;
+  return groups * cols >= 4 || (type == kKv4F32 && groups > 1) ? 4 : 7;
 }
 
 template <Kv4Type T, int kGroups, int kCols>
@@ -310,8 +327,9 @@ hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, i
   if constexpr (kMost >= 4)
     if (best == 4)
       return launch_shape<T, kGroups, kCols, 4>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
-  if (best == 2)
-    return launch_shape<T, kGroups, kCols, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  if constexpr (kMost >= 2)
+    if (best == 2)
+      return launch_shape<T, kGroups, kCols, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
   return launch_shape<T, kGroups, kCols, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
 }
 

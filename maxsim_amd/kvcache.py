@@ -25,26 +25,9 @@ attention).  ``append`` and ``attend`` can be captured in a HIP graph.
 """
 from __future__ import annotations
 
-import ctypes
-import math
-
 from maxsim_amd import _native
 
 HEAD_DIMS = (64, 96, 128, 192, 256)
-
-
-_TYPES: dict = {}  # torch dtype -> type number of the C ABI, once torch is there
-
-
-def _type_of(dtype) -> int:
-    if not _TYPES:
-        import torch
-
-        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-    kind = _TYPES.get(dtype)
-    if kind is None:
-        raise ValueError("dtype must be float32, float16 or bfloat16")
-    return kind
 
 
 def _cuda_device(device):
@@ -58,19 +41,17 @@ def _cuda_device(device):
     return device
 
 
-def _launch(device, call, *args) -> None:
-    """Calls the C ABI with the current stream of `device` as the last argument,
-    that device being current."""
+def _type_number(dtype) -> int:
+    """The C ABI's number of an element type (None: bfloat16)."""
     import torch
 
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _native.check(status)
+    if dtype is None or dtype is torch.bfloat16:
+        return 2
+    if dtype is torch.float16:
+        return 1
+    if dtype is torch.float32:
+        return 0
+    raise ValueError("dtype must be float32, float16 or bfloat16")
 
 
 class Int4KVCache:
@@ -96,18 +77,14 @@ class Int4KVCache:
         if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two from 16 to 65536")
         self.device = _cuda_device(device)
-        self._lib = _native.load()
-        self._tensor, self._int32 = torch.Tensor, torch.int32
-        self._workspaces = {}  # bytes of attend's workspace by its sizes
+        self._calls = _native.tensor_calls()
         shape = (num_pages, kv_heads, page_size)
         self._k_codes, self._v_codes = (torch.zeros((*shape, head_dim // 2), dtype=torch.uint8, device=self.device)
                                         for _ in range(2))
         self._k_scales, self._v_scales = (torch.zeros(shape, dtype=torch.float32, device=self.device)
                                           for _ in range(2))
         self.num_pages, self.kv_heads, self.head_dim, self.page_size = num_pages, kv_heads, head_dim, page_size
-        self._pool = _native.Kv4Pool(self._k_codes.data_ptr(), self._k_scales.data_ptr(), self._v_codes.data_ptr(),
-                                     self._v_scales.data_ptr(), num_pages, kv_heads, page_size, head_dim)
-        self._pool_ptr = ctypes.addressof(self._pool)
+        self._handle = self._calls.cache(self._k_codes, self._k_scales, self._v_codes, self._v_scales)
 
     @property
     def k_codes(self):
@@ -131,88 +108,29 @@ class Int4KVCache:
         return sum(t.numel() * t.element_size() for t in (self._k_codes, self._v_codes, self._k_scales,
                                                           self._v_scales))
 
-    # ------------------------------------------------------------- arguments
-
-    def _batch(self, page_table, lengths, offsets, rows):
-        """(table, lengths, offsets, batch, max_pages, rows) for the C ABI; the
-        int32 tensors must be dense."""
-        self._index("page_table", page_table, 2)
-        self._index("lengths", lengths, 1)
-        batch, max_pages = page_table.shape
-        if lengths.shape[0] != batch:
-            raise ValueError("lengths must have shape [batch]")
-        if offsets is None:
-            if rows != batch:
-                raise ValueError("without offsets there must be one row per sequence")
-            return page_table.data_ptr(), lengths.data_ptr(), None, batch, max_pages, rows
-        self._index("offsets", offsets, 1)
-        if offsets.shape[0] != batch + 1:
-            raise ValueError("offsets must have shape [batch + 1]")
-        return page_table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), batch, max_pages, rows
-
-    def _index(self, name, t, ndim) -> None:
-        if not isinstance(t, self._tensor) or t.dtype != self._int32 or t.ndim != ndim or t.device != self.device:
-            raise ValueError(f"{name} must be an int32 tensor of {ndim} dimension{'s' * (ndim > 1)} on {self.device}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-
-    def _rows(self, name, t, heads=None):
-        """Checks rows [rows, heads, head_dim]: any strides, dims dense."""
-        if not isinstance(t, self._tensor) or t.ndim != 3 or t.shape[2] != self.head_dim or \
-                (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name} must be a tensor of shape [rows, {heads or 'heads'}, {self.head_dim}]")
-        if t.device != self.device:
-            raise ValueError(f"{name} must be on {self.device}")
-        if t.stride(2) != 1 and t.numel() > 0:
-            raise ValueError(f"{name} must be dense in its last dimension")
-        return _type_of(t.dtype)
-
     # ----------------------------------------------------------------- calls
 
     def append(self, k, v, page_table, lengths, offsets=None) -> None:
         """Quantise keys and values [rows, kv_heads, head_dim] (float32, float16
         or bfloat16, any strides with dense rows) into the cache.  A row that
         holds an infinity or a NaN reads back as NaN."""
-        kind = self._rows("k", k, self.kv_heads)
-        if self._rows("v", v, self.kv_heads) != kind or v.shape[0] != k.shape[0]:
-            raise ValueError("k and v must have the same shape and dtype")
-        batch = self._batch(page_table, lengths, offsets, k.shape[0])
-        _launch(self.device, self._lib.msim_kv4_append_async, self._pool_ptr, *batch, k.data_ptr(), *k.stride()[:2],
-                v.data_ptr(), *v.stride()[:2], kind)
+        self._calls.append(self._handle, k, v, page_table, lengths, offsets)
 
     def read(self, page_table, lengths, offsets=None, *, rows=None, dtype=None, out=None):
         """The rows (keys, values) [rows, kv_heads, head_dim] read back, each
         value code * scale rounded once to ``dtype`` (default bfloat16).  ``rows``
         is their number; without it, and with offsets, the last offset is fetched
         from the device.  ``out`` is a pair of tensors to write."""
-        import torch
-
         if out is not None:
             k, v = out
-            kind = self._rows("out[0]", k, self.kv_heads)
-            if self._rows("out[1]", v, self.kv_heads) != kind or v.shape[0] != k.shape[0]:
-                raise ValueError("both outputs must have the same shape and dtype")
             if (rows is not None and int(rows) != k.shape[0]) or (dtype is not None and dtype != k.dtype):
                 raise ValueError("rows and dtype must be those of out")
-        else:
-            dtype = torch.bfloat16 if dtype is None else dtype
-            kind = _type_of(dtype)
-            if rows is None:
-                if offsets is not None:
-                    if not torch.is_tensor(offsets) or offsets.ndim != 1 or offsets.shape[0] < 1:
-                        raise ValueError("offsets must have shape [batch + 1]")
-                    rows = int(offsets[-1])
-                else:
-                    rows = lengths.shape[0]
-            rows = int(rows)
-            if rows < 0:
-                raise ValueError("rows must not be negative")
-            k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-                    for _ in range(2))
-        batch = self._batch(page_table, lengths, offsets, k.shape[0])
-        _launch(self.device, self._lib.msim_kv4_read_async, self._pool_ptr, *batch, k.data_ptr(), *k.stride()[:2],
-                v.data_ptr(), *v.stride()[:2], kind)
-        return k, v
+            return self._calls.read(self._handle, page_table, lengths, offsets, 0, 0, k, v)
+        if rows is None:
+            if offsets is not None and (offsets.ndim != 1 or offsets.shape[0] < 1):
+                raise ValueError("offsets must have shape [batch + 1]")
+            rows = lengths.shape[0] if offsets is None else int(offsets[-1])
+        return self._calls.read(self._handle, page_table, lengths, offsets, rows, _type_number(dtype), None, None)
 
     def attend(self, q, page_table, lengths, offsets=None, *, scale=None, causal=True, window=None, mask=None,
                out=None, return_lse=False):
@@ -228,44 +146,8 @@ class Int4KVCache:
         of each softmax's sum, float32 [rows, heads].  A row that sees nothing
         is zeros, with minus infinity.
         """
-        import torch
-
-        kind = self._rows("q", q)
-        rows, heads = q.shape[0], q.shape[1]
-        if heads < 1 or heads % self.kv_heads:
-            raise ValueError("heads must be a multiple of kv_heads")
-        batch = self._batch(page_table, lengths, offsets, rows)
-        scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError("scale must be finite")
-        if window is not None and int(window) < 1:
+        if window is not None and window < 1:
             raise ValueError("window must be positive")
-        mask_args = (None, 0, 0)
-        if mask is not None:
-            if not torch.is_tensor(mask) or mask.dtype != torch.bool or mask.ndim != 2 or mask.shape[0] != rows or \
-                    mask.device != self.device:
-                raise ValueError(f"mask must be a bool tensor of shape [rows, width] on {self.device}")
-            if mask.shape[1] > 1 and mask.stride(1) != 1:
-                raise ValueError("mask must be dense in its last dimension")
-            # An empty mask has no memory: it hides every key all the same.
-            mask_args = (mask.data_ptr() or self._k_scales.data_ptr(), mask.stride(0), mask.shape[1])
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif self._rows("out", out, heads) != kind or out.shape[0] != rows:
-            raise ValueError("out must have q's shape and dtype")
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        sizes = (batch[3], batch[4], rows, heads)
-        need = self._workspaces.get(sizes)
-        if need is None:
-            size = ctypes.c_uint64(0)
-            with torch.cuda.device(self.device):
-                _native.check(self._lib.msim_kv4_attend_workspace(self._pool_ptr, *sizes, ctypes.byref(size)))
-            if len(self._workspaces) >= 256:
-                self._workspaces.clear()
-            need = self._workspaces[sizes] = size.value
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _launch(self.device, self._lib.msim_kv4_attend_async, self._pool_ptr, *batch, q.data_ptr(), *q.stride()[:2],
-                heads, kind, scale, 1 if causal else 0, 0 if window is None else int(window), *mask_args,
-                out.data_ptr(), *out.stride()[:2], None if lse is None else lse.data_ptr(),
-                None if work is None else work.data_ptr(), need)
-        return (out, lse) if return_lse else out
+        return self._calls.attend(self._handle, q, page_table, lengths, offsets,
+                                  self.head_dim ** -0.5 if scale is None else scale, causal, window or 0, mask, out,
+                                  bool(return_lse))

@@ -11,7 +11,6 @@ from __future__ import annotations
 import ctypes
 
 from maxsim_amd import _native
-from maxsim_amd.kvcache import _launch, _type_of
 
 GROUP_SIZES = (32, 64, 128)
 
@@ -62,16 +61,18 @@ class Int4Linear:
             raise ValueError("bias must be a float tensor of shape [out_features] on the device of codes")
         self.out_features, self.in_features, self.group_size, self.device = n, k, group, codes.device
         self.bias = None if bias is None else bias.detach().to(torch.float32).contiguous()
-        self._lib = _native.load()
+        lib = _native.load()
         sizes = ctypes.c_uint64(0), ctypes.c_uint64(0)
-        _native.check(self._lib.msim_linear4_layout_bytes(n, k, group, *map(ctypes.byref, sizes)))
+        _native.check(lib.msim_linear4_layout_bytes(n, k, group, *map(ctypes.byref, sizes)))
         self._codes = torch.empty(sizes[0].value, dtype=torch.uint8, device=self.device)
         self._scales = torch.empty(sizes[1].value // 2, dtype=torch.bfloat16, device=self.device)
         codes, scales = codes.contiguous(), scales.contiguous()
-        _launch(self.device, self._lib.msim_linear4_layout_async, codes.data_ptr(), scales.data_ptr(), n, k, group,
-                self._codes.data_ptr(), self._scales.data_ptr())
-        self._matrix = (self._codes.data_ptr(), self._scales.data_ptr(), n, k, group,
-                        None if self.bias is None else self.bias.data_ptr())
+        with torch.cuda.device(self.device):
+            _native.check(lib.msim_linear4_layout_async(
+                codes.data_ptr(), scales.data_ptr(), n, k, group, self._codes.data_ptr(), self._scales.data_ptr(),
+                torch.cuda.current_stream().cuda_stream))
+        self._calls = _native.tensor_calls()
+        self._handle = self._calls.linear(self._codes, self._scales, self.bias, n, k, group)
 
     @classmethod
     def from_float(cls, weight, group_size: int = 128, bias=None) -> "Int4Linear":
@@ -87,21 +88,4 @@ class Int4Linear:
         out_features] in x's dtype: sums in single precision, rounded once.
         Enqueued on the current stream; records no gradients.  Meant for few
         rows: the matrix is read once per 32 of them."""
-        import torch
-
-        if not torch.is_tensor(x) or x.ndim < 1 or x.shape[-1] != self.in_features:
-            raise ValueError(f"x must be a tensor of shape [..., {self.in_features}]")
-        if x.device != self.device:
-            raise ValueError(f"x must be on {self.device}")
-        kind = _type_of(x.dtype)
-        rows = x if x.ndim == 2 else x.reshape(-1, self.in_features)
-        if rows.stride(1) != 1:
-            rows = rows.contiguous()
-        if out is None:
-            out = x.new_empty((*x.shape[:-1], self.out_features), requires_grad=False)
-        elif not torch.is_tensor(out) or out.shape != (*x.shape[:-1], self.out_features) or out.dtype != x.dtype or \
-                out.device != self.device or not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor of the result's shape, x's dtype and device")
-        _launch(self.device, self._lib.msim_linear4_async, *self._matrix, rows.data_ptr(), rows.shape[0],
-                rows.stride(0), kind, out.data_ptr(), self.out_features)
-        return out
+        return self._calls.multiply(self._handle, x, out)
