@@ -49,7 +49,8 @@ constexpr int attend_lds(int dim, int cols) {
 
 // Workgroups of 4 waves that a CU holds by their registers.
 constexpr int waves_per_simd(Kv4Type type, int dim, int cols) {
-  return type == kKv4F32 || dim > 128 || cols > 1 ? (dim > 192 || (type == kKv4F32 && dim * cols > 192) ? 1 : 2) : 3;
+  if (dim <= 128 && cols == 1) return 3;
+  return type == kKv4F32 && dim > 192 ? 1 : 2;
 }
 // ------------------------------------------------------------ the main kernel
 
@@ -154,24 +155,71 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   v4f start[kCols];
   int see_low[kCols], see_high[kCols];
   const uint8_t* mask[kCols];
+  int64_t query[kCols];  // first element of the lane's row; -1: a row of padding
   int all_low = 0, all_high = INT_MAX, any_low = INT_MAX, any_high = 0;
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
     const uint32_t r = tile * kRows + 16 * c + col;
     const int token = (int)(r / split.share), sub = (int)(r - token * split.share);
     const bool have = token < u.rows;
-    const int64_t base = have ? (int64_t)(u.first + token) * args.q_row_stride +
-                                    (int64_t)(head * split.share + sub) * args.q_head_stride
-                              : 0;
+    query[c] = have ? (int64_t)(u.first + token) * args.q_row_stride +
+                          (int64_t)(head * split.share + sub) * args.q_head_stride
+                    : -1;
+    const int pos = u.length - u.rows + token;
+    see_low[c] = pos >= args.window ? pos - args.window + 1 : 0;
+    see_high[c] = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
+    mask[c] = nullptr;
+    if (args.mask != nullptr) {
+      see_high[c] = (int)min((int64_t)see_high[c], args.mask_width);
+      mask[c] = args.mask + (have ? (int64_t)(u.first + token) * args.mask_row_stride : 0);
+    }
+    if (!have) {  // nothing depends on what it sees
+      see_low[c] = 0;
+      see_high[c] = args.mask != nullptr ? 0 : INT_MAX;
+    } else if (see_high[c] > see_low[c]) {
+      any_low = min(any_low, see_low[c]);
+      any_high = max(any_high, see_high[c]);
+    }
+    all_low = max(all_low, see_low[c]);
+    all_high = min(all_high, see_high[c]);
+  }
+  all_low = wave_reduce(all_low, [](int a, int b) { return max(a, b); });
+  all_high = wave_reduce(all_high, [](int a, int b) { return min(a, b); });
+  any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
+  any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
+  // This worker's keys of the item, cut to what some row sees.
+  const int begin = max(at.range.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
+  const int end = (int)min((int64_t)at.range.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
+
+  // A ring of tiles per wave: kStages - 1 of them on their way while one is
+  // worked on.
+  typedef TileLds<kDim> L;
+  constexpr int kStep = kWaves * kTileKeys, kAhead = kStages - 1;
+  const int key_first = begin + wave * kTileKeys;
+  const int tiles = end > key_first ? (end - key_first + kStep - 1) / kStep : 0;
+  const char* ring = s_raw + wave * kStages * L::kBytes;
+  const uint32_t ring_lds = lds_address(ring);
+  bool hole[kStages][2];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + i * kStep);
+    if (i < tiles) load_tile<kDim>(pool, pages, head, key_first + i * kStep, ring_lds + i * L::kBytes);
+    hole[i][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
+    hole[i][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
+  }
+
+  // The queries, while the first tiles come.
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
     float x[S::kKeyWords][8];
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < S::kKeyWords; ++i) {
       float y[8];
-      load8<T>(args.q, have ? base + g * (kDim / 4) + i * 8 : 0, args.q_wide != 0, y);
+      load8<T>(args.q, max(query[c], (int64_t)0) + g * (kDim / 4) + i * 8, args.q_wide != 0, y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        x[i][j] = have ? y[word_order(j)] : 0.0f;
+        x[i][j] = query[c] >= 0 ? y[word_order(j)] : 0.0f;
         top = max(top, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
       }
     }
@@ -196,31 +244,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 #pragma unroll
       for (int i = 0; i < S::kKeyWords; ++i) start[c] = mfma(__builtin_bit_cast(v8h, minus72), q[c][0][i], start[c]);
     }
-    const int pos = u.length - u.rows + token;
-    see_low[c] = pos >= args.window ? pos - args.window + 1 : 0;
-    see_high[c] = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
-    mask[c] = nullptr;
-    if (args.mask != nullptr) {
-      see_high[c] = (int)min((int64_t)see_high[c], args.mask_width);
-      mask[c] = args.mask + (have ? (int64_t)(u.first + token) * args.mask_row_stride : 0);
-    }
-    if (!have) {  // a row of padding: nothing depends on what it sees
-      see_low[c] = 0;
-      see_high[c] = args.mask != nullptr ? 0 : INT_MAX;
-    } else if (see_high[c] > see_low[c]) {
-      any_low = min(any_low, see_low[c]);
-      any_high = max(any_high, see_high[c]);
-    }
-    all_low = max(all_low, see_low[c]);
-    all_high = min(all_high, see_high[c]);
   }
-  all_low = wave_reduce(all_low, [](int a, int b) { return max(a, b); });
-  all_high = wave_reduce(all_high, [](int a, int b) { return min(a, b); });
-  any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
-  any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
-  // This worker's keys of the item, cut to what some row sees.
-  const int begin = max(at.range.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
-  const int end = (int)min((int64_t)at.range.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
 
   float ref[kCols], sum[kCols];
   v4f o[kCols][S::kTiles];
@@ -232,23 +256,16 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     for (int t = 0; t < S::kTiles; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // A ring of tiles per wave: kStages - 1 of them on their way while one is
-  // worked on.
-  typedef TileLds<kDim> L;
-  constexpr int kStep = kWaves * kTileKeys, kAhead = kStages - 1;
-  const int key_first = begin + wave * kTileKeys;
-  const int tiles = end > key_first ? (end - key_first + kStep - 1) / kStep : 0;
-  const char* ring = s_raw + wave * kStages * L::kBytes;
-  const uint32_t ring_lds = lds_address(ring);
-  bool hole[kStages][2];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    const TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + i * kStep);
-    if (i < tiles) load_tile<kDim>(pool, pages, head, key_first + i * kStep, ring_lds + i * L::kBytes);
-    hole[i][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
-    hole[i][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
-  }
   TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + kAhead * kStep);
+  uint32_t seen[kCols][2];  // mask bytes of the tile's keys of this lane
+  auto load_mask = [&](int key0) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        seen[c][h] = mask_bytes(mask[c], key0 + 16 * h + 4 * g, see_high[c]);
+  };
+  if (args.mask != nullptr) load_mask(key_first);
   int slot = 0, fill = kAhead * L::kBytes;  // offsets in the ring
   for (int n = 0; n < tiles; ++n) {
     const int key0 = key_first + n * kStep;
@@ -324,7 +341,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
         for (int i = 0; i < 8; ++i) {
           const int key = key0 + 16 * (i / 4) + 4 * g + i % 4;
           bool see = key >= see_low[c] && key < see_high[c] && !hole[0][i / 4];
-          if (args.mask != nullptr && see) see = mask[c][key] != 0;
+          if (args.mask != nullptr) see = see && (seen[c][i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
         }
@@ -396,6 +413,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
         }
       }
     }
+    if (args.mask != nullptr) load_mask(key0 + kStep);
     // All reads of the slot are behind this point: the next turn fills it.
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
@@ -593,12 +611,12 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     const int columns = columns_for(pool, batch, heads);
     s.tile_shift = columns == 2 ? 5 : 4;
     s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
-    s.least = 4;
+    s.few = num_cus;  // a granule each is the shortest way while every CU has one workgroup
   }
   s.share = heads / pool.kv_heads;
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
   s.one_launch = longest <= kShort;
-  if (s.one_launch) s.least = 1;
+  if (s.one_launch) s.few = s.workers;
   s.granule_shift = __builtin_ctz(s.one_launch ? kShort : kGranule);
   const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
   while (items * ((longest >> s.granule_shift) + 1) >= (int64_t)1 << 31) ++s.granule_shift;

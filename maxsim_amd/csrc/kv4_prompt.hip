@@ -260,11 +260,15 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           __ballot(scales[2 * kKeys + 32 * st + col] != 0.0f) != 0) {
         // A hidden key takes no part in the maxima, and its probability and
         // value scale are zeros whatever the cache holds there.
+        uint32_t seen[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          seen[i] = args.mask != nullptr ? mask_bytes(mask, first + 8 * i + 4 * g, see_high) : 0xFFFFFFFFu;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int local = 8 * (i / 4) + 4 * g + i % 4, k = first + local;
-          bool see = k >= see_low && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f;
-          if (args.mask != nullptr && see) see = mask[k] != 0;
+          const bool see = k >= see_low && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f &&
+                           (seen[i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
         }
@@ -393,7 +397,7 @@ Split kv4_prompt_split(int num_cus) {
   Split s{};
   s.tile_shift = __builtin_ctz(kPromptRows);
   s.workers = num_cus;  // LDS holds one workgroup per CU
-  s.least = 2;
+  s.few = 0;
   return s;
 }
 

@@ -38,7 +38,7 @@ struct Split {
   uint32_t tile_shift;  // log2(query rows of a tile)
   uint32_t workers;     // at most
   uint32_t granule_shift;
-  uint32_t least;       // granules of a worker, where that leaves more than one
+  uint32_t few;         // workers may have a single granule while there are no more of them
   uint32_t one_launch;  // no item is split
 };
 
@@ -125,7 +125,7 @@ __device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& b
   const uint32_t head_scan = wave_scan(head);
   deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
                                     : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
-  deal.workers = min(split.workers, max(1u, deal.total / split.least));
+  deal.workers = min(split.workers, max(max(1u, min(deal.total, split.few)), deal.total / 2));
   deal.each = deal.total / deal.workers;
   deal.extra = deal.total - deal.each * deal.workers;
   if (deal.total == 0 || worker >= deal.workers) return false;
@@ -274,6 +274,18 @@ __device__ __forceinline__ void store4(void* out, int64_t i, bool wide, v4f x) {
 // Multiplies a query row to f16's range: the exponent to add (its largest entry
 // in [2^14, 2^15)) from the bits of that entry.
 __device__ __forceinline__ int query_shift(uint32_t top) { return 141 - (int)(top >> 23); }
+
+// Four bytes of a mask row from key `key` on, none of them at `end` or past it
+// (zeros there); the row's address and the key may be odd.
+__device__ __forceinline__ uint32_t mask_bytes(const uint8_t* mask, int key, int end) {
+  uint32_t m = 0;
+  if (key + 4 <= end) {
+    __builtin_memcpy(&m, mask + key, 4);
+  } else {
+    for (int i = 0; i < 4 && key + i < end; ++i) m |= (uint32_t)mask[key + i] << (8 * i);
+  }
+  return m;
+}
 
 // The maximum of 8 or 16 values, three operands at a time.
 template <int N>
