@@ -56,4 +56,19 @@ __device__ __forceinline__ void split3(const uint32_t (&x)[8], v8b (&out)[3]) {
   for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(v8b, parts[k]);
 }
 
+// Eight as two: the upper eight bits of the significand, and the next eight.
+__device__ __forceinline__ void split2(const float (&x)[8], v8b (&out)[2]) {
+  v4u parts[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __float_as_uint(x[2 * i]), hi = __float_as_uint(x[2 * i + 1]);
+    parts[0][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+    const float a = x[2 * i] - __uint_as_float(lo & 0xFFFF0000u), b = x[2 * i + 1] - __uint_as_float(hi & 0xFFFF0000u);
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    parts[1][i] = __builtin_bit_cast(uint32_t, (v2b){(__bf16)a, (__bf16)b});
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) out[k] = __builtin_bit_cast(v8b, parts[k]);
+}
+
 }  // namespace msim

@@ -136,7 +136,11 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
                                             uint32_t from, uint32_t upto) {
   typedef Shape<kDim> S;
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
-  constexpr int kProbParts = T == kKv4F32 ? 3 : 1;  // of a probability
+  // Of a probability. One f16 part would be the larger half of an f16 result's
+  // error (2.8e-4 of the norm against 2.1e-4 with two, which is the rounding of the
+  // result; two cost 1 % at three sequences of 100,000 keys and 7 % at 32 of up to
+  // 8,000); bfloat16 results do not show it.
+  constexpr int kProbParts = T == kKv4F32 ? 3 : (T == kKv4F16 ? 2 : 1);
   typedef typename std::conditional<T == kKv4F32, v8b, v8h>::type Prob;
   constexpr int kRows = 16 * kCols;
   __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols)];
@@ -361,10 +365,14 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       for (int i = 0; i < 8; ++i) {
         const float p = exp2_hw(__builtin_fmaf(x[i], factor[c], -ref[c]));
         sum[c] += p;
-        if constexpr (T == kKv4F32)
-          product[i] = __float_as_uint(p * vs[i]);
-        else
-          probs[c][0][i] = (_Float16)(p * vs[i]);
+        const float y = p * vs[i];
+        if constexpr (T == kKv4F32) {
+          product[i] = __float_as_uint(y);
+        } else {
+          const _Float16 hi = (_Float16)y;
+          probs[c][0][i] = hi;
+          if constexpr (kProbParts == 2) probs[c][1][i] = (_Float16)(y - (float)hi);
+        }
       }
       if constexpr (T == kKv4F32) split3(product, probs[c]);
     }

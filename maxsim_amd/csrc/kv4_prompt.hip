@@ -16,11 +16,20 @@
 //   * row i of a value operand's tile t is dim 8 w + d with 32 t + i = w + d
 //     (dim / 8): the lanes that decode one word of codes each then write 16-byte
 //     pieces side by side.
+// A probability times its value scale is the sum of two bfloat16 (16 bits, at any
+// size: the smallest is single precision's). One f16 would do for the larger
+// products and take 1010 us where this takes 1220, but outputs to which only
+// products below 2^-22 of the row's largest contribute would lose bits, as happens
+// in ordinary peaked rows.
 // Per (row, key) the scores cost a lane a product with the key scale, half a
 // maximum, a fused multiply-add, an exponential (four slots), a sum, a product
-// with the value scale and half a conversion: about 9.5 issue slots for 32 x 32
-// scores' 16 per lane, 600 clocks against the MFMAs' 512; two waves per SIMD run
-// one's products beside the other's exponentials.
+// with the value scale and three slots for its parts: 12 issue slots for each of a
+// lane's 16 of 32 x 32 scores, 770 clocks, and with the decoding of the codes
+// about 900 against the MFMAs' 24 x 32. Two waves per SIMD run one's products
+// beside the other's exponentials, which hides only a part: 32 MFMAs of 521 ns
+// beside 144 vector operations of 480 ns took 727.
+// 2 x 2048 tokens behind up to 15,000, 32 heads of 128 on 8, bfloat16: 0.83 TFLOP
+// (4 dim per row and key that it sees) in 1.22 ms, 0.68 PFLOP/s.
 #include "kv4_split.hpp"
 
 namespace msim {
@@ -32,8 +41,12 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int kPromptWaves = 8;
 constexpr int kPromptRows = 32 * kPromptWaves;
 constexpr int kKeys = 128;  // of a buffer
+// A row's reference moves, to the row's largest score, when a probability passes
+// 2^6 (the moves cost nothing that shows: limits up to 2^40 took the same time).
+constexpr float kTopLimit = 6.0f;
 
 __device__ __forceinline__ v16f mfma32(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f mfma32(v8b a, v8b b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 template <int kDim>
 struct Buffer {
@@ -106,21 +119,21 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
     const int g = kg % 2;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      v8h pair[4];  // [pair of keys]: four dims of both
+      v8b pair[4];  // [pair of keys]: four dims of both
 #pragma unroll
       for (int p = 0; p < 4; ++p)
-        pair[p] = decode_word(
+        pair[p] = decode_word_bf16(
             __builtin_amdgcn_perm(s.words[2 * p + 1], s.words[2 * p], half ? 0x07060302u : 0x05040100u));
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        v8h a;
+        v8b a;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           a[2 * p] = pair[p][2 * d];
           a[2 * p + 1] = pair[p][2 * d + 1];
         }
         const int line = (half * 4 + d) * (kDim / 8) + w;
-        *reinterpret_cast<v8h*>(values + (line / 32 * 64 + g * 32 + line % 32) * 16) = a;
+        *reinterpret_cast<v8b*>(values + (line / 32 * 64 + g * 32 + line % 32) * 16) = a;
       }
     }
   }
@@ -230,7 +243,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     }
     const float* scales = reinterpret_cast<const float*>(now + B::kScales);
     const v8h* keys = reinterpret_cast<const v8h*>(now) + lane;
-    const v8h* values = reinterpret_cast<const v8h*>(now + B::kKeyBytes) + lane;
+    const v8b* values = reinterpret_cast<const v8b*>(now + B::kKeyBytes) + lane;
     // The 32-key steps that this wave's rows see something of.
     const int step0 = max(0, any_low - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
 #pragma unroll 1
@@ -247,7 +260,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
       for (int i = 0; i < kChunks; ++i) s = mfma32(keys[(st * kChunks + i) * kWave], q[i], s);
       // The step's values are read beside the products.
       __builtin_amdgcn_sched_barrier(0);
-      v8h va[2][kTiles];
+      v8b va[2][kTiles];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -273,28 +286,35 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           vs[i] = see ? vs[i] : 0.0f;
         }
       }
-      const float top = max_of(x) * factor, product = top + __builtin_amdgcn_logf(max_of(vs));
-      if (__ballot(product > ref + kProductLimit || top > ref + kProbLimit) != 0) {
-        const float next = fmaxf(ref, fmaxf(other_half_max(product) - kProductGoal, other_half_max(top) - kProbGoal));
+      const float top = max_of(x) * factor;
+      if (__ballot(top > ref + kTopLimit) != 0) {
+        const float next = fmaxf(ref, other_half_max(top));
         const float alpha = exp2_hw(ref - next);
         ref = next;
         sum *= alpha;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t] *= alpha;
       }
-      v8h probs[2];
+      v8b probs[2][2];
       float more = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = exp2_hw(__builtin_fmaf(x[i], factor, -ref));
-        (i & 1 ? more : sum) += p;
-        probs[i / 8][i % 8] = (_Float16)(p * vs[i]);
+      for (int c = 0; c < 2; ++c) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = exp2_hw(__builtin_fmaf(x[8 * c + i], factor, -ref));
+          (i & 1 ? more : sum) += p;
+          y[i] = p * vs[8 * c + i];
+        }
+        split2(y, probs[c]);
       }
       sum += more;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) o[t] = mfma32(va[c][t], probs[c], o[t]);
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) o[t] = mfma32(va[c][t], probs[c][p], o[t]);
     }
     char* swap = now;
     now = other;

@@ -499,6 +499,102 @@ def test_step_on_another_stream_and_in_a_graph(gpu):
         assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1])
 
 
+# ---------------------------------------------------------------- prompts
+#
+# Many new tokens per sequence: rows times shared heads reach half a workgroup's
+# 256 on average.
+
+
+def _prompts(dim, page, seed, lengths=(301, 128, 700, 0, 150), new=(301, 128, 130, 0, 97), spare=0):
+    cache = Int4KVCache(sum(-(-n // page) for n in lengths) + 2, 2, dim, page_size=page)
+    _fill(cache, seed)
+    return cache, Batch(cache, list(lengths), list(new), seed=seed, spare=spare)
+
+
+@pytest.mark.parametrize("kind", [F16, BF16, F32])
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 32), (128, 64), (256, 16)])
+@pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, 70), (False, 200)])
+def test_prompts(gpu, kind, dim, page, causal, window):
+    cache, batch = _prompts(dim, page, dim)
+    q = _queries(batch.rows, 8, dim, kind, 3)
+    got, lse = cache.attend(q, *batch.args, causal=causal, window=window, return_lse=True)
+    _check(cache, batch, q, got, lse, causal=causal, window=window)
+    assert torch.equal(cache.attend(q, *batch.args, causal=causal, window=window), got)
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("share", [1, 3, 5, 16])
+def test_prompts_of_any_sharing(gpu, kind, share):
+    """Tiles of rows that end inside a token's heads."""
+    cache, batch = _prompts(128, 16, share, lengths=(400, 333), new=(260, 300))
+    q = _queries(batch.rows, 2 * share, 128, kind, 3, size=2.0)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check(cache, batch, q, got, lse)
+    _check(cache, batch, q, cache.attend(q, *batch.args, scale=-0.2), scale=-0.2)
+    _check(cache, batch, q, cache.attend(q, *batch.args, scale=0.0), scale=0.0)
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("width", [0, 3, 300, 700])
+def test_prompts_under_masks(gpu, kind, width):
+    cache, batch = _prompts(64, 32, 4)
+    mask = torch.rand((batch.rows, width + 3), generator=_rng(width)) < 0.5
+    mask[::7] = False
+    mask[40:300, :128] = False  # whole buffers of keys that most rows do not see
+    mask = mask.cuda()[:, 1:1 + width]
+    q = _queries(batch.rows, 6, 64, kind, 5)
+    got, lse = cache.attend(q, *batch.args, mask=mask, return_lse=True)
+    _check(cache, batch, q, got, lse, mask=mask)
+    assert not bool(got[::7].any()) and bool((lse[::7] == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+def test_prompts_over_holes_and_strides(gpu, kind):
+    cache, batch = _prompts(96, 16, 6, lengths=(400, 300), new=(270, 300))
+    batch.host_table[0, 3], batch.host_table[0, 11], batch.host_table[1, 0] = -1, cache.num_pages, -5
+    batch.table = batch.host_table.cuda()
+    fused = torch.randn((batch.rows, 4 * 96 + 31), generator=_rng(2)).to(kind).cuda()
+    q = fused[:, 5:5 + 4 * 96].view(batch.rows, 4, 96)
+    out = torch.full((4, batch.rows, 96 + 3), 5.0, dtype=kind, device="cuda")
+    view = out.permute(1, 0, 2)[..., 1:97]
+    cache.attend(q, *batch.args, out=view)
+    _check(cache, batch, q, view)
+    assert bool((out[..., :1] == 5).all()) and bool((out[..., 97:] == 5).all())
+    # Rows outside the offsets come out as rows that see nothing.
+    more = torch.cat((q[:2], q, q[:3]))
+    got, lse = cache.attend(more, batch.table, batch.lengths, batch.offsets + 2, return_lse=True)
+    assert torch.equal(got[2:-3], view)
+    assert not bool(got[:2].any()) and not bool(got[-3:].any()) and bool((lse[-3:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("junk", [math.nan, math.inf, 3e38, 1e-38])
+def test_prompts_do_not_see_what_is_hidden(gpu, junk):
+    """Rows before a spoilt token, and tokens past the end."""
+    cache, batch = _prompts(128, 16, 8, lengths=(500,), new=(400,))
+    q = _queries(400, 8, 128, BF16, 6)
+    clean = cache.attend(q, *batch.args)
+    held = torch.zeros((cache.num_pages, 16), dtype=torch.bool)
+    for pos in range(300):
+        held[int(batch.host_table[0, pos // 16]), pos % 16] = True
+    for scales in (cache.k_scales, cache.v_scales):
+        scales.transpose(1, 2)[~held.cuda()] = junk
+    got = cache.attend(q, *batch.args)
+    assert bool(torch.isfinite(got[:200]).all())
+    assert torch.equal(got[:200], clean[:200])
+    if math.isnan(junk):
+        assert bool(torch.isnan(got[200:]).all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+def test_prompts_of_large_scores(gpu, kind):
+    """References that move often, and scores of one key."""
+    cache, batch = _prompts(128, 32, 9, lengths=(600, 290), new=(300, 290))
+    for size in (0.0, 8.0, 300.0):
+        q = _queries(batch.rows, 8, 128, kind, 8, size=size)
+        got, lse = cache.attend(q, *batch.args, return_lse=True)
+        _check(cache, batch, q, got, lse)
+
+
 # -------------------------------------------------------------- refusals
 
 
