@@ -41,7 +41,7 @@ __device__ __forceinline__ void split3(uint32_t x, uint32_t (&part)[3]) {
   part[2] = __float_as_uint(r1 - __uint_as_float(b));
 }
 
-// Eight single precision values as three operands.
+// Eight single precision values as three operands, which sum to them exactly.
 __device__ __forceinline__ void split3(const uint32_t (&x)[8], v8b (&out)[3]) {
   v4u parts[3];
 #pragma unroll
@@ -56,8 +56,9 @@ __device__ __forceinline__ void split3(const uint32_t (&x)[8], v8b (&out)[3]) {
   for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(v8b, parts[k]);
 }
 
-// Eight as two: the upper eight bits of the significand, and the next eight.
-__device__ __forceinline__ void split2(const float (&x)[8], v8b (&out)[2]) {
+// Eight as two, 16 bits of them: the upper eight bits of the significand, and the
+// rest rounded.
+__device__ __forceinline__ void in_parts(const float (&x)[8], v8b (&out)[2]) {
   v4u parts[2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -69,6 +70,12 @@ __device__ __forceinline__ void split2(const float (&x)[8], v8b (&out)[2]) {
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k) out[k] = __builtin_bit_cast(v8b, parts[k]);
+}
+__device__ __forceinline__ void in_parts(const float (&x)[8], v8b (&out)[3]) {
+  uint32_t bits[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(x[i]);
+  split3(bits, out);
 }
 
 }  // namespace msim

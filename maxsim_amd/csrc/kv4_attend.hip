@@ -4,9 +4,9 @@
 //   k_j = c_j s_j and v_j = d_j t_j with int4 codes c, d and row scales s, t
 //
 // The query rows of one sequence and key/value head (its new tokens times the
-// query heads that share it) are taken 16 to 64 at a time against tiles of 32
+// query heads that share it) are taken 16 or 32 at a time against tiles of 32
 // keys.  A tile's scores are S^T = C Q^T and its part of the output is
-// O^T = D^T P^T, both on v_mfma_f32_16x16x32_f16, so that a lane keeps one query
+// O^T = D^T P^T, on v_mfma_f32_16x16x32_f16 and _bf16, so that a lane keeps one query
 // row throughout (column lane % 16) and the probabilities leave the first
 // product in the registers in which the second one takes them:
 //   * a lane's keys of the two 16-key halves, 4 g .. 4 g + 3 and 16 + the same
@@ -15,21 +15,28 @@
 //     eighth or a sixteenth of eight value rows; the words of two value rows
 //     are merged by halves, so that the pairs a decoded register holds are two
 //     keys of one dim.
-// Codes become f16 by one bitwise operation per pair (0x6400 | code ^ 8 is
-// 1032 + code, exactly) and one packed subtraction.  The key scale multiplies
-// the score, the value scale the probability; nothing else is dequantised.
+// Keys' codes become f16 by one bitwise operation per pair (0x6400 | code ^ 8 is
+// 1032 + code, exactly) and one packed subtraction, values' codes bfloat16 by a
+// conversion each and a merge.  The key scale multiplies the score, the value scale
+// the probability; nothing else is dequantised.
 //
 // Queries are scaled to f16 by a power of two per row, largest entry in
 // [2^14, 2^15): bfloat16 entries keep all their bits down to 2^-28 of the
 // largest, f16 ones too.  Single precision queries are a sum of two f16 (22
-// bits).  A probability times its value scale is taken relative to the row's
-// largest such product, at 2^13 to 2^15, and rounded to f16: 11 bits down to
-// 2^-27 of the largest, fewer below.  Single precision calls take it exactly, as
-// three bfloat16 parts.  Scores, maxima, sums and outputs are single precision.
+// bits).  A probability times its value scale is the sum of two bfloat16 (16 bits;
+// single precision calls: of three, exactly), at any size that single precision
+// has: with one f16 outputs to which only small products contribute lost bits, as
+// happens in peaked rows, and f16 results had an error of 2.8e-4 of the norm in
+// place of 2.1e-4, the rounding of the result.  The second part costs 3 % at 32
+// tokens behind up to 8,000 keys, and nothing at three behind 100,000.  Scores,
+// maxima, sums and outputs are single precision.
 //
 // Bytes bound it: dim + 8 per key and head against 4 dim operations per query
 // row.  The keys of a sequence are split among workgroups when there are few
 // query rows; each leaves its unnormalised sum and a second launch joins them.
+// 32 heads of 128 on 8: three tokens behind 100,000 to 131,072 keys (f16) take
+// 86 us, 4.5 TB/s, of which the main launch has 79 and the join 5; 32 behind 100 to
+// 8,000 (bfloat16) 40 us, 3.8 TB/s (34 and 5).
 #include "kv4_split.hpp"
 
 namespace msim {
@@ -136,12 +143,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
                                             uint32_t from, uint32_t upto) {
   typedef Shape<kDim> S;
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
-  // Of a probability. One f16 part would be the larger half of an f16 result's
-  // error (2.8e-4 of the norm against 2.1e-4 with two, which is the rounding of the
-  // result; two cost 1 % at three sequences of 100,000 keys and 7 % at 32 of up to
-  // 8,000); bfloat16 results do not show it.
-  constexpr int kProbParts = T == kKv4F32 ? 3 : (T == kKv4F16 ? 2 : 1);
-  typedef typename std::conditional<T == kKv4F32, v8b, v8h>::type Prob;
+  constexpr int kProbParts = T == kKv4F32 ? 3 : 2;  // of a probability times its value scale
   constexpr int kRows = 16 * kCols;
   __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols)];
   const int lane = lane_id(), col = lane % 16, g = lane / 16, wave = wave_uniform(threadIdx.x / kWave);
@@ -329,7 +331,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 
     const bool whole = key0 >= all_low && key0 + kTileKeys <= all_high && args.mask == nullptr && !hole[0][0] &&
                        !hole[0][1];
-    Prob probs[kCols][kProbParts];
+    v8b probs[kCols][kProbParts];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       float x[8], vs[8];
@@ -350,31 +352,23 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
           vs[i] = see ? vs[i] : 0.0f;
         }
       }
-      // The largest score, and a bound of the largest product.
-      const float top = max_of(x) * factor[c], most = top + __builtin_amdgcn_logf(max_of(vs));
-      if (__ballot(most > ref[c] + kProductLimit || top > ref[c] + kProbLimit) != 0) {
-        const float now = fmaxf(ref[c], fmaxf(across_groups_max(most) - kProductGoal, across_groups_max(top) - kProbGoal));
+      const float top = max_of(x) * factor[c];
+      if (__ballot(top > ref[c] + kTopLimit) != 0) {
+        const float now = fmaxf(ref[c], across_groups_max(top));
         const float alpha = exp2_hw(ref[c] - now);
         ref[c] = now;
         sum[c] *= alpha;
 #pragma unroll
         for (int t = 0; t < S::kTiles; ++t) o[c][t] *= alpha;
       }
-      uint32_t product[8];
+      float y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p = exp2_hw(__builtin_fmaf(x[i], factor[c], -ref[c]));
         sum[c] += p;
-        const float y = p * vs[i];
-        if constexpr (T == kKv4F32) {
-          product[i] = __float_as_uint(y);
-        } else {
-          const _Float16 hi = (_Float16)y;
-          probs[c][0][i] = hi;
-          if constexpr (kProbParts == 2) probs[c][1][i] = (_Float16)(y - (float)hi);
-        }
+        y[i] = p * vs[i];
       }
-      if constexpr (T == kKv4F32) split3(product, probs[c]);
+      in_parts(y, probs[c]);
     }
 
     // The tile's part of the output: the codes of two keys side by side.
@@ -395,17 +389,12 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       }
 #pragma unroll
       for (int half = 0; half < (S::kValueDims >= 8 ? 2 : 1); ++half) {
-        Prob pair[4];  // [pair of keys]: four dims of both
+        v8b pair[4];  // [pair of keys]: four dims of both
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          if constexpr (T == kKv4F32)
-            pair[p] = decode_word_bf16(half ? high[p] : low[p]);
-          else
-            pair[p] = decode_word(half ? high[p] : low[p]);
-        }
+        for (int p = 0; p < 4; ++p) pair[p] = decode_word_bf16(half ? high[p] : low[p]);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          Prob a;
+          v8b a;
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
             a[2 * p] = pair[p][2 * d];
@@ -431,6 +420,10 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     for (int i = 0; i < kAhead; ++i) hole[i][0] = hole[i + 1][0], hole[i][1] = hole[i + 1][1];
   }
   mfma_results_fence();
+#pragma unroll
+  for (int c = 0; c < kCols; ++c)
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t) o[c][t] *= kCodeUnit;
 
   // The waves' results joined in their order, in LDS.
   float* s_ref = reinterpret_cast<float*>(s_raw);  // [waves][rows]
@@ -604,7 +597,9 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
 }
 
 // Column tiles per workgroup: as many as a sequence's rows fill on average (one
-// for wide heads, whose outputs take the registers).
+// for wide heads, whose outputs take the registers). At 8 sequences of 4,000 keys,
+// 32 heads of 128 on 8, two took 30.2 us for 5 tokens each and one 32.0; 32.7 and
+// 33.3 for 8; 38.2 and 41.7 for 16.
 int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   const int64_t rows = (int64_t)batch.rows * (heads / pool.kv_heads) / std::max(1, batch.batch);
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
@@ -619,7 +614,9 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     const int columns = columns_for(pool, batch, heads);
     s.tile_shift = columns == 2 ? 5 : 4;
     s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
-    s.few = num_cus;  // a granule each is the shortest way while every CU has one workgroup
+    // A granule each is the shortest way while every CU has one workgroup (one token
+    // behind 1,000 keys: 12.2 us against 13.2).
+    s.few = num_cus;
   }
   s.share = heads / pool.kv_heads;
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;

@@ -2,11 +2,11 @@
 // sequence (prompts and their pieces), bfloat16 and f16.
 //
 // The products are those of kv4_attend.hip, S^T = C Q^T and O^T = D^T P^T, here
-// on v_mfma_f32_32x32x16_f16, and operations bound them instead of bytes: 4 dim
+// on v_mfma_f32_32x32x16_f16 and _bf16, and operations bound them instead of bytes: 4 dim
 // per (row, key).  So the codes are decoded once per workgroup of 256 query rows
 // and not once per wave:
 //   * eight waves have 32 rows each, in registers, and 128 keys at a time: four
-//     waves decode the keys to f16, four the values, into one of two buffers of
+//     waves decode the keys to f16, four the values to bfloat16, into one of two buffers of
 //     LDS, while all work on the other; one barrier per 128 keys;
 //   * LDS holds the MFMAs' A operands in lane order (16 bytes a lane), so every
 //     read of it is contiguous: keys [32 keys][16 dims], values [16 keys][32 dims];
@@ -41,10 +41,6 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int kPromptWaves = 8;
 constexpr int kPromptRows = 32 * kPromptWaves;
 constexpr int kKeys = 128;  // of a buffer
-// A row's reference moves, to the row's largest score, when a probability passes
-// 2^6 (the moves cost nothing that shows: limits up to 2^40 took the same time).
-constexpr float kTopLimit = 6.0f;
-
 __device__ __forceinline__ v16f mfma32(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v16f mfma32(v8b a, v8b b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
@@ -306,7 +302,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           (i & 1 ? more : sum) += p;
           y[i] = p * vs[8 * c + i];
         }
-        split2(y, probs[c]);
+        in_parts(y, probs[c]);
       }
       sum += more;
 #pragma unroll
@@ -346,7 +342,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     const int tok = (int)(row / split.share), qh = at.head * split.share + (int)(row - tok * split.share);
     const float all = __shfl(ref, local), total = __shfl(sum, local);
     if (tok >= u.rows) continue;
-    v4f y = *reinterpret_cast<const v4f*>(mine + local * kPitch + d);
+    v4f y = *reinterpret_cast<const v4f*>(mine + local * kPitch + d) * kCodeUnit;
     if (!whole_item) {
       float* dst = partial_slot(partial, split, kDim, blockIdx.x, from == 0);
       *reinterpret_cast<v4f*>(dst + (wave * 32 + local) * kDim + d) = y;
@@ -408,9 +404,15 @@ hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArg
 }  // namespace
 
 bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type) {
-  // Half a workgroup's rows per sequence and head, on average.
+  // Two workgroups' rows per sequence and head on average, or one where the items
+  // fill half the CUs: fewer leave CUs, or parts of them, without work. Heads of
+  // 128, 32 on 8, this kernel against kv4_attend.hip's: 8 x 128 tokens behind 4,000
+  // keys 136 us against 151, 8 x 96 129 against 123, 8 x 64 87 against 85, 8 x 32 70
+  // against 52; 2 x 128 behind 16,000 135 against 141; 32 x 256 behind 1,000, 8 heads
+  // on 8, 71 against 114.
+  const int64_t rows = (int64_t)batch.rows * (heads / pool.kv_heads), whole = (int64_t)batch.batch * kPromptRows;
   return type != kKv4F32 && pool.dim <= 128 && batch.offsets != nullptr &&
-         (int64_t)batch.rows * (heads / pool.kv_heads) >= (int64_t)batch.batch * (kPromptRows / 2);
+         (rows >= 2 * whole || (rows >= whole && rows * pool.kv_heads >= 128 * kPromptRows));
 }
 
 Split kv4_prompt_split(int num_cus) {

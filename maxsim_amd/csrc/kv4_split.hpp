@@ -10,9 +10,9 @@
 namespace msim {
 
 constexpr float kUnset = -FLT_MAX;
-// A row's reference moves when a product passes 2^15 or a probability 2^100, to
-// where the largest are 2^13 and 2^90.
-constexpr float kProductLimit = 15.0f, kProductGoal = 13.0f, kProbLimit = 100.0f, kProbGoal = 90.0f;
+// A row's reference moves, to its largest score, when a probability passes 2^6
+// (the moves cost nothing that shows: limits up to 2^40 took the same time).
+constexpr float kTopLimit = 6.0f;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -26,7 +26,9 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // it came in from the worker before (it has at most one of each).
 //
 // Where no sequence can be longer than kShort keys a granule is kShort: no item
-// is split, and the call is one launch.
+// is split, and the call is one launch. Another 128 keys cost a workgroup about
+// 1 us, the second launch 4 (one token behind 120 keys 7.5 us against 12.2 split,
+// behind 391 10.3 against 12.2; 64 tokens behind 500 14.5 against 24.7).
 constexpr int kKeyAlign = 32;  // a tile's first key
 constexpr int kGranule = 128;
 constexpr int kShort = 4 * kGranule;
@@ -188,9 +190,19 @@ struct Cursor {
 
 // -------------------------------------------------------- queries and outputs
 
-// Eight codes of a word as bfloat16, in the order of decode_word.
+// Eight codes of a word over 16 as bfloat16, in the order of decode_word: the
+// conversion of four bits (-8 .. 7 to sixteenths in single precision, a byte's low
+// half being any byte of a register) and the upper halves of two.
+constexpr float kCodeUnit = 16.0f;
 __device__ __forceinline__ v8b decode_word_bf16(uint32_t w) {
-  return __builtin_bit_cast(v8b, (v4u){pair_bf16(w << 3), pair_bf16(w >> 1), pair_bf16(w >> 5), pair_bf16(w >> 9)});
+  uint32_t odd = w >> 4;
+  asm("" : "+v"(odd));  // so that bytes of it are taken, and not others of w by shifts
+  auto pair = [](uint32_t x, int byte) -> uint32_t {
+    return __builtin_amdgcn_perm(
+        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte + 16, 8))),
+        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte, 8))), 0x07060302u);
+  };
+  return __builtin_bit_cast(v8b, (v4u){pair(w, 0), pair(odd, 0), pair(w, 1), pair(odd, 1)});
 }
 
 // Eight codes of a word as f16: pairs (code i, code i + 4).

@@ -394,9 +394,7 @@ def test_large_and_small_scores(gpu, kind):
         _check(cache, batch, q, got, lse)
 
 
-@pytest.mark.parametrize("kind", [F32, F16, pytest.param(BF16, marks=pytest.mark.xfail(
-    strict=True, reason="outputs of less than 2^-27 of their row's largest probability times value scale have fewer "
-                        "bits than bfloat16 could hold: the f16 product is subnormal there"))])
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
 def test_value_scales_far_apart(gpu, kind):
     """Rows of zeros under large scales, others 2^-24 of them."""
     cache = Int4KVCache(16, 1, 128, page_size=32)
@@ -546,6 +544,32 @@ def test_prompts_under_masks(gpu, kind, width):
     got, lse = cache.attend(q, *batch.args, mask=mask, return_lse=True)
     _check(cache, batch, q, got, lse, mask=mask)
     assert not bool(got[::7].any()) and bool((lse[::7] == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("width", [0, 3, 300, 700])
+def test_longer_prompts_under_masks(gpu, kind, width):
+    """The same where every sequence has two workgroups' rows or more, on average."""
+    cache, batch = _prompts(64, 32, 4)
+    mask = torch.rand((batch.rows, width + 3), generator=_rng(width)) < 0.5
+    mask[::7] = False
+    mask[40:300, :128] = False
+    mask = mask.cuda()[:, 1:1 + width]
+    q = _queries(batch.rows, 12, 64, kind, 5)
+    got, lse = cache.attend(q, *batch.args, mask=mask, return_lse=True)
+    _check(cache, batch, q, got, lse, mask=mask)
+    assert not bool(got[::7].any()) and bool((lse[::7] == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [255, 256, 257, 511, 512, 513, 700])
+def test_rows_about_a_workgroup(gpu, kind, dim, rows):
+    """Numbers of rows at which tiles are full and other kernels are chosen."""
+    cache, batch = _prompts(dim, 64, rows, lengths=(rows + 44,), new=(rows,))
+    q = _queries(rows, 2, dim, kind, 4)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check(cache, batch, q, got, lse)
 
 
 @pytest.mark.parametrize("kind", [F16, BF16])
