@@ -35,8 +35,8 @@
 // row.  The keys of a sequence are split among workgroups when there are few
 // query rows; each leaves its unnormalised sum and a second launch joins them.
 // 32 heads of 128 on 8: three tokens behind 100,000 to 131,072 keys (f16) take
-// 86 us, 4.5 TB/s, of which the main launch has 79 and the join 5; 32 behind 100 to
-// 8,000 (bfloat16) 40 us, 3.8 TB/s (34 and 5).
+// 86 us, 4.5 TB/s, of which the main launch has 81 and the join 5; 32 behind 100 to
+// 8,000 (bfloat16) 40 us, 3.8 TB/s (35 and 5).
 #include "kv4_split.hpp"
 
 namespace msim {

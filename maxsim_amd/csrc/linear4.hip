@@ -22,7 +22,7 @@
 // Bytes bound it: n k / 2 and the scales, for any number of rows that fits a
 // pass (32).  Waves of a workgroup take the 128-column tiles of the same rows of W
 // in turn and join in LDS in a fixed order.  One row by 4096 x 4096 takes 4.7 us
-// (3.6 in the kernel, 2.4 TB/s; the call's host side is the rest), 16 rows by
+// (4.4 in the kernel; the host side of a call is 4.2), 16 rows by
 // 28672 x 8192 in groups of 64 take 25.1 us, 5.0 TB/s.
 #include "codes4.hpp"
 #include "linear4.hpp"
