@@ -276,7 +276,9 @@ hipError_t launch_rows(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows
   constexpr int kRows = 256 / row_lanes(kDim);
   const int size = T == kKv4F32 ? 4 : 2;
   const bool wide = rows_aligned(rows[0], size) && rows_aligned(rows[1], size);
-  // All heads in one workgroup, or as few as give every CU some workgroups.
+  // All heads in one workgroup, or as few as give every CU some workgroups. 8 heads
+  // of 128, append in bfloat16: 512 rows 3.8 us with one each against 7.4 with all,
+  // 45,000 rows 78 against 64 (read 58 against 37).
   const int64_t tiles = (batch.rows + kRows - 1) / kRows;
   int heads = pool.kv_heads;
   while (heads > 1 && tiles * 2 * ((pool.kv_heads + heads - 1) / heads) < kEnoughGroups) heads = (heads + 1) / 2;

@@ -290,7 +290,8 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
   const int64_t gx = ((w.n + 15) / 16 + kRowTiles - 1) / kRowTiles, gy = (rows + 16 * kCols - 1) / (16 * kCols);
   if (gy > 65535) return hipErrorInvalidValue;
   // Enough waves for the CUs' latency, within the tiles there are and the LDS
-  // that joins them.
+  // that joins them (one row by 4096 x 4096 4.3 us, with four waves 5.6; by 28672 x
+  // 8192 22.3 and 29.2).
   const int tiles_k = (w.k + 127) / 128;
   int waves = 4;
   while (waves < most_waves(T, kGroups, kCols, kRowTiles) && waves * 2 <= tiles_k && gx * gy * waves < num_cus * 16)
@@ -313,7 +314,9 @@ hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, i
                           int64_t out_row_stride, int num_cus, hipStream_t stream) {
   // Row tiles of a workgroup: the busiest CU has its workgroups' row tiles to do,
   // and with each workgroup the rows of x, whose loads (16 rows apart) cost as
-  // much as two row tiles; one row costs half of one.
+  // much as two row tiles; one row costs half of one. At 4096 x 4096 one tile takes
+  // 4.3 us for a row and 6.8 for 16, as many as the registers hold 9.2 and 12.7; at
+  // 28672 x 8192 57 us against 25 for 16 rows.
   const int64_t tiles = (w.n + 15) / 16, columns = (rows + 16 * kCols - 1) / (16 * kCols);
   auto cost = [&](int row_tiles) -> int64_t {
     const int64_t groups = (tiles + row_tiles - 1) / row_tiles * columns;
@@ -338,6 +341,8 @@ hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, i
 template <Kv4Type T, int kGroups>
 hipError_t launch_group(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
                         int64_t out_row_stride, int num_cus, hipStream_t stream) {
+  // Two column tiles read a large matrix once (32 rows by 28672 x 8192 33 us against
+  // 45, by 4096 x 4096, which the caches hold, 10.4 against 8.6).
   if (rows <= 16) return launch_columns<T, kGroups, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
   return launch_columns<T, kGroups, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
 }
