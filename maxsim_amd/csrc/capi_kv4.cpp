@@ -13,6 +13,9 @@ namespace {
 
 constexpr int64_t kMaxRows = int64_t{1} << 26;  // of a call: keeps every launch within the grid limits
 constexpr double kLog2e = 1.4426950408889634;
+// The kernels hold key positions in 32 bits and look ahead of a sequence's end by up
+// to 640 keys (the tiles on their way, the page numbers of the next ones).
+constexpr int64_t kMostKeys = INT_MAX - 4096;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -44,8 +47,8 @@ Kv4Batch check_batch(const Kv4Pool& pool, const int32_t* table, const int32_t* l
                      int64_t batch, int64_t max_pages, int64_t rows) {
   if (batch < 0 || rows < 0 || max_pages < 0) throw InvalidArgument("batch, max_pages and rows must not be negative");
   if (rows > kMaxRows || batch > kMaxRows) throw NotSupported("a call takes at most 2^26 rows and sequences");
-  if (max_pages > (int64_t)INT_MAX >> pool.page_shift)
-    throw NotSupported("a page table holds sequences of less than 2^31 tokens");
+  if (max_pages > kMostKeys >> pool.page_shift)
+    throw NotSupported("a page table holds sequences of less than 2^31 - 4096 tokens");
   if (offsets == nullptr && rows != batch)
     throw InvalidArgument("without offsets there is one row per sequence");
   if (batch > 0 && (lengths == nullptr || (table == nullptr && max_pages > 0)))

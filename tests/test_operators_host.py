@@ -61,6 +61,18 @@ def test_attend_checks(change, status, text):
     assert got[0] == status and text in got[1]
 
 
+def test_key_positions_stay_within_32_bits():
+    """Kernels look past a sequence's end: a table whose last keys' successors pass 2^31 is refused."""
+    for page_size, most in ((16, (2**31 - 4097) // 16), (4096, 2**19 - 2), (65536, 2**15 - 1)):
+        pool = _pool(page_size=page_size)
+        need = ctypes.c_uint64(0)
+        for pages, status in ((most, 0), (most + 1, 3)):
+            got = _status("msim_kv4_attend_workspace", ctypes.addressof(pool), 1, pages, 1, 4, ctypes.byref(need))
+            assert got[0] == status and (status == 0 or "2^31" in got[1])
+            args = [P, P, None, 0, pages, 0, P, 128, 64, P, 128, 64, 0, None]
+            assert _status("msim_kv4_append_async", ctypes.addressof(pool), *args)[0] == status
+
+
 def test_calls_of_no_rows_do_nothing():
     pool = _pool()
     assert _status("msim_kv4_append_async", ctypes.addressof(pool), None, None, None, 0, 0, 0, None, 0, 0, None, 0, 0, 0,
