@@ -14,18 +14,32 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v4f mfma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// A pair of codes under a constant exponent, bits 3..6 of both halves: 24 + code
-// in bfloat16 and 136 + code in f16 (the sign bit turned).
-__device__ __forceinline__ uint32_t pair_bf16_24(uint32_t w) { return (w & 0x00780078u) ^ 0x41C041C0u; }
+// A pair of codes, bits 3..6 of both halves.  Under a constant exponent they are
+// 136 + code in f16 and 24 + code in bfloat16 (the sign bit turned); the
+// differences, in f16 and in single precision, are exact.
 __device__ __forceinline__ uint32_t pair_f16(uint32_t w) {
   const v2h base = {(_Float16)136.0f, (_Float16)136.0f};
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & 0x00780078u) ^ 0x58405840u) - base);
 }
-// The codes themselves in bfloat16: single precision differences, all exact.
 __device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
-  const uint32_t r = pair_bf16_24(w);
+  const uint32_t r = (w & 0x00780078u) ^ 0x41C041C0u;
   const float lo = __uint_as_float(r << 16) - 24.0f, hi = __uint_as_float(r & 0xFFFF0000u) - 24.0f;
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// Eight codes of a word over 16 as bfloat16, pairs (code i, code i + 4): the
+// conversion of four bits (-8 .. 7 to sixteenths in single precision, a byte's low
+// half being any byte of a register) and the upper halves of two.
+constexpr float kCodeUnit = 16.0f;
+__device__ __forceinline__ v8b decode_word_bf16(uint32_t w) {
+  uint32_t odd = w >> 4;
+  asm("" : "+v"(odd));  // so that bytes of it are taken, and not others of w by shifts
+  auto pair = [](uint32_t x, int byte) -> uint32_t {
+    return __builtin_amdgcn_perm(
+        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte + 16, 8))),
+        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte, 8))), 0x07060302u);
+  };
+  return __builtin_bit_cast(v8b, (v4u){pair(w, 0), pair(odd, 0), pair(w, 1), pair(odd, 1)});
 }
 
 // Three bfloat16 parts (in the upper halves) that sum to x exactly: the upper

@@ -190,21 +190,6 @@ struct Cursor {
 
 // -------------------------------------------------------- queries and outputs
 
-// Eight codes of a word over 16 as bfloat16, in the order of decode_word: the
-// conversion of four bits (-8 .. 7 to sixteenths in single precision, a byte's low
-// half being any byte of a register) and the upper halves of two.
-constexpr float kCodeUnit = 16.0f;
-__device__ __forceinline__ v8b decode_word_bf16(uint32_t w) {
-  uint32_t odd = w >> 4;
-  asm("" : "+v"(odd));  // so that bytes of it are taken, and not others of w by shifts
-  auto pair = [](uint32_t x, int byte) -> uint32_t {
-    return __builtin_amdgcn_perm(
-        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte + 16, 8))),
-        __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4(__builtin_amdgcn_ubfe(x, 8 * byte, 8))), 0x07060302u);
-  };
-  return __builtin_bit_cast(v8b, (v4u){pair(w, 0), pair(odd, 0), pair(w, 1), pair(odd, 1)});
-}
-
 // Eight codes of a word as f16: pairs (code i, code i + 4).
 __device__ __forceinline__ v8h decode_word(uint32_t w) {
   const v2h base = {(_Float16)1032.0f, (_Float16)1032.0f};

@@ -9,15 +9,16 @@
 // dequantised.
 //
 // Codes in the registers of the MFMA.  A word holds eight columns of a row as
-// nibbles, turned left by three bits: bits 3..6 of a half, under a constant
-// exponent, make 16 + (code ^ 8) = 24 + code in bfloat16 (7 mantissa bits) and
-// 136 + code in f16 (10 bits), by one bitwise operation per pair.
-//   bfloat16 x: the 24 stays; the chain starts from -24 sum(x), which one more
-//     MFMA gives (every row of its A is -24), so the sum is of the codes again.
-//     The products are exact and the offset costs 24 / |c| times the rounding
-//     of single precision sums, 2^-19 or so against bfloat16's 2^-9.
-//   f16 x: 136 is subtracted (exactly) before the product.
-//   f32 x: three bfloat16 parts that sum to x exactly, codes made exact.
+// nibbles, turned left by three bits, and becomes eight exact values:
+//   bfloat16 x: turned back, the conversion of four bits to sixteenths and a merge
+//     per pair, 14 operations a word.
+//   f16 x: bits 3..6 of a half, under a constant exponent, make 136 + code; 136 is
+//     subtracted, 11 operations.
+//   f32 x: three bfloat16 parts that sum to x exactly; codes as 24 + code in
+//     bfloat16, 24 subtracted in single precision.
+// So every product is exact, and a column whose code is zero adds nothing: with the
+// 24 left in the codes and taken off the sum (7 operations) a column of x 1e6 times
+// the others left its rounding in results that it has no part in.
 //
 // Bytes bound it: n k / 2 and the scales, for any number of rows that fits a
 // pass (32).  Waves of a workgroup take the 128-column tiles of the same rows of W
@@ -74,14 +75,19 @@ struct Operand<kKv4F32> {
   static constexpr int kParts = 3;
 };
 
+// Eight codes of a word, over code_unit().
+constexpr float code_unit(Kv4Type type) { return type == kKv4BF16 ? kCodeUnit : 1.0f; }
 template <Kv4Type T>
 __device__ __forceinline__ typename Operand<T>::type decode(uint32_t w) {
-  const uint32_t p[4] = {w, w >> 4, w >> 8, __builtin_amdgcn_alignbit(w, w, 12)};
-  v4u r;
+  if constexpr (T == kKv4BF16) {
+    return decode_word_bf16(__builtin_amdgcn_alignbit(w, w, 3));
+  } else {
+    const uint32_t p[4] = {w, w >> 4, w >> 8, __builtin_amdgcn_alignbit(w, w, 12)};
+    v4u r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = T == kKv4F16 ? pair_f16(p[i]) : (T == kKv4BF16 ? pair_bf16_24(p[i]) : pair_bf16(p[i]));
-  return __builtin_bit_cast(typename Operand<T>::type, r);
+    for (int i = 0; i < 4; ++i) r[i] = T == kKv4F16 ? pair_f16(p[i]) : pair_bf16(p[i]);
+    return __builtin_bit_cast(typename Operand<T>::type, r);
+  }
 }
 
 // Eight elements of a row of x as they lie in memory.
@@ -174,19 +180,6 @@ __global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) vo
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int j = 0; j < kCols; ++j) operands<T>(t[c][j], b[c][j]);
-    v4f start[kGroups][kCols];
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        start[i][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (T == kKv4BF16) {
-          const v4u offset = {0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u};  // -24
-#pragma unroll
-          for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c)
-            start[i][j] = mfma(__builtin_bit_cast(v8b, offset), b[c][j][0], start[i][j]);
-        }
-      }
     // A row tile's sums meet their scales one row tile later, behind the next
     // one's decoding and products: MFMA results are not read right after they are
     // issued.
@@ -207,7 +200,7 @@ __global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) vo
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) sum[r % 2][i][j] = start[i][j];
+        for (int j = 0; j < kCols; ++j) sum[r % 2][i][j] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = i * 4 / kGroups; c < (i + 1) * 4 / kGroups; ++c) {
           const typename Operand<T>::type a = decode<T>(codes[r][c]);
@@ -274,6 +267,7 @@ __global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) vo
     if (n >= w.n || m >= rows) continue;
     float y = 0.0f;
     for (int v = 0; v < waves; ++v) y += s_acc[v * kPerWave + ((r * kCols + j) * 4 + e) * kWave + l];
+    y *= code_unit(T);
     if (w.bias != nullptr) y += w.bias[n];
     const int64_t at = m * out_row_stride + n;
     if constexpr (T == kKv4F32) static_cast<float*>(out)[at] = y;

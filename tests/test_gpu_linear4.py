@@ -160,3 +160,37 @@ def test_refusals(gpu):
                  (torch.zeros(64, device="cuda"), 32), (torch.full((4, 64), math.nan, device="cuda"), 32)):
         with pytest.raises(ValueError):
             pack_int4_groups(*args)
+
+
+# ------------------------------------------------- product by product
+#
+# No product may weigh on another column's: bounds by the products themselves.
+
+
+def _between(got, exp, tol):
+    """Every value is the rounding of one within tol of the expected (float64)."""
+    low, high = (exp - tol).to(got.dtype), (exp + tol).to(got.dtype)
+    off = ~((low <= got) & (got <= high))
+    assert not bool(off.any()), float(((got.double() - exp).abs() / tol)[off].max())
+
+
+def _check_by_products(got, x, w, group, bias=None):
+    """A group's sum is group exact products added in single precision; groups, waves
+    and the bias are added to it.  ``w`` is [n, k]; all in float64 on the GPU."""
+    x, w = x.cuda().double(), w.cuda().t().contiguous()
+    exp = x @ w + (0 if bias is None else bias.cuda().double())
+    mass = x.abs() @ w.abs() + (0 if bias is None else bias.cuda().double().abs())
+    _between(got, exp, 2.0**-24 * (group + w.shape[0] // group + 20) * mass + 1e-37)
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("m", [1, 7, 24])
+def test_large_inputs_under_zero_codes(gpu, kind, m):
+    """A column far larger than the others weighs nothing where its code is zero."""
+    codes, scales, w = _matrix(300, 512, 128)
+    codes[::2, 50] = 0  # columns 100 and 101
+    w[::2, 100:102] = 0.0
+    x = _rows(m, 512, kind)
+    x[:, 100] = 6e4 if kind == F16 else 1e7
+    x[:, 101] = -3e4 if kind == F16 else 1e8
+    _check_by_products(Int4Linear(codes.cuda(), scales.cuda())(x.cuda()), x, w, 128)
