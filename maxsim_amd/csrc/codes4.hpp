@@ -15,15 +15,15 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdg
 __device__ __forceinline__ v4f mfma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // A pair of codes, bits 3..6 of both halves.  Under a constant exponent they are
-// 136 + code in f16 and 24 + code in bfloat16 (the sign bit turned); the
+// 136 + code in f16 and (24 + code) / 1024 in bfloat16 (the sign bit turned); the
 // differences, in f16 and in single precision, are exact.
 __device__ __forceinline__ uint32_t pair_f16(uint32_t w) {
   const v2h base = {(_Float16)136.0f, (_Float16)136.0f};
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & 0x00780078u) ^ 0x58405840u) - base);
 }
 __device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
-  const uint32_t r = (w & 0x00780078u) ^ 0x41C041C0u;
-  const float lo = __uint_as_float(r << 16) - 24.0f, hi = __uint_as_float(r & 0xFFFF0000u) - 24.0f;
+  const uint32_t r = (w & 0x00780078u) ^ 0x3CC03CC0u;
+  const float base = 24.0f / 1024.0f, lo = __uint_as_float(r << 16) - base, hi = __uint_as_float(r & 0xFFFF0000u) - base;
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 

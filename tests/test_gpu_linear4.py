@@ -194,3 +194,17 @@ def test_large_inputs_under_zero_codes(gpu, kind, m):
     x[:, 100] = 6e4 if kind == F16 else 1e7
     x[:, 101] = -3e4 if kind == F16 else 1e8
     _check_by_products(Int4Linear(codes.cuda(), scales.cuda())(x.cuda()), x, w, 128)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 20])
+def test_largest_inputs(gpu, kind, group, m):
+    """Inputs up to the largest of their type, results well inside it."""
+    codes, scales, w = _matrix(40, 384, group)
+    scales, w = (scales.float() / 4096).to(BF16), w / 4096  # exactly
+    g = torch.Generator()
+    g.manual_seed(2)
+    x = ((2 * torch.rand((m, 384), generator=g) - 1) * 3.38e38).to(kind)
+    x[0] = torch.finfo(kind).max
+    _check_by_products(Int4Linear(codes.cuda(), scales.cuda())(x.cuda()), x, w, group)
