@@ -154,11 +154,6 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   // Query rows of this tile: row r is new token r / share, head r % share.
   v8h q[kCols][kParts][S::kKeyWords];
   float factor[kCols];       // of a product with the codes, towards log2 scores
-  // 16-bit queries meet codes with 72 added, and the sums start from -72 sum(q):
-  // two instructions less per word. It costs 72 / |c| times the rounding of four
-  // single precision sums, which single precision queries do not take.
-  constexpr bool kOffset = T != kKv4F32;
-  v4f start[kCols];
   int see_low[kCols], see_high[kCols];
   const uint8_t* mask[kCols];
   int64_t query[kCols];  // first element of the lane's row; -1: a row of padding
@@ -244,12 +239,6 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       }
     // Above zero, so that a hidden score stays minus infinity.
     factor[c] = fmaxf(ldexpf(fabsf(args.scale_log2), -shift), 1e-30f);
-    start[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (kOffset) {
-      const v4u minus72 = {0xD480D480u, 0xD480D480u, 0xD480D480u, 0xD480D480u};
-#pragma unroll
-      for (int i = 0; i < S::kKeyWords; ++i) start[c] = mfma(__builtin_bit_cast(v8h, minus72), q[c][0][i], start[c]);
-    }
   }
 
   float ref[kCols], sum[kCols];
@@ -292,7 +281,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     // Scores of the tile.
     v4f s[kCols][2];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) s[c][0] = s[c][1] = start[c];
+    for (int c = 0; c < kCols; ++c) s[c][0] = s[c][1] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t words[S::kKeyWords];
@@ -312,7 +301,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       }
 #pragma unroll
       for (int i = 0; i < S::kKeyWords; ++i) {
-        const v8h a = kOffset ? decode_word_72(words[i]) : decode_word(words[i]);
+        const v8h a = decode_word(words[i]);
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll

@@ -202,16 +202,6 @@ __device__ __forceinline__ v8h decode_word(uint32_t w) {
   return (v8h){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// The same with 72 added to every code: no subtraction, 64 + (code ^ 8) from bits
-// 4..7 of a half.
-__device__ __forceinline__ v8h decode_word_72(uint32_t w) {
-  const uint32_t p[4] = {w << 4, w, w >> 4, w >> 8};
-  v4u r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = (p[i] & 0x00F000F0u) ^ 0x54805480u;
-  return __builtin_bit_cast(v8h, r);
-}
-
 // The order of a word's codes in decode_word's result.
 __device__ __forceinline__ constexpr int word_order(int i) { return (i & 1) * 4 + i / 2; }
 

@@ -662,3 +662,51 @@ def test_refusals(gpu):
     cache.append(x[:0], x[:0], *none)
     assert cache.attend(q[:0], *none).shape == (0, 4, 64)
     assert cache.read(*none)[0].shape == (0, 2, 64)
+
+
+# --------------------------------------------------- product by product
+#
+# 16-bit queries are taken whole, and a probability times its value scale in 16 bits.
+
+
+def _check_by_products(cache, batch, q, got, got_lse=None, **kw):
+    """As _check, for 16-bit queries, by what the products themselves can lose: a score
+    is exact products added in single precision (a quarter of the dims, and four
+    roundings of factors), a probability times its scale keeps 2^-16.  Every result
+    is the rounding of one within that of the expected."""
+    out, lse, mass, _ = _expected(cache, batch, q, **kw)
+    share, dim = q.shape[1] // cache.kv_heads, cache.head_dim
+    scale = abs(kw.get("scale") or dim**-0.5)
+    delta = torch.zeros(q.shape[:2], dtype=torch.float64)
+    pool_k = _pool(cache)[0].abs()
+    for b, (n, m) in enumerate(zip(batch.host_lengths, batch.new)):
+        keep = torch.arange(n)
+        k = pool_k[batch.host_table[b].long()[keep // cache.page_size], :, keep % cache.page_size]  # [n, heads, dim]
+        rows = slice(int(batch.host_offsets[b]), int(batch.host_offsets[b]) + m)
+        for h in range(q.shape[1]) if n else ():
+            sums = (q[rows, h].cpu().double().abs() @ k[:, h // share].t()).amax(-1) * scale
+            delta[rows, h] = 2.0**-24 * (dim / 4 + 4) * sums + 2.0**-23
+    sums = 2.0**-24 * (max(batch.host_lengths) / 8 + 16)
+    tol = (2.0**-16 + 2 * delta[..., None] + 2 * sums) * mass + 1e-30
+    got = got.cpu()
+    off = ~(((out - tol).to(q.dtype) <= got) & (got <= (out + tol).to(q.dtype)))
+    assert not bool(off.any()), (int(off.sum()), float(((got.double() - out).abs() / tol)[off].max()))
+    if got_lse is not None:
+        seen = ~torch.isinf(lse)
+        assert bool(((got_lse.cpu().double() - lse).abs() <= delta + sums + 2.0**-22 * (1 + lse.abs()))[seen].all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 1), (128, 9), (256, 3), (128, 300)])
+def test_large_queries_over_zero_codes(gpu, kind, dim, rows):
+    """A channel of the queries that is far larger than the others weighs nothing
+    where the keys' codes are zero."""
+    cache = Int4KVCache(12, 1, dim, page_size=32)
+    _fill(cache, 3)
+    cache.k_codes[..., 5] = 0  # channels 10 and 11
+    batch = Batch(cache, [310], [rows], seed=1)
+    q = _queries(rows, 8, dim, kind, 2, size=4.0)
+    q[..., 10] = 6e4 if kind == F16 else 1e7
+    q[..., 11] = 6e4 if kind == F16 else 3e6
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check_by_products(cache, batch, q, got, lse)
