@@ -314,7 +314,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     for (int h = 0; h < 2; ++h) {
       const v4f* scales = reinterpret_cast<const v4f*>(now + L::kScales + h * 64);
       key_scale[h] = scales[g];
-      value_scale[h] = scales[8 + g];
+      value_scale[h] = scales[8 + g] * (1.0f / kValueUnit);
     }
     mfma_results_fence();
 
@@ -409,10 +409,6 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     for (int i = 0; i < kAhead; ++i) hole[i][0] = hole[i + 1][0], hole[i][1] = hole[i + 1][1];
   }
   mfma_results_fence();
-#pragma unroll
-  for (int c = 0; c < kCols; ++c)
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) o[c][t] *= kCodeUnit;
 
   // The waves' results joined in their order, in LDS.
   float* s_ref = reinterpret_cast<float*>(s_raw);  // [waves][rows]
@@ -467,7 +463,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     const int64_t row = u.first + token;
     if (args.lse != nullptr && d == 0)
       args.lse[row * args.heads + qh] = log_sum(all, total);
-    sum4 *= total == 0.0f ? 0.0f : 1.0f / total;
+    sum4 *= output_factor(total);
     store4<T>(args.out, row * args.out_row_stride + (int64_t)qh * args.out_head_stride + d, args.out_wide != 0, sum4);
   }
 }
@@ -575,7 +571,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
     }
     if (direct || wave == 0) {
       const int64_t row = item.first + token;
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      const float inv = output_factor(total);
       if (args.lse != nullptr && lane == 0) args.lse[row * args.heads + qh] = log_sum(all, total);
       const int64_t base = row * args.out_row_stride + (int64_t)qh * args.out_head_stride;
 #pragma unroll

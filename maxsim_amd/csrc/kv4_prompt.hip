@@ -107,7 +107,7 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
           decode_word(s.words[i]);
     }
     float* scales = reinterpret_cast<float*>(buffer + B::kScales);
-    scales[thread] = s.scale;
+    scales[thread] = thread < kKeys ? s.scale : s.scale * (1.0f / kValueUnit);
     if (thread < kKeys) scales[2 * kKeys + key] = s.hole ? 1.0f : 0.0f;
   } else if (thread % 16 < kDim / 8) {
     const int w = thread % 16, kg = (thread - 256) / 16;
@@ -342,7 +342,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     const int tok = (int)(row / split.share), qh = at.head * split.share + (int)(row - tok * split.share);
     const float all = __shfl(ref, local), total = __shfl(sum, local);
     if (tok >= u.rows) continue;
-    v4f y = *reinterpret_cast<const v4f*>(mine + local * kPitch + d) * kCodeUnit;
+    v4f y = *reinterpret_cast<const v4f*>(mine + local * kPitch + d);
     if (!whole_item) {
       float* dst = partial_slot(partial, split, kDim, blockIdx.x, from == 0);
       *reinterpret_cast<v4f*>(dst + (wave * 32 + local) * kDim + d) = y;
@@ -354,7 +354,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     }
     const int64_t out_row = u.first + tok;
     if (args.lse != nullptr && d == 0) args.lse[out_row * args.heads + qh] = log_sum(all, total);
-    y *= total == 0.0f ? 0.0f : 1.0f / total;
+    y *= output_factor(total);
     store4<T>(args.out, out_row * args.out_row_stride + (int64_t)qh * args.out_head_stride + d, args.out_wide != 0, y);
   }
 }

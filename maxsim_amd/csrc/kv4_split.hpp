@@ -10,9 +10,14 @@
 namespace msim {
 
 constexpr float kUnset = -FLT_MAX;
-// A row's reference moves, to its largest score, when a probability passes 2^6
-// (the moves cost nothing that shows: limits up to 2^40 took the same time).
+// A row's reference moves, to its largest score, when a probability passes 2^6 (limits
+// up to 2^40 took the same time; 2^2 took 1.5 % more at prompts).
 constexpr float kTopLimit = 6.0f;
+// Value scales are taken over 2^20 and codes over kCodeUnit, so that the sums of
+// probabilities times values stay numbers before they are divided, for 2^18 keys and
+// values of any size.  The other end: the 16 bits of a product hold from values of
+// 2^-94 up.
+constexpr float kValueUnit = 0x1p20f;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -283,7 +288,10 @@ __device__ __forceinline__ float max_of(const float (&x)[N]) {
   return fmaxf(m, x[N - 1]);
 }
 
-// A row of the output, and of lse, by the last sums.
+// What an output row's sums are multiplied by, and its lse, by the last sums.
+__device__ __forceinline__ float output_factor(float total) {
+  return total == 0.0f ? 0.0f : kCodeUnit * kValueUnit / total;
+}
 __device__ __forceinline__ float log_sum(float ref, float total) {
   return total == 0.0f ? kNegInf : (ref + __log2f(total)) * 0.69314718055994531f;
 }

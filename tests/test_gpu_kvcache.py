@@ -710,3 +710,18 @@ def test_large_queries_over_zero_codes(gpu, kind, dim, rows):
     q[..., 11] = 6e4 if kind == F16 else 3e6
     got, lse = cache.attend(q, *batch.args, return_lse=True)
     _check_by_products(cache, batch, q, got, lse)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("lengths,new", [([300], [1]), ([3000], [1]), ([400], [20]), ([700], [300])])
+def test_largest_values(gpu, kind, lengths, new):
+    """Values up to nearly the largest number of the type, over scores that rise along the keys."""
+    cache = Int4KVCache(50, 1, 128, page_size=64)
+    _fill(cache, 3)
+    batch = Batch(cache, lengths, new, seed=1)
+    for pos in range(lengths[0]):
+        cache.k_scales[int(batch.host_table[0, pos // 64]), 0, pos % 64] = 0.1 + 0.4 * pos / lengths[0]
+    cache.v_scales.fill_(4.5e37)
+    q = _queries(batch.rows, 8, 128, kind, 2, size=0.5)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check(cache, batch, q, got, lse)
