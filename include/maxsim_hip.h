@@ -449,7 +449,8 @@ int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t 
  * != 0 (mask NULL: all; keys past mask_width are hidden).  out = softmax(scale
  * q.k) v in the queries' type; lse f32 [rows, heads] (NULL: not wanted) the
  * logarithm of the softmax's sum.  A row that sees nothing: zeros, -infinity.
- * The workspace (16-byte aligned) is used until the call's work is done. */
+ * The workspace (16-byte aligned) is used until the call's work is done.  out may be
+ * q itself (same pointer and strides), and must not overlap it otherwise. */
 int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
                           const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
                           const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads, int type,
@@ -473,7 +474,7 @@ int msim_linear4_layout_async(const uint8_t* codes, const uint16_t* scales, int6
 /* x [rows, k] (row stride in elements) times the matrix's rows, sums in single
  * precision, rounded once to `type` into out [rows, n].  bias f32 [n] or NULL.
  * Meant for few rows (it reads the matrix once per 32 of them); an infinity in x
- * may come out as a NaN. */
+ * may come out as a NaN.  x and out must not overlap. */
 int msim_linear4_async(const uint8_t* codes, const uint16_t* scales, int64_t n, int64_t k, int64_t group,
                        const float* bias, const void* x, int64_t rows, int64_t x_row_stride, int type, void* out,
                        int64_t out_row_stride, void* stream);

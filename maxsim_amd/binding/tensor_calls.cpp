@@ -13,6 +13,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+#include <cstdlib>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -146,6 +149,46 @@ const at::Tensor& row_tensor(const Cache& c, PyObject* o, const char* name, int6
   return t;
 }
 
+// First byte of a tensor's elements and the one behind its last (strides are not negative).
+struct Span {
+  uintptr_t first = 0, last = 0;
+  explicit Span(const at::Tensor& t) {
+    if (t.numel() == 0) return;
+    int64_t most = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) most += (t.size(d) - 1) * t.stride(d);
+    first = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    last = first + (most + 1) * t.element_size();
+  }
+  bool meets(const Span& o) const { return first < o.last && o.first < last; }
+};
+
+// Whether two tensors [rows, heads, dim] of one type share memory, other than an element
+// with itself if `in_place`.  Views of one buffer may lie between each other: with equal
+// strides the rows and heads that far apart are looked for, other strides count as shared.
+bool share_memory(const at::Tensor& a, const at::Tensor& b, bool in_place) {
+  if (!Span(a).meets(Span(b))) return false;
+  int64_t step[2];
+  for (int d = 0; d < 2; ++d) {
+    step[d] = a.size(d) > 1 ? a.stride(d) : b.stride(d);
+    if (b.size(d) > 1 && b.stride(d) != step[d]) return true;
+  }
+  const int64_t dim = a.size(2), size = a.element_size();
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.const_data_ptr()) - reinterpret_cast<intptr_t>(a.const_data_ptr());
+  if (bytes % size != 0) return true;
+  for (int64_t h = 1 - b.size(1); h < a.size(1); ++h) {
+    const int64_t low = 1 - b.size(0), high = a.size(0) - 1;
+    const int64_t away = bytes / size - h * step[1], near = step[0] > 0 ? away / step[0] : 0;
+    const int64_t i0 = std::clamp(near, low, high);  // rows of that distance, or nearly
+    for (int64_t i = std::max(low, i0 - 1); i <= std::min(high, i0 + 1); ++i)
+      if (!(in_place && bytes == 0 && h == 0 && i == 0) && std::abs(i * step[0] - away) < dim) return true;
+  }
+  return false;
+}
+
+void check_output(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!share_memory(t, t, true), name, " must not overlap itself");
+}
+
 void same_rows(const at::Tensor& k, const at::Tensor& v, const char* what) {
   TORCH_CHECK_VALUE(k.scalar_type() == v.scalar_type() && k.size(0) == v.size(0), what,
                     " must have the same shape and dtype");
@@ -234,6 +277,9 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     k = row_tensor(c, a[6], "out[0]", c.pool.kv_heads);
     v = row_tensor(c, a[7], "out[1]", c.pool.kv_heads);
     same_rows(k, v, "both outputs");
+    check_output(k, "out[0]");
+    check_output(v, "out[1]");
+    TORCH_CHECK_VALUE(!share_memory(k, v, false), "out[0] and out[1] must not overlap");
   }
   const Batch b = read_batch(c, a[1], a[2], a[3], k.size(0));
   const Launch launch(c.device);
@@ -274,6 +320,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else {
     out = row_tensor(c, a[9], "out", heads);
     TORCH_CHECK_VALUE(out.scalar_type() == q.scalar_type() && out.size(0) == rows, "out must have q's shape and dtype");
+    check_output(out, "out");
+    // In place of q is fine: a workgroup writes rows that it alone read, or the join does.
+    TORCH_CHECK_VALUE(!share_memory(out, q, true), "out must not overlap q, unless it is q");
   }
   const bool want_lse = a[10] == Py_True;
   if (want_lse) lse = at::empty({rows, heads}, at::TensorOptions().device(c.device).dtype(at::kFloat));
@@ -331,6 +380,17 @@ PyObject* multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(sizes) && out.scalar_type() == x.scalar_type() &&
                           out.device() == x.device() && out.is_contiguous(),
                       "out must be a contiguous tensor of the result's shape, x's dtype and device");
+    // Out is one piece of memory: it meets x where it meets one of x's rows.
+    const Span to(out), from(*m);
+    bool meets = to.meets(from);
+    if (meets && m->size(0) > 1 && m->stride(0) > 0) {
+      const int64_t step = m->stride(0) * x.element_size(), bytes = w.k * x.element_size();
+      // The first row that ends behind out's start.
+      const int64_t before = (int64_t)(to.first - from.first) - bytes;
+      const int64_t row = to.first < from.first + bytes ? 0 : before / step + 1;
+      meets = row < m->size(0) && from.first + row * step < to.last;
+    }
+    TORCH_CHECK_VALUE(!meets, "out must not overlap x");
   }
   const Launch launch(x.device());
   check(abi.linear(static_cast<const uint8_t*>(w.codes.const_data_ptr()),

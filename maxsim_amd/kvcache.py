@@ -144,7 +144,8 @@ class Int4KVCache:
         head_dim ** -0.5.  Returns [rows, heads, head_dim] in q's dtype, rounded
         once from single precision sums, and with ``return_lse`` the logarithm
         of each softmax's sum, float32 [rows, heads].  A row that sees nothing
-        is zeros, with minus infinity.
+        is zeros, with minus infinity.  ``out`` may be q itself, and must not
+        overlap it otherwise.
         """
         if window is not None and window < 1:
             raise ValueError("window must be positive")

@@ -86,6 +86,7 @@ class Int4Linear:
     def __call__(self, x, out=None):
         """x [..., in_features] (float32, float16 or bfloat16) to [...,
         out_features] in x's dtype: sums in single precision, rounded once.
+        ``out`` is contiguous and does not overlap x.
         Enqueued on the current stream; records no gradients.  Meant for few
         rows: the matrix is read once per 32 of them."""
         return self._calls.multiply(self._handle, x, out)

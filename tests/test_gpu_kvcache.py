@@ -725,3 +725,32 @@ def test_largest_values(gpu, kind, lengths, new):
     q = _queries(batch.rows, 8, 128, kind, 2, size=0.5)
     got, lse = cache.attend(q, *batch.args, return_lse=True)
     _check(cache, batch, q, got, lse)
+
+
+# ------------------------------------------------ outputs over inputs
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 300]])
+def test_outputs_that_overlap(gpu, new):
+    """In place of the queries and between them, but not across."""
+    cache = Int4KVCache(90, 2, 64, page_size=16)
+    _fill(cache, 1)
+    batch = Batch(cache, [700, 20, 310], new, seed=1)
+    rows = batch.rows
+    fused = _queries(rows + 1, 8, 64, BF16, 2)
+    exp = cache.attend(fused[:rows, :4], *batch.args)
+    q, other = fused[:rows, :4], fused[:rows, 4:]
+    assert torch.equal(cache.attend(q, *batch.args, out=other), exp)  # row by row beside q
+    for out in (fused[1:, :4], fused[:rows, 1:5], fused[:rows, 3:7], fused.view(-1)[1:1 + rows * 256].view(rows, 4, 64),
+                fused.view(-1)[8:].as_strided(q.shape, q.stride()), exp[:1].expand(rows, 4, 64) if rows > 1 else exp[:, :1],
+                exp[:, :1].expand(rows, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attend(q, *batch.args, out=out)
+    assert torch.equal(cache.attend(q, *batch.args, out=q), exp) and torch.equal(q, exp)
+    both = torch.zeros((rows, 2, 2, 64), dtype=BF16, device="cuda")
+    k, v = cache.read(*batch.args, rows=rows)
+    cache.read(*batch.args, out=(both[:, 0], both[:, 1]))
+    assert torch.equal(both[:, 0], k) and torch.equal(both[:, 1], v)
+    for out in ((k, k), (k[:1].expand(rows, 2, 64), v), (both[:, 0], both.view(-1)[2:].as_strided(k.shape, both[:, 0].stride()))):
+        with pytest.raises(ValueError, match="overlap"):
+            cache.read(*batch.args, out=out)

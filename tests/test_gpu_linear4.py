@@ -208,3 +208,23 @@ def test_largest_inputs(gpu, kind, group, m):
     x = ((2 * torch.rand((m, 384), generator=g) - 1) * 3.38e38).to(kind)
     x[0] = torch.finfo(kind).max
     _check_by_products(Int4Linear(codes.cuda(), scales.cuda())(x.cuda()), x, w, group)
+
+
+def test_outputs_that_overlap_inputs(gpu):
+    """An output over x is refused; one between the rows of x is not."""
+    codes, scales, w = _matrix(128, 128, 32)
+    linear = Int4Linear(codes.cuda(), scales.cuda())
+    wide = _rows(3, 500, F32)
+    flat = wide.cuda().view(-1)
+    x = flat.view(3, 500)[:, :128]
+    for out in (flat[:384], flat[127:511], flat[500:884], flat[1000 + 100:1000 + 484], flat[400:784]):
+        with pytest.raises(ValueError, match="overlap"):
+            linear(x, out=out.view(3, 128))
+    with pytest.raises(ValueError, match="overlap"):
+        linear(x[0], out=x[0])
+    square = x.contiguous()
+    with pytest.raises(ValueError, match="overlap"):
+        linear(square, out=square)
+    _check_by_products(linear(x, out=torch.empty_like(square)), x.cpu(), w, 32)
+    _check_by_products(linear(x[:2], out=flat[128:128 + 256].view(2, 128)), wide[:2, :128], w, 32)  # in row 0's gap
+    assert torch.equal(x.cpu(), wide[:, :128])
