@@ -429,7 +429,9 @@ typedef struct msim_kv4_pool {
 #define MSIM_BF16 2
 
 /* Keys and values [rows, kv_heads, dim] (strides in elements, dims dense)
- * quantised into the cache.  Rows that share a slot leave one of them. */
+ * quantised into the cache.  A slot that two rows of a call share (overlapping
+ * pages) is left with parts of both: codes of one under the scale of the other,
+ * heads of either, the key of one beside the value of the other. */
 int msim_kv4_append_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
                           const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
                           const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,

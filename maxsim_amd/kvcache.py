@@ -113,7 +113,9 @@ class Int4KVCache:
     def append(self, k, v, page_table, lengths, offsets=None) -> None:
         """Quantise keys and values [rows, kv_heads, head_dim] (float32, float16
         or bfloat16, any strides with dense rows) into the cache.  A row that
-        holds an infinity or a NaN reads back as NaN."""
+        holds an infinity or a NaN reads back as NaN.  Sequences may share pages
+        that are only read: a slot given to two rows of one call is left with
+        parts of both."""
         self._calls.append(self._handle, k, v, page_table, lengths, offsets)
 
     def read(self, page_table, lengths, offsets=None, *, rows=None, dtype=None, out=None):

@@ -288,6 +288,23 @@ def test_holes_and_bad_indices(gpu):
     assert not bool(got.any())
 
 
+def test_slots_given_to_two_rows(gpu):
+    """Words and scales of either row in the shared slots, and nothing elsewhere."""
+    caches = [Int4KVCache(4, 3, 128, page_size=16) for _ in range(3)]
+    table = torch.tensor([[1], [1]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([9, 9], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, 5, 10], dtype=torch.int32, device="cuda")
+    x = (torch.randn((10, 3, 128), generator=_rng(1)) * torch.arange(1, 11)[:, None, None]).cuda()
+    caches[0].append(x, -x, table, lengths, offsets)
+    for cache, rows in zip(caches[1:], (x[:5], x[5:])):
+        cache.append(rows, -rows, table[:1], lengths[:1], offsets[:2])
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        got, one, other = (getattr(cache, name) for cache in caches)
+        if name.endswith("codes"):
+            got, one, other = (t.view(torch.int32) for t in (got, one, other))
+        assert bool(((got == one) | (got == other)).all())
+
+
 # ------------------------------------------------------------- attention
 
 
