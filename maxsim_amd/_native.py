@@ -188,14 +188,15 @@ def tensor_calls():
     global _calls
     if _calls is not None:
         return _calls
-    import torch  # noqa: F401  (its libraries come first)
+    import torch  # its libraries come first
 
     lib = load()
     try:
         from maxsim_amd import _tensor_calls
     except ImportError as exc:
-        raise NativeLibraryMissing(
-            f"{os.path.join(HERE, '_tensor_calls.so')} is not built; run `python -m maxsim_amd.build`") from exc
+        path = os.path.join(HERE, "_tensor_calls.so")
+        why = f"cannot be loaded beside torch {torch.__version__} ({exc})" if os.path.exists(path) else "is not built"
+        raise NativeLibraryMissing(f"{path} {why}; run `python -m maxsim_amd.build`") from exc
     names = ("msim_last_error", "msim_kv4_append_async", "msim_kv4_read_async", "msim_kv4_attend_workspace",
              "msim_kv4_attend_async", "msim_linear4_async")
     _tensor_calls.setup(*(ctypes.cast(getattr(lib, name), c_vp).value for name in names))

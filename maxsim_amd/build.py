@@ -63,6 +63,13 @@ def binding_command(out: str) -> list[str]:
             "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python"]
 
 
+def _binding_command_or_none(out: str) -> list[str] | None:
+    try:
+        return binding_command(out)
+    except ImportError:
+        return None
+
+
 def sources() -> list[str]:
     names = sorted(os.listdir(CSRC))
     return [os.path.join(CSRC, n) for n in names if n.endswith((".hip", ".cpp"))]
@@ -86,12 +93,15 @@ def build(verbose: bool = False) -> str:
             print(f"compiling {len(srcs)} sources with {jobs} jobs: " + " ".join(cmds[0][:-4]), flush=True)
         rates_tmp = RATES_LIB + ".tmp"
         cmds.append([hipcc, *FLAGS, RATES_SRC, "-o", rates_tmp])
+        # The library needs no torch: without it, or where the module does not
+        # compile, the C ABI is built all the same.
         binding_tmp = BINDING + ".tmp"
-        cmds.append(binding_command(binding_tmp))
+        binding = _binding_command_or_none(binding_tmp)
         with ThreadPoolExecutor(max_workers=jobs) as pool:
+            binding_result = pool.submit(_run, binding) if binding else None
             results = list(pool.map(_run, cmds))
         messages: list[str] = []
-        for src, (rc, lines) in zip(srcs + [RATES_SRC, BINDING_SRC], results):
+        for src, (rc, lines) in zip(srcs + [RATES_SRC], results):
             if rc != 0:
                 raise RuntimeError(f"compiler failed on {os.path.basename(src)}:\n" + "\n".join(lines))
             messages.extend(lines)
@@ -100,11 +110,18 @@ def build(verbose: bool = False) -> str:
         if rc != 0:
             raise RuntimeError("hipcc link failed:\n" + "\n".join(lines))
         messages.extend(lines)
+    if binding is None:
+        messages.append(f"torch cannot be imported: {os.path.basename(BINDING)} (Int4KVCache, Int4Linear) is not built")
     if verbose and messages:
         print("\n".join(messages))
     os.replace(tmp, LIB)
     os.replace(rates_tmp, RATES_LIB)
-    os.replace(binding_tmp, BINDING)
+    if binding_result is not None:
+        rc, lines = binding_result.result()
+        if rc != 0:
+            raise RuntimeError(f"compiler failed on {os.path.basename(BINDING_SRC)} (the library is built):\n"
+                               + "\n".join(lines))
+        os.replace(binding_tmp, BINDING)
     return LIB
 
 
