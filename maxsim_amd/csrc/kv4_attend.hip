@@ -472,10 +472,13 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 template <Kv4Type T, int kDim, int kCols>
 __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
                                                                    Split split, float* __restrict__ partial) {
+  if (__builtin_expect(blockIdx.x >= split.workers, 0)) {
+    loose_rows<T, kDim>(batch, args, split);
+    return;
+  }
   Deal deal;
   Cursor at;
   if (!find_work(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
-    if (blockIdx.x == gridDim.x - 1) loose_rows<T>(pool, batch, args);  // this workgroup never has work
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
@@ -627,8 +630,8 @@ hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const S
 template <Kv4Type T, int kDim, int kCols>
 hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                          float* partial, hipStream_t stream) {
-  kv4_attend_kernel<T, kDim, kCols><<<dim3(split.workers + 1), dim3(kWaves * kWave), 0, stream>>>(pool, batch, args,
-                                                                                                split, partial);
+  const dim3 grid(split.workers + loose_groups(batch)), block(kWaves * kWave);
+  kv4_attend_kernel<T, kDim, kCols><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
   return hipGetLastError();
 }
 

@@ -366,10 +366,13 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   constexpr int kOutputs = kPromptRows * (kDim + 4) * 4;
   __shared__ __attribute__((aligned(16)))
   char s_raw[2 * Buffer<kDim>::kBytes > kOutputs ? 2 * Buffer<kDim>::kBytes : kOutputs];
+  if (__builtin_expect(blockIdx.x >= split.workers, 0)) {
+    loose_rows<T, kDim>(batch, args, split);
+    return;
+  }
   Deal deal;
   Cursor at;
   if (!find_work(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
-    if (blockIdx.x == gridDim.x - 1) loose_rows<T>(pool, batch, args);  // this workgroup never has work
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
 template <Kv4Type T>
 hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                   float* partial, hipStream_t stream) {
-  const dim3 grid(split.workers + 1), block(kPromptWaves * kWave);
+  const dim3 grid(split.workers + loose_groups(batch)), block(kPromptWaves * kWave);
   switch (pool.dim) {
     case 64: kv4_prompt_kernel<T, 64><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
     case 96: kv4_prompt_kernel<T, 96><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;

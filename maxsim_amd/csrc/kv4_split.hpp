@@ -2,6 +2,7 @@
 // work is dealt out, queries read and outputs written.
 #pragma once
 
+#include <algorithm>
 #include <cfloat>
 
 #include "codes4.hpp"
@@ -296,18 +297,24 @@ __device__ __forceinline__ float log_sum(float ref, float total) {
   return total == 0.0f ? kNegInf : (ref + __log2f(total)) * 0.69314718055994531f;
 }
 
-// Rows of no sequence come out as rows that see nothing.
-template <Kv4Type T>
-__device__ __forceinline__ void loose_rows(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args) {
-  if (batch.offsets == nullptr) return;
+// Rows of no sequence come out as rows that see nothing: a padded batch has many.  They
+// belong to workgroups of their own behind the workers, one per 64 rows of the call, up
+// to 256 (one that did them all held a call of 8 rows behind 3,000 keys and 4,088 loose
+// ones, 32 heads of 128, for 4,500 us; these make it 69).
+inline uint32_t loose_groups(const Kv4Batch& batch) {
+  return batch.offsets == nullptr ? 0 : std::min(std::max(1, batch.rows / 64), 256);
+}
+template <Kv4Type T, int kDim>
+__device__ __forceinline__ void loose_rows(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split) {
   const int first = kv4_first_row(batch, 0), last = max(first, kv4_first_row(batch, batch.batch));
-  for (int row = 0; row < batch.rows; ++row) {
-    if (row == first) row = last;
-    if (row >= batch.rows) break;
-    for (int i = threadIdx.x; i < args.heads * pool.dim; i += blockDim.x)
-      store_out<T>(args.out, row * args.out_row_stride + i / pool.dim * args.out_head_stride + i % pool.dim, 0.0f);
+  const int step = (int)(gridDim.x - split.workers), count = first + batch.rows - last;
+  for (int i = (int)(blockIdx.x - split.workers); i < count; i += step) {
+    const int64_t row = i < first ? i : i - first + last;
+    for (int j = threadIdx.x; j < args.heads * (kDim / 4); j += blockDim.x)
+      store4<T>(args.out, row * args.out_row_stride + j / (kDim / 4) * args.out_head_stride + j % (kDim / 4) * 4,
+                args.out_wide != 0, (v4f){0.0f, 0.0f, 0.0f, 0.0f});
     for (int h = threadIdx.x; h < args.heads && args.lse != nullptr; h += blockDim.x)
-      args.lse[(int64_t)row * args.heads + h] = kNegInf;
+      args.lse[row * args.heads + h] = kNegInf;
   }
 }
 

@@ -771,3 +771,25 @@ def test_outputs_that_overlap(gpu, new):
     for out in ((k, k), (k[:1].expand(rows, 2, 64), v), (both[:, 0], both.view(-1)[2:].as_strided(k.shape, both[:, 0].stride()))):
         with pytest.raises(ValueError, match="overlap"):
             cache.read(*batch.args, out=out)
+
+
+# --------------------------------------------------- rows of no sequence
+
+
+@pytest.mark.parametrize("kind,new", [(BF16, [1, 2]), (BF16, [300, 700]), (F32, [300, 5]), (F16, [0, 0])])
+@pytest.mark.parametrize("before,behind", [(0, 4000), (3000, 0), (129, 1000)])
+def test_padded_batches(gpu, kind, new, before, behind):
+    """Many rows before the first offset and behind the last, in strided outputs."""
+    cache = Int4KVCache(80, 1, 64, page_size=16)
+    _fill(cache, 1)
+    batch = Batch(cache, [320, 700], new, seed=1)
+    rows = before + batch.rows + behind
+    q = _queries(rows, 6, 64, kind, 2)
+    out = torch.full((rows, 6, 70), 3.0, dtype=kind, device="cuda")
+    _, lse = cache.attend(q, batch.table, batch.lengths, batch.offsets + before, out=out[..., 1:65], return_lse=True)
+    used = slice(before, before + batch.rows)
+    if batch.rows:
+        _check(cache, batch, q[used], out[used, :, 1:65], lse[used])
+    for loose in (slice(0, before), slice(before + batch.rows, rows)):
+        assert not bool(out[loose, :, 1:65].any()) and bool((lse[loose] == -math.inf).all())
+    assert bool((out[..., 0] == 3).all()) and bool((out[..., 65:] == 3).all())
