@@ -228,3 +228,44 @@ def test_outputs_that_overlap_inputs(gpu):
     _check_by_products(linear(x, out=torch.empty_like(square)), x.cpu(), w, 32)
     _check_by_products(linear(x[:2], out=flat[128:128 + 256].view(2, 128)), wide[:2, :128], w, 32)  # in row 0's gap
     assert torch.equal(x.cpu(), wide[:, :128])
+
+
+# ------------------------------------------------------- shapes of tiles
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("group,k", [(32, 416), (64, 448), (128, 384)])
+def test_row_tiles_of_a_workgroup(gpu, kind, group, k):
+    """Widths at which workgroups have one, two, four and seven row tiles (256 CUs), the
+    last of them partly or wholly past the end; rows of one and two column tiles."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(k)
+    for n in (4081, 8163, 16345, 28629):
+        w = torch.randn((n, k), generator=g, device="cuda")
+        codes, scales = pack_int4_groups(w, group)
+        bias = torch.randn(n, generator=g, device="cuda")
+        linear = Int4Linear(codes, scales, bias)
+        c = torch.stack((codes & 15, codes >> 4), -1).flatten(1).to(torch.int8)
+        w = torch.where(c > 7, c - 16, c).double() * scales.double().repeat_interleave(group, 1)
+        for m in (1, 5, 16, 19, 32, 75):
+            x = torch.randn((m, k), generator=g, device="cuda").to(kind)
+            out = torch.full((m + 1, n), 7.0, dtype=kind, device="cuda")
+            linear(x, out=out[:m])
+            _check_by_products(out[:m], x, w, group, bias)
+            assert bool((out[m] == 7).all())
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("m,n", [(32, 28672), (17, 28629), (1, 28672), (16, 16345)])
+def test_row_tiles_and_many_waves(gpu, kind, m, n):
+    """As many row tiles as the registers hold and eight or sixteen waves, which join in
+    up to 112 KiB of LDS."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n + m)
+    codes = torch.randint(0, 256, (n, 512), generator=g, device="cuda", dtype=torch.uint8)  # -8 too
+    scales = (0.01 * (1 + torch.rand((n, 8), generator=g, device="cuda"))).to(BF16)
+    linear = Int4Linear(codes, scales)
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(1).to(torch.int8)
+    w = torch.where(c > 7, c - 16, c).double() * scales.double().repeat_interleave(128, 1)
+    x = torch.randn((m, 1024), generator=g, device="cuda").to(kind)
+    _check_by_products(linear(x), x, w, 128)
