@@ -793,3 +793,52 @@ def test_padded_batches(gpu, kind, new, before, behind):
     for loose in (slice(0, before), slice(before + batch.rows, rows)):
         assert not bool(out[loose, :, 1:65].any()) and bool((lse[loose] == -math.inf).all())
     assert bool((out[..., 0] == 3).all()) and bool((out[..., 65:] == 3).all())
+
+
+# ------------------------------------------ shapes that the others miss
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [64, 192, 256])
+@pytest.mark.parametrize("length,new", [(20011, 1), (9100, 3)])
+def test_joins_of_many_parts(gpu, kind, dim, length, new):
+    """One key/value head: more parts of an item than a wave joins at once."""
+    cache = Int4KVCache(-(-length // 128), 1, dim, page_size=128)
+    _fill(cache, 2)
+    batch = Batch(cache, [length], [new], seed=2)
+    q = _queries(new, 8, dim, kind, 3)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check(cache, batch, q, got, lse)
+    if kind != F32:
+        _check_by_products(cache, batch, q, got, lse)
+    mask = torch.zeros((new, length), dtype=torch.bool, device="cuda")
+    mask[:, 5000:5002] = True  # two keys of one part
+    got, lse = cache.attend(q, *batch.args, mask=mask, return_lse=True)
+    _check(cache, batch, q, got, lse, mask=mask)
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("causal,window", [(True, None), (False, 50)])
+def test_many_tokens_of_192_dims(gpu, kind, causal, window):
+    cache = Int4KVCache(64, 2, 192, page_size=16)
+    _fill(cache, 6)
+    batch = Batch(cache, [75, 64, 0, 130, 5, 33], [75, 1, 0, 37, 5, 2], seed=1)
+    q = _queries(batch.rows, 6, 192, kind, 3)
+    got, lse = cache.attend(q, *batch.args, causal=causal, window=window, return_lse=True)
+    _check(cache, batch, q, got, lse, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("lengths,new", [((201, 60), (2, 1)), ((700, 400), (600, 400))])
+def test_all_bits_of_the_products(gpu, kind, dim, lengths, new):
+    """Rows of zeros under large value scales, others 2^-24 of them: single tokens and
+    prompts of two workgroups' rows."""
+    cache, batch = _prompts(dim, 32, 5, lengths=lengths, new=new)
+    q = _queries(batch.rows, 4, dim, kind, 3, size=2.0)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check_by_products(cache, batch, q, got, lse)
+    cache.v_scales.mul_(torch.exp2(torch.randint(-12, 13, cache.v_scales.shape, generator=_rng(1)).float()).cuda())
+    cache.v_codes[::2, :, ::3] = 0
+    _check_by_products(cache, batch, q, cache.attend(q, *batch.args))
+    _check_by_products(cache, batch, q, cache.attend(q, *batch.args, scale=-0.3), scale=-0.3)
