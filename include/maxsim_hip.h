@@ -451,6 +451,7 @@ int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t 
  * != 0 (mask NULL: all; keys past mask_width are hidden).  out = softmax(scale
  * q.k) v in the queries' type; lse f32 [rows, heads] (NULL: not wanted) the
  * logarithm of the softmax's sum.  A row that sees nothing: zeros, -infinity.
+ * Queries and values may have any size, keys up to 2^102 (about 5e30).
  * The workspace (16-byte aligned) is used until the call's work is done.  out may be
  * q itself (same pointer and strides), and must not overlap it otherwise. */
 int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,

@@ -237,8 +237,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
         q[c][0][i][j] = hi;
         if constexpr (kParts == 2) q[c][1][i][j] = (_Float16)(y - (float)hi);
       }
-    // Above zero, so that a hidden score stays minus infinity.
-    factor[c] = fmaxf(ldexpf(fabsf(args.scale_log2), -shift), 1e-30f);
+    factor[c] = score_factor(args.scale_log2, shift);
   }
 
   float ref[kCols], sum[kCols];

@@ -197,8 +197,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
         const float x = value(raw[i][word_order(j) / 2], word_order(j));
         q[i][j] = (_Float16)ldexpf(args.scale_log2 < 0.0f ? -x : x, shift);
       }
-    // It stays above zero, so that a hidden score stays minus infinity.
-    factor = fmaxf(ldexpf(fabsf(args.scale_log2), -shift), 1e-30f);
+    factor = score_factor(args.scale_log2, shift);
   }
   const int pos = u.length - u.rows + token;
   int see_low = pos >= args.window ? pos - args.window + 1 : 0;

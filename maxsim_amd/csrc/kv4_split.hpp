@@ -265,8 +265,14 @@ __device__ __forceinline__ void store4(void* out, int64_t i, bool wide, v4f x) {
 }
 
 // Multiplies a query row to f16's range: the exponent to add (its largest entry
-// in [2^14, 2^15)) from the bits of that entry.
-__device__ __forceinline__ int query_shift(uint32_t top) { return 141 - (int)(top >> 23); }
+// in [2^14, 2^15), below it from 2^-106 down) from the bits of that entry.
+__device__ __forceinline__ int query_shift(uint32_t top) { return min(141 - (int)(top >> 23), 120); }
+// What turns its products into log2 scores: above zero, so that a hidden score stays
+// minus infinity, and else as small as it is (small queries may meet large keys).
+// Scores over it are numbers for keys up to 2^102.
+__device__ __forceinline__ float score_factor(float scale_log2, int shift) {
+  return fmaxf(ldexpf(fabsf(scale_log2), -shift), 0x1p-149f);
+}
 
 // Four bytes of a mask row from key `key` on, none of them at `end` or past it
 // (zeros there); the row's address and the key may be odd.

@@ -842,3 +842,19 @@ def test_all_bits_of_the_products(gpu, kind, dim, lengths, new):
     cache.v_codes[::2, :, ::3] = 0
     _check_by_products(cache, batch, q, cache.attend(q, *batch.args))
     _check_by_products(cache, batch, q, cache.attend(q, *batch.args, scale=-0.3), scale=-0.3)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("size", [2.0**-90, 2.0**-96, 2.0**-110, 2.0**90])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_queries_of_any_size(gpu, kind, size, rows):
+    """Very small queries over large keys, and the other way round."""
+    cache = Int4KVCache(12, 1, 128, page_size=32)
+    _fill(cache, 3)
+    cache.k_scales.mul_(2.0**96 if size < 1 else 2.0**-90)
+    batch = Batch(cache, [310], [rows], seed=1)
+    q = _queries(rows, 8, 128, kind, 2, size=size)
+    got, lse = cache.attend(q, *batch.args, return_lse=True)
+    _check(cache, batch, q, got, lse)
+    got, lse = cache.attend(q, *batch.args, scale=0.0, return_lse=True)
+    _check(cache, batch, q, got, lse, scale=0.0)
