@@ -131,7 +131,8 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     const Kv4Batch b = check_batch(p, page_table, lengths, offsets, batch, max_pages, rows);
     const Kv4Type t = check_type(type);
     check_heads(p, b, heads);
-    if (!std::isfinite(scale)) throw InvalidArgument("scale must be finite");
+    const float scale_log2 = (float)(scale * kLog2e);
+    if (!std::isfinite(scale_log2)) throw InvalidArgument("scale must be finite in single precision");
     if (window < 0) throw InvalidArgument("window must not be negative");
     if (mask != nullptr && mask_width < 0) throw InvalidArgument("mask width must not be negative");
     if (rows == 0) return;
@@ -158,7 +159,7 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     a.heads = (int32_t)heads;
     a.causal = causal != 0;
     a.window = window == 0 || window > INT_MAX ? INT_MAX : (int32_t)window;
-    a.scale_log2 = (float)(scale * kLog2e);
+    a.scale_log2 = scale_log2;
     check_hip(launch_kv4_attend(p, b, a, t, workspace, cus, as_stream(stream)), "launch cache attention kernels");
   });
 }

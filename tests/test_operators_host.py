@@ -73,6 +73,14 @@ def test_key_positions_stay_within_32_bits():
             assert _status("msim_kv4_append_async", ctypes.addressof(pool), *args)[0] == status
 
 
+@pytest.mark.parametrize("scale,status", [(1e300, 1), (2.5e38, 1), (-1e39, 1), (float("inf"), 1), (2.3e38, 0), (0.0, 0)])
+def test_scales_that_single_precision_has_not(scale, status):
+    args = [None, None, None, 0, 0, 0, None, 0, 0, 4, 0, scale, 1, 0, None, 0, 0, None, 0, 0, None, None, 0, None]
+    pool = _pool()
+    got = _status("msim_kv4_attend_async", ctypes.addressof(pool), *args)
+    assert got[0] == status and (status == 0 or "scale" in got[1])
+
+
 def test_calls_of_no_rows_do_nothing():
     pool = _pool()
     assert _status("msim_kv4_append_async", ctypes.addressof(pool), None, None, None, 0, 0, 0, None, 0, 0, None, 0, 0, 0,
