@@ -476,7 +476,7 @@ int msim_linear4_layout_async(const uint8_t* codes, const uint16_t* scales, int6
                               uint8_t* out_codes, uint16_t* out_scales, void* stream);
 /* x [rows, k] (row stride in elements) times the matrix's rows, sums in single
  * precision, rounded once to `type` into out [rows, n].  bias f32 [n] or NULL.
- * Meant for few rows (it reads the matrix once per 32 of them); an infinity in x
+ * Meant for few rows (it reads the matrix once per 16 or 32 of them); an infinity in x
  * may come out as a NaN.  x and out must not overlap. */
 int msim_linear4_async(const uint8_t* codes, const uint16_t* scales, int64_t n, int64_t k, int64_t group,
                        const float* bias, const void* x, int64_t rows, int64_t x_row_stride, int type, void* out,

@@ -21,10 +21,10 @@
 // the others left its rounding in results that it has no part in.
 //
 // Bytes bound it: n k / 2 and the scales, for any number of rows that fits a
-// pass (32).  Waves of a workgroup take the 128-column tiles of the same rows of W
-// in turn and join in LDS in a fixed order.  One row by 4096 x 4096 takes 4.7 us
-// (4.4 in the kernel; the host side of a call is 4.2), 16 rows by
-// 28672 x 8192 in groups of 64 take 25.1 us, 5.0 TB/s.
+// pass (16; 32 in groups of 128 and 16 bits).  Waves of a workgroup take the 128-column tiles of the same rows of W
+// in turn and join in LDS in a fixed order.  One row by 4096 x 4096 takes 4.8 us (the
+// host side of a call is 4.2); 16 rows by 28672 x 8192 in groups of 64 take 30.2 us,
+// 4.2 TB/s, of which the decoding that does not hide costs two.
 #include "codes4.hpp"
 #include "linear4.hpp"
 
@@ -249,13 +249,12 @@ __global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) vo
 
   // The next tile of x is on its way during a tile's products, and the next tiles
   // of W too where the registers hold them.
-  constexpr bool kBoth = kRowTiles <= 4 && kGroups * kCols * kRowTiles <= 8 && (T != kKv4F32 || kCols == 1);
-  constexpr bool kRowsAhead = T != kKv4F32 || kCols == 1;
+  constexpr bool kBoth = kRowTiles <= 4 && kGroups * kCols * kRowTiles <= 8;
   v4u codes[kBoth ? 2 : 1][kRowTiles];
   uint32_t scales[kBoth ? 2 : 1][kRowTiles][kGroups * 2];
   XTile xs[2];
   if (wave < tiles_k) {
-    if constexpr (kRowsAhead) load_rows(wave, xs[0]);
+    load_rows(wave, xs[0]);
     load_w(wave, codes[0], scales[0]);
   }
   for (int k0 = wave; k0 < tiles_k; k0 += 2 * waves) {
@@ -264,8 +263,7 @@ __global__ __launch_bounds__(kWave* most_waves(T, kGroups, kCols, kRowTiles)) vo
       const int kt = k0 + d * waves;
       if (kt >= tiles_k) break;
       const bool more = kt + waves < tiles_k;
-      if constexpr (!kRowsAhead) load_rows(kt, xs[d]);
-      if (kRowsAhead && more) load_rows(kt + waves, xs[1 - d]);
+      if (more) load_rows(kt + waves, xs[1 - d]);
       if constexpr (kBoth) {
         if (more) load_w(kt + waves, codes[1 - d], scales[1 - d]);
         multiply(codes[d], scales[d], xs[d]);
@@ -316,8 +314,8 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
   const int64_t gx = ((w.n + 15) / 16 + kRowTiles - 1) / kRowTiles, gy = (rows + 16 * kCols - 1) / (16 * kCols);
   if (gy > 65535) return hipErrorInvalidValue;
   // Enough waves for the CUs' latency, within the tiles there are and the LDS
-  // that joins them (one row by 4096 x 4096 4.3 us, with four waves 5.6; by 28672 x
-  // 8192 22.3 and 29.2).
+  // that joins them (one row by 4096 x 4096 5.1 us, with four waves 5.8; by 28672 x
+  // 8192 27.8 and 32.2; three matrices in turn).
   const int tiles_k = (w.k + 127) / 128;
   int waves = 4;
   while (waves < most_waves(T, kGroups, kCols, kRowTiles) && waves * 2 <= tiles_k && gx * gy * waves < num_cus * 16)
@@ -330,8 +328,6 @@ hipError_t launch_shape(const Linear4Matrix& w, const void* x, int64_t rows, int
 
 // Row tiles that the registers hold without spilling.
 constexpr int most_row_tiles(Kv4Type type, int groups, int cols) {
-  if (type == kKv4F32 && cols > 1) return 1;
-  if (groups * cols >= 8) return 2;
   return groups * cols >= 4 || (type == kKv4F32 && groups > 1) ? 4 : 7;
 }
 
@@ -341,8 +337,8 @@ hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, i
   // Row tiles of a workgroup: the busiest CU has its workgroups' row tiles to do,
   // and with each workgroup the rows of x, whose loads (16 rows apart) cost as
   // much as two row tiles; one row costs half of one. At 4096 x 4096 one tile takes
-  // 4.3 us for a row and 6.8 for 16, as many as the registers hold 9.2 and 12.7; at
-  // 28672 x 8192 57 us against 25 for 16 rows.
+  // 5.1 us for a row and 7.0 for 16, as many as the registers hold (seven)
+  // 12.0 and 15.0; at 28672 x 8192 60 us against 31 for 16 rows.
   const int64_t tiles = (w.n + 15) / 16, columns = (rows + 16 * kCols - 1) / (16 * kCols);
   auto cost = [&](int row_tiles) -> int64_t {
     const int64_t groups = (tiles + row_tiles - 1) / row_tiles * columns;
@@ -367,10 +363,14 @@ hipError_t launch_columns(const Linear4Matrix& w, const void* x, int64_t rows, i
 template <Kv4Type T, int kGroups>
 hipError_t launch_group(const Linear4Matrix& w, const void* x, int64_t rows, int64_t x_row_stride, void* out,
                         int64_t out_row_stride, int num_cus, hipStream_t stream) {
-  // Two column tiles read a large matrix once (32 rows by 28672 x 8192 33 us against
-  // 45, by 4096 x 4096, which the caches hold, 10.4 against 8.6).
-  if (rows <= 16) return launch_columns<T, kGroups, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
-  return launch_columns<T, kGroups, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  // From 17 rows on, two column tiles read and decode W once for both, where the
+  // registers leave them as many row tiles: 16-bit x, groups of 128. 32 rows by 28672 x
+  // 8192 take 40 us against 54 with one, by 4096 x 4096, which one spreads over more
+  // CUs, 10.7 against 9.4. The others lose: by 28672 x 8192 in groups of 32 86 us with
+  // two and 76 with one, in single precision 220 to 238 and 97 to 143; groups of 64 tie.
+  if constexpr (kGroups == 1 && T != kKv4F32)
+    if (rows > 16) return launch_columns<T, kGroups, 2>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
+  return launch_columns<T, kGroups, 1>(w, x, rows, x_row_stride, out, out_row_stride, num_cus, stream);
 }
 
 template <Kv4Type T>

@@ -88,5 +88,5 @@ class Int4Linear:
         out_features] in x's dtype: sums in single precision, rounded once.
         ``out`` is contiguous and does not overlap x.
         Enqueued on the current stream; records no gradients.  Meant for few
-        rows: the matrix is read once per 32 of them."""
+        rows: the matrix is read once per 16 or 32 of them."""
         return self._calls.multiply(self._handle, x, out)
