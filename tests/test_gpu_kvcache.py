@@ -683,14 +683,14 @@ def test_refusals(gpu):
 
 # --------------------------------------------------- product by product
 #
-# 16-bit queries are taken whole, and a probability times its value scale in 16 bits.
+# Queries are taken whole, and a probability times its value scale in 16 bits or whole.
 
 
 def _check_by_products(cache, batch, q, got, got_lse=None, **kw):
-    """As _check, for 16-bit queries, by what the products themselves can lose: a score
-    is exact products added in single precision (a quarter of the dims, and four
-    roundings of factors), a probability times its scale keeps 2^-16.  Every result
-    is the rounding of one within that of the expected."""
+    """As _check, by what the products themselves can lose: a score is exact products
+    added in single precision (a quarter of the dims, and four roundings of factors), a
+    probability times its scale keeps 2^-16 in 16-bit calls.  Every result is the
+    rounding of one within that of the expected."""
     out, lse, mass, _ = _expected(cache, batch, q, **kw)
     share, dim = q.shape[1] // cache.kv_heads, cache.head_dim
     scale = abs(kw.get("scale") or dim**-0.5)
@@ -704,7 +704,7 @@ def _check_by_products(cache, batch, q, got, got_lse=None, **kw):
             sums = (q[rows, h].cpu().double().abs() @ k[:, h // share].t()).amax(-1) * scale
             delta[rows, h] = 2.0**-24 * (dim / 4 + 4) * sums + 2.0**-23
     sums = 2.0**-24 * (max(batch.host_lengths) / 8 + 16)
-    tol = (2.0**-16 + 2 * delta[..., None] + 2 * sums) * mass + 1e-30
+    tol = ((2.0**-21 if q.dtype == F32 else 2.0**-16) + 2 * delta[..., None] + 2 * sums) * mass + 1e-30
     got = got.cpu()
     off = ~(((out - tol).to(q.dtype) <= got) & (got <= (out + tol).to(q.dtype)))
     assert not bool(off.any()), (int(off.sum()), float(((got.double() - out).abs() / tol)[off].max()))
@@ -858,3 +858,19 @@ def test_queries_of_any_size(gpu, kind, size, rows):
     _check(cache, batch, q, got, lse)
     got, lse = cache.attend(q, *batch.args, scale=0.0, return_lse=True)
     _check(cache, batch, q, got, lse, scale=0.0)
+
+
+@pytest.mark.parametrize("dim,share,rows", [(64, 8, 1), (96, 2, 5), (128, 8, 1), (128, 8, 9), (192, 4, 2), (256, 8, 3),
+                                            (128, 8, 70)])
+def test_single_precision_queries_are_whole(gpu, dim, share, rows):
+    """All bits of a query count, beside a channel far larger than the others too."""
+    cache = Int4KVCache(12, 1, dim, page_size=32)
+    _fill(cache, 3)
+    cache.k_codes[..., 5] = 0  # channels 10 and 11
+    batch = Batch(cache, [310], [rows], seed=1)
+    q = _queries(rows, share, dim, F32, 2, size=4.0)
+    for size in (4.0, 3e7):
+        q[..., 10] = size
+        q[..., 11] = size / 7
+        got, lse = cache.attend(q, *batch.args, return_lse=True)
+        _check_by_products(cache, batch, q, got, lse)
