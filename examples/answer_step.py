@@ -3,7 +3,9 @@
 A MaxSim search finds passages for a batch of queries; one attention layer of a
 reader takes the passages' tokens into its key/value cache and decodes a few
 tokens over them: projections by ``Int4Linear``, keys and values into
-``Int4KVCache``, attention over it.  Synthetic corpus, random weights.
+``Int4KVCache``, attention over it.  Synthetic corpus, random weights; the passages'
+token embeddings stand for the hidden states that a reader's lower layers would make
+of their text.
 
     python examples/answer_step.py
 """

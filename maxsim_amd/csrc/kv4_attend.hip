@@ -16,14 +16,15 @@
 //     are merged by halves, so that the pairs a decoded register holds are two
 //     keys of one dim.
 // Keys' codes become f16 by one bitwise operation per pair (0x6400 | code ^ 8 is
-// 1032 + code, exactly) and one packed subtraction, values' codes bfloat16 by a
-// conversion each and a merge.  The key scale multiplies the score, the value scale
-// the probability; nothing else is dequantised.
+// 1032 + code) and one packed subtraction or multiply-add, exactly; values' codes
+// bfloat16 by a conversion each and a merge.  The key scale multiplies the score, the
+// value scale the probability; nothing else is dequantised.
 //
 // Queries are scaled to f16 by a power of two per row, largest entry in
 // [2^14, 2^15): bfloat16 entries keep all their bits down to 2^-28 of the
-// largest, f16 ones too.  Single precision queries are a sum of two f16 (22
-// bits).  A probability times its value scale is the sum of two bfloat16 (16 bits;
+// largest, f16 ones too.  Single precision queries are a sum of two f16: 22 bits of
+// entries down to 2^-16 of the largest, 2^-40 of the largest below, which the rounding of
+// a score's sum exceeds.  A probability times its value scale is the sum of two bfloat16 (16 bits;
 // single precision calls: of three, exactly), at any size that single precision
 // has: with one f16 outputs to which only small products contribute lost bits, as
 // happens in peaked rows, and f16 results had an error of 2.8e-4 of the norm in
@@ -35,8 +36,8 @@
 // row.  The keys of a sequence are split among workgroups when there are few
 // query rows; each leaves its unnormalised sum and a second launch joins them.
 // 32 heads of 128 on 8: three tokens behind 100,000 to 131,072 keys (f16) take
-// 86 us, 4.5 TB/s, of which the main launch has 81 and the join 5; 32 behind 100 to
-// 8,000 (bfloat16) 40 us, 3.8 TB/s (35 and 5).
+// 89 us, 4.3 TB/s, of which the main launch has 84 and the join 5; 32 behind 100 to
+// 8,000 (bfloat16) 43 to 44 us, 3.5 TB/s (38 and 5).
 #include "kv4_split.hpp"
 
 namespace msim {

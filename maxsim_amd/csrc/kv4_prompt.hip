@@ -29,7 +29,8 @@
 // beside the other's exponentials, which hides only a part: 32 MFMAs of 521 ns
 // beside 144 vector operations of 480 ns took 727.
 // 2 x 2048 tokens behind up to 15,000, 32 heads of 128 on 8, bfloat16: 0.83 TFLOP
-// (4 dim per row and key that it sees) in 1.22 ms, 0.68 PFLOP/s.
+// (4 dim per row and key that it sees) in 1.20 to 1.30 ms, by the card, 0.64 to 0.69
+// PFLOP/s.
 #include "kv4_split.hpp"
 
 namespace msim {

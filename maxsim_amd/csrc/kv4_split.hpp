@@ -31,10 +31,10 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // leaves a partial result, in its slot 1 if the item begins there, in slot 0 if
 // it came in from the worker before (it has at most one of each).
 //
-// Where no sequence can be longer than kShort keys a granule is kShort: no item
-// is split, and the call is one launch. Another 128 keys cost a workgroup about
-// 1 us, the second launch 4 (one token behind 120 keys 7.5 us against 12.2 split,
-// behind 391 10.3 against 12.2; 64 tokens behind 500 14.5 against 24.7).
+// Where the page table has no room for sequences longer than kShort keys a granule is
+// kShort: no item is split, and the call is one launch. Another 128 keys cost a workgroup
+// about 1 us, the second launch 3 to 4 (one token behind 120 keys 7.3 us against 9.8
+// split, behind 391 and 500 the same 10.4; 64 tokens behind 500 17.3 against 22.7).
 constexpr int kKeyAlign = 32;  // a tile's first key
 constexpr int kGranule = 128;
 constexpr int kShort = 4 * kGranule;

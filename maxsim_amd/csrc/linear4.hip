@@ -14,10 +14,10 @@
 //     per pair, 14 operations a word.
 //   f16 x: bits 3..6 of a half, under a constant exponent, make 136 + code; 136 is
 //     subtracted, 11 operations.
-//   f32 x: three bfloat16 parts that sum to x exactly; codes as 24 + code in
-//     bfloat16, 24 subtracted in single precision.
+//   f32 x: three bfloat16 parts that sum to x exactly; codes under a constant
+//     exponent as (24 + code) / 1024, 24 / 1024 subtracted in single precision.
 // So every product is exact, and a column whose code is zero adds nothing: with the
-// 24 left in the codes and taken off the sum (7 operations) a column of x 1e6 times
+// 24 left in the codes and taken off the sum (7 operations) a column of x 1e7 times
 // the others left its rounding in results that it has no part in.
 //
 // Bytes bound it: n k / 2 and the scales, for any number of rows that fits a
