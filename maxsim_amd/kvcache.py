@@ -147,7 +147,8 @@ class Int4KVCache:
         once from single precision sums, and with ``return_lse`` the logarithm
         of each softmax's sum, float32 [rows, heads].  A row that sees nothing
         is zeros, with minus infinity.  ``out`` may be q itself, and must not
-        overlap it otherwise.
+        overlap it otherwise.  Queries and values may have any size, keys up to
+        2^102.
         """
         if window is not None and window < 1:
             raise ValueError("window must be positive")
