@@ -462,6 +462,69 @@ int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* page_table, 
                           int64_t out_head_stride, float* lse, void* workspace, uint64_t workspace_bytes,
                           void* stream);
 
+/* The same, and:
+ * sinks: under a window, keys j < sinks stay visible.
+ * parents i32 [rows] (NULL: none; with causal only): the rows of a sequence are a tree.
+ * parents[row] is the number, among the sequence's rows, of an earlier one that the row
+ * comes after; any other number: the last token before them.  A row sees the tokens
+ * before the sequence's rows, the rows that it comes after, and itself; its position p
+ * is length - rows + the number of rows that it comes after, and a window counts those
+ * positions.  A sequence may have 1,024 rows; rows of a longer one see nothing. */
+int msim_kv4_attend_ex_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                             const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                             const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads, int type,
+                             double scale, int causal, int64_t window, const uint8_t* mask,
+                             int64_t mask_row_stride, int64_t mask_width, int64_t sinks, const int32_t* parents,
+                             void* out, int64_t out_row_stride, int64_t out_head_stride, float* lse,
+                             void* workspace, uint64_t workspace_bytes, void* stream);
+/* Of the rows of a call those that stay move up to the end of what their sequence held
+ * before: kept i32 [batch, width], row b the numbers, ascending, of sequence b's rows
+ * that stay; the list ends at the first entry that is no such number (-1).  new_lengths
+ * i32 [batch]: length - rows + their count, 0 at least; it must not overlap the other
+ * arrays.  The slots behind keep what they held.  A row that comes from a hole is zeros.  At most 2^20
+ * sequences. */
+int msim_kv4_keep_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                        const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                        const int32_t* kept, int64_t width, int32_t* new_lengths, void* stream);
+
+/* Which pages of a pool the sequences of a batch hold, and where their rows go.  All in
+ * device memory: page_table i32 [batch, max_pages] (sequence b holds its first
+ * ceil(lengths[b] / page_size) entries; -1 behind them), lengths i32 [batch],
+ * free_pages i32 [num_pages] of which the first *free_count are a stack of the pages that no
+ * sequence holds (-1 behind them).  An update
+ *   cuts sequence b to cut[b] tokens (NULL: none; larger or equal numbers cut nothing) and
+ *     puts its pages past those on the stack, all sequences' in reverse order;
+ *   gives it new_tokens[b] more (NULL, or negative: none) and pages from the stack, in the
+ *     order of the sequences.
+ * A sequence gets none of its tokens where they do not fit its row of the table, or where
+ * the tokens asked for by it and those before it are more than `rows`, or where it needs
+ * pages and those asked for by it and those before it are more than the stack holds.
+ * offsets i32 [batch + 1], positions i32 [rows] and slots i64 [rows] describe the tokens
+ * given: their rows packed by sequence, their positions, page * page_size + place in the
+ * page; -1 behind the last.  page_size is a power of two from 16 to 65536. */
+int msim_pages_update_async(int32_t* page_table, int32_t* lengths, int32_t* free_pages, int32_t* free_count,
+                            int64_t batch, int64_t max_pages, int64_t num_pages, int64_t page_size,
+                            const int32_t* new_tokens, const int32_t* cut, int64_t rows, int32_t* offsets,
+                            int32_t* positions, int64_t* slots, void* stream);
+
+/* ===================================================================== */
+/* Rotary positions (no counterpart in the reference).                    */
+/* ===================================================================== */
+/* Pairs of dims of queries and keys [rows, heads, dim] turned by their positions: pair i
+ * < pairs is (i, i + pairs), or (2 i, 2 i + 1) if adjacent; its angle is positions[axes[i],
+ * row] * turns[i] / 2^64 turns (turns u64 [pairs], axes i32 [pairs] from 0 to num_axes - 1,
+ * positions i32 [num_axes, rows] with axis_stride elements from axis to axis: device
+ * memory).  (x, y) becomes (x cos - y sin, x sin + y cos), in single precision, rounded once;
+ * dims from 2 pairs on are copied.  2 pairs <= dim <= 256.  Strides in elements, dims dense.
+ * heads or kv_heads may be 0.  An output may be its input (same pointer and strides), and
+ * must not overlap an input or the other output otherwise.  At most 2^25 rows. */
+int msim_rotary_async(const uint64_t* turns, const int32_t* axes, int64_t pairs, int64_t dim, int64_t num_axes,
+                      int adjacent, const int32_t* positions, int64_t axis_stride, int64_t rows, int type,
+                      const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads, void* q_out,
+                      int64_t q_out_row_stride, int64_t q_out_head_stride, const void* k, int64_t k_row_stride,
+                      int64_t k_head_stride, int64_t kv_heads, void* k_out, int64_t k_out_row_stride,
+                      int64_t k_out_head_stride, void* stream);
+
 /* ===================================================================== */
 /* Products with a matrix in 4 bits and group scales (no counterpart in   */
 /* the reference): y = x W^T (+ bias), w[n, k] = code[n, k] * scale[n,    */

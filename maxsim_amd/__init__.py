@@ -33,16 +33,20 @@ from maxsim_amd.experimental import (
 )
 from maxsim_amd.kvcache import Int4KVCache
 from maxsim_amd.linear4 import Int4Linear, pack_int4_groups
+from maxsim_amd.pages import CachePages
+from maxsim_amd.rotary import Rotary
 from maxsim_amd.sdk import MODE_PRESETS, Corpus, CorpusMemoryReport, Index, Reranker, SearchResult
 
 __all__ = [
     "BinaryResidualPackedDocs",
+    "CachePages",
     "Corpus",
     "CorpusMemoryReport",
     "Index",
     "MODE_PRESETS",
     "Reranker",
     "ResidualInt4PackedDocs",
+    "Rotary",
     "SearchResult",
     "binres_cascade_topk",
     "binres_score",

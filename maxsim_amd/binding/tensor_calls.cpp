@@ -7,7 +7,7 @@
 // the C ABI (include/maxsim_hip.h) on the current stream.  It knows no kernels:
 // the library's entry points are handed over when it is set up.
 //
-// Functions take a handle (a capsule) made by `cache` or `linear`, and return
+// Functions take a handle (a capsule) made by `cache`, `linear`, `pages` or `rotary`, and return
 // tensors.  ValueError, NotImplementedError and RuntimeError as elsewhere in the
 // package.
 #define PY_SSIZE_T_CLEAN
@@ -31,8 +31,11 @@ struct {
   decltype(&msim_kv4_append_async) append = nullptr;
   decltype(&msim_kv4_read_async) read = nullptr;
   decltype(&msim_kv4_attend_workspace) attend_workspace = nullptr;
-  decltype(&msim_kv4_attend_async) attend = nullptr;
+  decltype(&msim_kv4_attend_ex_async) attend = nullptr;
   decltype(&msim_linear4_async) linear = nullptr;
+  decltype(&msim_kv4_keep_async) keep = nullptr;
+  decltype(&msim_pages_update_async) pages = nullptr;
+  decltype(&msim_rotary_async) rotary = nullptr;
 } abi;
 
 struct Cache {
@@ -46,12 +49,27 @@ struct Linear {
   int64_t n, k, group;
 };
 
+struct Pages {
+  at::Tensor table, lengths, free_pages, free_count;
+  int64_t page_size;
+};
+
+struct Rotary {
+  at::Tensor turns, axes;
+  int64_t pairs, dim, num_axes;
+  bool adjacent;
+};
+
 template <typename T>
 const char* handle_name();
 template <>
 const char* handle_name<Cache>() { return "maxsim_amd.cache"; }
 template <>
 const char* handle_name<Linear>() { return "maxsim_amd.linear"; }
+template <>
+const char* handle_name<Pages>() { return "maxsim_amd.pages"; }
+template <>
+const char* handle_name<Rotary>() { return "maxsim_amd.rotary"; }
 
 template <typename T>
 T* handle(PyObject* o) {
@@ -119,6 +137,8 @@ struct Batch {
   int64_t batch, max_pages, rows;
 };
 
+constexpr int64_t kMostRows = int64_t{1} << 26;  // of a call
+
 const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 
 Batch read_batch(const Cache& c, PyObject* table, PyObject* lengths, PyObject* offsets, int64_t rows) {
@@ -136,17 +156,19 @@ Batch read_batch(const Cache& c, PyObject* table, PyObject* lengths, PyObject* o
   return b;
 }
 
-// Rows [rows, heads, head_dim] with any strides, dense in the last dimension;
-// heads 0: any.
-const at::Tensor& row_tensor(const Cache& c, PyObject* o, const char* name, int64_t heads) {
+// Rows [rows, heads, dim] with any strides, dense in the last dimension; heads -1: any.
+const at::Tensor& row_tensor(const at::Device& device, int64_t dim, PyObject* o, const char* name, int64_t heads) {
   const at::Tensor& t = tensor(o, name);
-  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(2) == c.pool.dim && (heads == 0 || t.size(1) == heads), name,
-                    " must be a tensor of shape [rows, ", heads == 0 ? std::string("heads") : std::to_string(heads), ", ",
-                    c.pool.dim, "]");
-  TORCH_CHECK_VALUE(t.device() == c.device, name, " must be on ", c.device);
+  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(2) == dim && (heads < 0 || t.size(1) == heads), name,
+                    " must be a tensor of shape [rows, ", heads < 0 ? std::string("heads") : std::to_string(heads), ", ",
+                    dim, "]");
+  TORCH_CHECK_VALUE(t.device() == device, name, " must be on ", device);
   TORCH_CHECK_VALUE(t.stride(2) == 1 || t.numel() == 0, name, " must be dense in its last dimension");
   type_of(t.scalar_type());
   return t;
+}
+const at::Tensor& row_tensor(const Cache& c, PyObject* o, const char* name, int64_t heads) {
+  return row_tensor(c.device, c.pool.dim, o, name, heads == 0 ? -1 : heads);
 }
 
 // First byte of a tensor's elements and the one behind its last (strides are not negative).
@@ -214,10 +236,11 @@ PyObject* pair(const at::Tensor& a, const at::Tensor& b) {
   return both;
 }
 
-// setup(last_error, append, read, attend_workspace, attend, linear): addresses.
+// setup(last_error, append, read, attend_workspace, attend, linear, keep, pages, rotary):
+// addresses.
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 6);
+  arguments(n, 9);
   auto address = [&](int i) { return reinterpret_cast<void*>(integer(a[i])); };
   abi.last_error = reinterpret_cast<decltype(abi.last_error)>(address(0));
   abi.append = reinterpret_cast<decltype(abi.append)>(address(1));
@@ -225,6 +248,9 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   abi.attend_workspace = reinterpret_cast<decltype(abi.attend_workspace)>(address(3));
   abi.attend = reinterpret_cast<decltype(abi.attend)>(address(4));
   abi.linear = reinterpret_cast<decltype(abi.linear)>(address(5));
+  abi.keep = reinterpret_cast<decltype(abi.keep)>(address(6));
+  abi.pages = reinterpret_cast<decltype(abi.pages)>(address(7));
+  abi.rotary = reinterpret_cast<decltype(abi.rotary)>(address(8));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -295,10 +321,11 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// attend(cache, q, page_table, lengths, offsets, scale, causal, window, mask, out, return_lse)
+// attend(cache, q, page_table, lengths, offsets, scale, causal, window, mask, out, return_lse,
+// sinks, parents)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 11);
+  arguments(n, 13);
   const Cache& c = *handle<Cache>(a[0]);
   const at::Tensor& q = row_tensor(c, a[1], "q", 0);
   const int64_t rows = q.size(0), heads = q.size(1);
@@ -320,6 +347,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // An empty mask has no memory: it hides every key all the same.
     mask = mask_width > 0 ? static_cast<const uint8_t*>(m.const_data_ptr()) : c.pool.k_codes;
   }
+  const int32_t* parents = nullptr;
+  if (a[12] != Py_None) {
+    const at::Tensor& p = index_tensor(a[12], "parents", 1, c.device);
+    TORCH_CHECK_VALUE(p.size(0) == rows, "parents must have shape [rows]");
+    static const int32_t none = -1;  // a call of no rows has no parents to read
+    parents = rows > 0 ? ints(p) : &none;
+  }
   at::Tensor out, lse, work;
   if (a[9] == Py_None) {
     out = at::empty({rows, heads, c.pool.dim}, q.options().requires_grad(false));
@@ -338,10 +372,138 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (need > 0) work = at::empty({(int64_t)need}, at::TensorOptions().device(c.device).dtype(at::kByte));
   check(abi.attend(&c.pool, b.table, b.lengths, b.offsets, b.batch, b.max_pages, rows, q.const_data_ptr(), q.stride(0),
                    q.stride(1), heads, type_of(q.scalar_type()), scale, causal, integer(a[7]), mask, mask_stride,
-                   mask_width, out.data_ptr(), out.stride(0), out.stride(1),
+                   mask_width, integer(a[11]), parents, out.data_ptr(), out.stride(0), out.stride(1),
                    want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, need > 0 ? work.data_ptr() : nullptr, need,
                    launch.stream));
   return want_lse ? pair(out, lse) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// keep(cache, page_table, lengths, offsets, kept): the new lengths.
+PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 5);
+  const Cache& c = *handle<Cache>(a[0]);
+  // The rows are not given here: as many as the offsets say, or one per sequence.
+  const int64_t batch = index_tensor(a[2], "lengths", 1, c.device).size(0);
+  const Batch b = read_batch(c, a[1], a[2], a[3], a[3] == Py_None ? batch : kMostRows);
+  const at::Tensor& kept = index_tensor(a[4], "kept", 2, c.device);
+  TORCH_CHECK_VALUE(kept.size(0) == b.batch, "kept must have shape [batch, width]");
+  const at::Tensor out = at::empty({b.batch}, kept.options());
+  const Launch launch(c.device);
+  check(abi.keep(&c.pool, b.table, b.lengths, b.offsets, b.batch, b.max_pages, b.rows, ints(kept), kept.size(1),
+                 static_cast<int32_t*>(out.data_ptr()), launch.stream));
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// pages(table, lengths, free_pages, free_count, page_size): a handle on their state.
+PyObject* make_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 5);
+  const at::Device device = tensor(a[0], "table").device();
+  return make_handle(new Pages{index_tensor(a[0], "table", 2, device), index_tensor(a[1], "lengths", 1, device),
+                               index_tensor(a[2], "free", 1, device), index_tensor(a[3], "free_count", 1, device),
+                               integer(a[4])});
+  END_HANDLE_TH_ERRORS
+}
+
+// update(pages, new, lengths, rows): offsets, positions and slots of the new rows.
+PyObject* update(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 4);
+  const Pages& p = *handle<Pages>(a[0]);
+  const int64_t batch = p.table.size(0);
+  auto counts = [&](PyObject* o, const char* name) -> const int32_t* {
+    if (o == Py_None) return nullptr;
+    const at::Tensor& t = index_tensor(o, name, 1, p.table.device());
+    TORCH_CHECK_VALUE(t.size(0) == batch, name, " must have shape [batch]");
+    return ints(t);
+  };
+  const int32_t *fresh = counts(a[1], "new"), *cut = counts(a[2], "lengths");
+  const int64_t rows = integer(a[3]);
+  TORCH_CHECK_VALUE(rows >= 0, "rows must not be negative");
+  TORCH_CHECK_NOT_IMPLEMENTED(rows <= kMostRows, "a call takes at most 2^26 rows");
+  const at::Tensor offsets = at::empty({batch + 1}, p.table.options()), positions = at::empty({rows}, p.table.options());
+  const at::Tensor slots = at::empty({rows}, p.table.options().dtype(at::kLong));
+  const Launch launch(p.table.device());
+  auto address = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  check(abi.pages(address(p.table), address(p.lengths), address(p.free_pages), address(p.free_count), batch,
+                  p.table.size(1), p.free_pages.size(0), p.page_size, fresh, cut, rows, address(offsets),
+                  address(positions), static_cast<int64_t*>(slots.data_ptr()), launch.stream));
+  PyObject* both = pair(offsets, positions);
+  PyObject* last = THPVariable_Wrap(slots);
+  PyObject* all = last ? PyTuple_Pack(3, PyTuple_GET_ITEM(both, 0), PyTuple_GET_ITEM(both, 1), last) : nullptr;
+  Py_XDECREF(both);
+  Py_XDECREF(last);
+  if (all == nullptr) throw python_error();
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary(turns, axes, dim, num_axes, adjacent): a handle on the frequencies.
+PyObject* make_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 5);
+  const at::Tensor &turns = tensor(a[0], "turns"), &axes = tensor(a[1], "axes");
+  TORCH_CHECK_VALUE(turns.scalar_type() == at::kLong && axes.scalar_type() == at::kInt && turns.is_contiguous() &&
+                        axes.is_contiguous() && turns.dim() == 1 && turns.sizes() == axes.sizes() &&
+                        turns.device() == axes.device(),
+                    "turns and axes must be dense and of one shape");
+  return make_handle(new Rotary{turns, axes, turns.size(0), integer(a[2]), integer(a[3]), a[4] == Py_True});
+  END_HANDLE_TH_ERRORS
+}
+
+// rotate(rotary, q, k, positions, q_out, k_out): k and k_out may be None, and both outputs.
+PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 6);
+  const Rotary& r = *handle<Rotary>(a[0]);
+  const at::Device device = r.turns.device();
+  const at::Tensor& q = row_tensor(device, r.dim, a[1], "q", -1);
+  const bool two = a[2] != Py_None;
+  const at::Tensor& k = two ? row_tensor(device, r.dim, a[2], "k", -1) : q;
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.size(0) == q.size(0),
+                    "q and k must have the same rows and dtype");
+  const at::Tensor& p = tensor(a[3], "positions");
+  const int64_t rows = q.size(0);
+  TORCH_CHECK_VALUE(p.scalar_type() == at::kInt && p.device() == device &&
+                        (p.dim() == 2 ? p.size(0) == r.num_axes : p.dim() == 1 && r.num_axes == 1) && p.size(-1) == rows,
+                    "positions must be an int32 tensor of shape ", r.num_axes == 1 ? "[rows] or " : "", "[", r.num_axes,
+                    ", rows] on ", device);
+  TORCH_CHECK_VALUE(rows <= 1 || p.stride(-1) == 1, "positions must be dense in their last dimension");
+  at::Tensor out[2];
+  if (a[4] == Py_None) {
+    TORCH_CHECK_VALUE(a[5] == Py_None, "out must hold a tensor for q");
+    out[0] = at::empty(q.sizes(), q.options().requires_grad(false));
+    if (two) out[1] = at::empty(k.sizes(), k.options().requires_grad(false));
+  } else {
+    TORCH_CHECK_VALUE((a[5] != Py_None) == two, "out must hold a tensor for each of q and k");
+    for (int i = 0; i < 1 + two; ++i) {
+      const at::Tensor& from = i ? k : q;
+      out[i] = row_tensor(device, r.dim, a[4 + i], i ? "out[1]" : "out[0]", from.size(1));
+      TORCH_CHECK_VALUE(out[i].scalar_type() == from.scalar_type() && out[i].size(0) == rows,
+                        "outputs must have the shape and dtype of q and k");
+      check_output(out[i], i ? "out[1]" : "out[0]");
+      TORCH_CHECK_VALUE(!share_memory(out[i], from, true) && (!two || !share_memory(out[i], i ? q : k, false)),
+                        "an output must not overlap q or k, unless it is its own input");
+    }
+    TORCH_CHECK_VALUE(!two || !share_memory(out[0], out[1], false), "out[0] and out[1] must not overlap");
+  }
+  const Launch launch(device);
+  const int64_t none = 0;
+  check(abi.rotary(static_cast<const uint64_t*>(r.turns.const_data_ptr()), ints(r.axes), r.pairs, r.dim, r.num_axes,
+                   r.adjacent, ints(p), p.dim() == 2 ? p.stride(0) : none, rows, type_of(q.scalar_type()),
+                   q.const_data_ptr(), q.stride(0), q.stride(1), q.size(1), out[0].data_ptr(), out[0].stride(0),
+                   out[0].stride(1), two ? k.const_data_ptr() : nullptr, two ? k.stride(0) : none,
+                   two ? k.stride(1) : none, two ? k.size(1) : none, two ? out[1].data_ptr() : nullptr,
+                   two ? out[1].stride(0) : none, two ? out[1].stride(1) : none, launch.stream));
+  if (two) return pair(out[0], out[1]);
+  PyObject* first = THPVariable_Wrap(out[0]);
+  PyObject* both = first ? PyTuple_Pack(2, first, Py_None) : nullptr;
+  Py_XDECREF(first);
+  if (both == nullptr) throw python_error();
+  return both;
   END_HANDLE_TH_ERRORS
 }
 
@@ -410,7 +572,9 @@ PyObject* multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define CALL(name, function) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(function)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     CALL("setup", setup),   CALL("cache", make_cache),   CALL("append", append),     CALL("read", read),
-    CALL("attend", attend), CALL("linear", make_linear), CALL("multiply", multiply), {nullptr, nullptr, 0, nullptr}};
+    CALL("attend", attend), CALL("linear", make_linear), CALL("multiply", multiply),
+    CALL("keep", keep),     CALL("pages", make_pages),   CALL("update", update),     CALL("rotary", make_rotary),
+    CALL("rotate", rotate), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

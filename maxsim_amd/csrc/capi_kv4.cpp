@@ -1,5 +1,5 @@
 // capi_kv4.cpp -- C ABI of the 4-bit key/value cache (kv4_rows.hip,
-// kv4_attend.hip): argument checks and launches.  The pool, the batch and the
+// kv4_attend.hip, kv4_keep.hip): argument checks and launches.  The pool, the batch and the
 // workspace are the caller's device memory.
 #include <climits>
 #include <cmath>
@@ -126,6 +126,20 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
                                      int64_t mask_row_stride, int64_t mask_width, void* out, int64_t out_row_stride,
                                      int64_t out_head_stride, float* lse, void* workspace, uint64_t workspace_bytes,
                                      void* stream) {
+  return msim_kv4_attend_ex_async(pool, page_table, lengths, offsets, batch, max_pages, rows, q, q_row_stride,
+                                  q_head_stride, heads, type, scale, causal, window, mask, mask_row_stride, mask_width,
+                                  0, nullptr, out, out_row_stride, out_head_stride, lse, workspace, workspace_bytes,
+                                  stream);
+}
+
+extern "C" int msim_kv4_attend_ex_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                                        const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                                        const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t heads,
+                                        int type, double scale, int causal, int64_t window, const uint8_t* mask,
+                                        int64_t mask_row_stride, int64_t mask_width, int64_t sinks,
+                                        const int32_t* parents, void* out, int64_t out_row_stride,
+                                        int64_t out_head_stride, float* lse, void* workspace, uint64_t workspace_bytes,
+                                        void* stream) {
   return guarded([&] {
     const Kv4Pool p = check_pool(pool);
     const Kv4Batch b = check_batch(p, page_table, lengths, offsets, batch, max_pages, rows);
@@ -135,6 +149,8 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     if (!std::isfinite(scale_log2)) throw InvalidArgument("scale must be finite in single precision");
     if (window < 0) throw InvalidArgument("window must not be negative");
     if (mask != nullptr && mask_width < 0) throw InvalidArgument("mask width must not be negative");
+    if (sinks < 0) throw InvalidArgument("sinks must not be negative");
+    if (parents != nullptr && causal == 0) throw InvalidArgument("parents need a causal call");
     if (rows == 0) return;
     check_rows(q, t, "q");
     check_rows(out, t, "out");
@@ -159,7 +175,24 @@ extern "C" int msim_kv4_attend_async(const msim_kv4_pool* pool, const int32_t* p
     a.heads = (int32_t)heads;
     a.causal = causal != 0;
     a.window = window == 0 || window > INT_MAX ? INT_MAX : (int32_t)window;
+    a.sinks = a.window == INT_MAX ? 0 : (int32_t)std::min<int64_t>(sinks, INT_MAX);
+    a.parents = parents;
     a.scale_log2 = scale_log2;
     check_hip(launch_kv4_attend(p, b, a, t, workspace, cus, as_stream(stream)), "launch cache attention kernels");
+  });
+}
+
+extern "C" int msim_kv4_keep_async(const msim_kv4_pool* pool, const int32_t* page_table, const int32_t* lengths,
+                                   const int32_t* offsets, int64_t batch, int64_t max_pages, int64_t rows,
+                                   const int32_t* kept, int64_t width, int32_t* new_lengths, void* stream) {
+  return guarded([&] {
+    const Kv4Pool p = check_pool(pool);
+    const Kv4Batch b = check_batch(p, page_table, lengths, offsets, batch, max_pages, rows);
+    if (width < 0) throw InvalidArgument("width must not be negative");
+    if (width > kMaxRows || batch > int64_t{1} << 20) throw NotSupported("a call keeps rows of at most 2^20 sequences");
+    if (batch == 0) return;
+    if (new_lengths == nullptr || (kept == nullptr && width > 0))
+      throw InvalidArgument("kept and new_lengths must not be NULL");
+    check_hip(launch_kv4_keep(p, b, kept, (int)width, new_lengths, as_stream(stream)), "launch cache keep kernel");
   });
 }

@@ -205,6 +205,26 @@ __device__ __forceinline__ T wave_reduce(T v, Op op) {
   return op(op(r0, r1), op(r2, r3));
 }
 
+// Inclusive scan over the lanes of an operation whose neutral element is 0 (DPP row
+// shifts, then the rows' last lanes).
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, Op op) {
+  auto step = [&](auto ctrl, auto rows) {
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+  };
+  typedef std::integral_constant<int, 0xF> All;
+  step(std::integral_constant<int, 0x111>{}, All{});
+  step(std::integral_constant<int, 0x112>{}, All{});
+  step(std::integral_constant<int, 0x114>{}, All{});
+  step(std::integral_constant<int, 0x118>{}, All{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  return wave_scan(v, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
 __device__ __forceinline__ float fmax3(float a, float b, float c) { return fmaxf(a, fmaxf(b, c)); }
 // One v_max3_f32 (the compiler splits fmax chains into two-operand maxima to
 // shorten dependencies; where issue slots are the limit, one instruction per

@@ -109,6 +109,11 @@ hipError_t launch_kv4_append(const Kv4Pool& pool, const Kv4Batch& batch, const K
 hipError_t launch_kv4_read(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Rows rows[2], Kv4Type type,
                            hipStream_t stream);
 
+// Of each sequence's rows those of the list kept [batch, width] stay, in its order; lengths
+// [batch] are written.
+hipError_t launch_kv4_keep(const Kv4Pool& pool, const Kv4Batch& batch, const int32_t* kept, int width, int32_t* lengths,
+                           hipStream_t stream);
+
 // ---------------------------------------------------------------- attention
 
 struct Kv4AttendArgs {
@@ -124,8 +129,16 @@ struct Kv4AttendArgs {
   int32_t heads;
   int32_t causal;
   int32_t window;  // keys at p - window + 1 .. p; INT32_MAX: all
+  int32_t sinks;   // and those below, whatever the window
+  // [rows] or nullptr: the row of its sequence's that a row comes after (an earlier one;
+  // any other number: the last token before them). It sees the tokens before the
+  // sequence's rows, the rows that it comes after, and itself, and its position counts those.
+  const int32_t* parents;
   float scale_log2;  // softmax scale * log2(e)
 };
+
+// Rows of a sequence in a call with parents, at most: rows of a longer one see nothing.
+constexpr int kMostDrafts = 1024;
 
 size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus);
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,

@@ -138,9 +138,12 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 
 // Granules from .. upto of an item.  kCols 16-row column tiles of queries per
 // workgroup; its waves take the key tiles in turn.
-template <Kv4Type T, int kDim, int kCols>
+//
+// kMore: calls with sinks or parents. Keys are numbered as TileRange says then, else by
+// themselves.
+template <Kv4Type T, int kDim, int kCols, bool kMore>
 __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                            const Split& split, float* __restrict__ partial, const Cursor& at,
+                                            const Split& split, float* __restrict__ partial, const Cursor<kMore>& at,
                                             uint32_t from, uint32_t upto) {
   typedef Shape<kDim> S;
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
@@ -151,6 +154,37 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   const SeqWork& u = at.work;
   const uint32_t tile = at.tile;
   const int seq = at.seq, head = at.head;
+
+  // With parents: of each row of the tile the rows that it comes after and itself, a bit
+  // each (a word more is read than has any), and how many they are.
+  constexpr int kLineWords = kMostDrafts / 32, kLinePitch = kLineWords + 3;  // odd: rows spread over the banks
+  __shared__ uint32_t s_line[kMore ? kRows * kLinePitch : 1];
+  __shared__ int s_parent[kMore ? kMostDrafts : 1], s_depth[kMore ? kRows : 1];
+  const bool tree = kMore && args.parents != nullptr;
+  const int start = u.length - u.rows;  // the first row's position
+  if (tree) {
+    const int drafts = min(u.rows, kMostDrafts);
+    for (int i = threadIdx.x; i < drafts; i += kWaves * kWave) s_parent[i] = args.parents[u.first + i];
+    for (int i = threadIdx.x; i < kRows * kLinePitch; i += kWaves * kWave) s_line[i] = 0;
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+      const int token = (int)((tile * kRows + threadIdx.x) / split.share);
+      auto up = [&](int row) -> int {  // -1 past the first
+        const int parent = s_parent[row];
+        return (uint32_t)parent < (uint32_t)row ? parent : -1;
+      };
+      int depth = 0;
+      if (token < drafts) {
+        for (int row = up(token); row >= 0; row = up(row)) ++depth;
+        int back = 0;
+        for (int row = token; row >= 0; row = up(row), ++back)
+          if (back < args.window || start + depth - back < args.sinks)
+            s_line[threadIdx.x * kLinePitch + row / 32] |= 1u << (row % 32);
+      }
+      s_depth[threadIdx.x] = depth;
+    }
+    __syncthreads();
+  }
 
   // Query rows of this tile: row r is new token r / share, head r % share.
   v8h q[kCols][kParts][S::kKeyWords];
@@ -167,9 +201,10 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     query[c] = have ? (int64_t)(u.first + token) * args.q_row_stride +
                           (int64_t)(head * split.share + sub) * args.q_head_stride
                     : -1;
-    const int pos = u.length - u.rows + token;
+    const int own = start + token, pos = tree ? start + s_depth[16 * c + col] : own;
     see_low[c] = pos >= args.window ? pos - args.window + 1 : 0;
-    see_high[c] = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
+    see_high[c] = args.causal ? max(0, min(u.length, own + 1)) : u.length;
+    if (tree && u.rows > kMostDrafts) see_high[c] = 0;
     mask[c] = nullptr;
     if (args.mask != nullptr) {
       see_high[c] = (int)min((int64_t)see_high[c], args.mask_width);
@@ -178,7 +213,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     if (!have) {  // nothing depends on what it sees
       see_low[c] = 0;
       see_high[c] = args.mask != nullptr ? 0 : INT_MAX;
-    } else if (see_high[c] > see_low[c]) {
+    } else if (kMore ? see_high[c] > 0 : see_high[c] > see_low[c]) {
       any_low = min(any_low, see_low[c]);
       any_high = max(any_high, see_high[c]);
     }
@@ -189,9 +224,14 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   all_high = wave_reduce(all_high, [](int a, int b) { return min(a, b); });
   any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
   any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
+  if (tree) all_high = min(all_high, max(0, start));
   // This worker's keys of the item, cut to what some row sees.
-  const int begin = max(at.range.low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
-  const int end = (int)min((int64_t)at.range.low + ((int64_t)upto << split.granule_shift), (int64_t)any_high);
+  const int low = kMore ? 0 : at.range.low;
+  auto key_of = [&](int number) -> int { return kMore ? at.range.key_of(number) : number; };
+  const int begin = kMore ? (int)(from << split.granule_shift)
+                          : max(low + (int)(from << split.granule_shift), min(any_low, u.length) / kTileKeys * kTileKeys);
+  const int end = (int)min((int64_t)low + ((int64_t)upto << split.granule_shift),
+                           (int64_t)(kMore ? at.range.number_of(any_high) : any_high));
 
   // A ring of tiles per wave: kStages - 1 of them on their way while one is
   // worked on.
@@ -204,8 +244,9 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   bool hole[kStages][2];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + i * kStep);
-    if (i < tiles) load_tile<kDim>(pool, pages, head, key_first + i * kStep, ring_lds + i * L::kBytes);
+    const int key = key_of(key_first + i * kStep);
+    const TilePages pages = tile_pages(pool, batch, seq, u.length, key);
+    if (i < tiles) load_tile<kDim>(pool, pages, head, key, ring_lds + i * L::kBytes);
     hole[i][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
     hole[i][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
   }
@@ -251,7 +292,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     for (int t = 0; t < S::kTiles; ++t) o[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  TilePages pages = tile_pages(pool, batch, seq, u.length, key_first + kAhead * kStep);
+  TilePages pages = tile_pages(pool, batch, seq, u.length, key_of(key_first + kAhead * kStep));
   uint32_t seen[kCols][2];  // mask bytes of the tile's keys of this lane
   auto load_mask = [&](int key0) {
 #pragma unroll
@@ -260,20 +301,20 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       for (int h = 0; h < 2; ++h)
         seen[c][h] = mask_bytes(mask[c], key0 + 16 * h + 4 * g, see_high[c]);
   };
-  if (args.mask != nullptr) load_mask(key_first);
+  if (args.mask != nullptr) load_mask(key_of(key_first));
   int slot = 0, fill = kAhead * L::kBytes;  // offsets in the ring
   for (int n = 0; n < tiles; ++n) {
-    const int key0 = key_first + n * kStep;
+    const int number = key_first + n * kStep, key0 = key_of(number);
     hole[kAhead][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
     hole[kAhead][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
     if (n + kAhead < tiles) {
-      load_tile<kDim>(pool, pages, head, key0 + kAhead * kStep, ring_lds + fill);
+      load_tile<kDim>(pool, pages, head, key_of(number + kAhead * kStep), ring_lds + fill);
       vm_wait_lds<kAhead * L::kLoads>();
     } else {
       vm_wait_lds<0>();
     }
     // The page numbers of the tile after that.
-    pages = tile_pages(pool, batch, seq, u.length, key0 + (kAhead + 1) * kStep);
+    pages = tile_pages(pool, batch, seq, u.length, key_of(number + (kAhead + 1) * kStep));
     const char* now = ring + slot;
     slot = slot + L::kBytes == kStages * L::kBytes ? 0 : slot + L::kBytes;
     fill = fill + L::kBytes == kStages * L::kBytes ? 0 : fill + L::kBytes;
@@ -318,8 +359,8 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     }
     mfma_results_fence();
 
-    const bool whole = key0 >= all_low && key0 + kTileKeys <= all_high && args.mask == nullptr && !hole[0][0] &&
-                       !hole[0][1];
+    const bool whole = (key0 >= all_low || (kMore && key0 + kTileKeys <= args.sinks)) && key0 + kTileKeys <= all_high &&
+                       args.mask == nullptr && !hole[0][0] && !hole[0][1];
     v8b probs[kCols][kProbParts];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
@@ -332,10 +373,21 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       if (!whole) {
         // A hidden key takes no part in the maxima, and its probability and
         // value scale are zeros whatever the cache holds there.
+        uint32_t line[2] = {};  // bits of the lane's keys among the sequence's rows
+        if (tree && key0 + kTileKeys > start) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = key0 + 16 * h + 4 * g - start;
+            const uint32_t* words = s_line + (16 * c + col) * kLinePitch + max(row, 0) / 32;
+            line[h] = row >= 0 ? __builtin_amdgcn_alignbit(words[1], words[0], row % 32)
+                               : (row > -4 ? words[0] << -row : 0);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = key0 + 16 * (i / 4) + 4 * g + i % 4;
-          bool see = key >= see_low[c] && key < see_high[c] && !hole[0][i / 4];
+          bool see = (key >= see_low[c] || (kMore && key < args.sinks)) && key < see_high[c] && !hole[0][i / 4];
+          if (tree && key >= start) see = key < see_high[c] && !hole[0][i / 4] && (line[i / 4] >> (i % 4) & 1u) != 0;
           if (args.mask != nullptr) see = see && (seen[c][i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
@@ -399,7 +451,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
         }
       }
     }
-    if (args.mask != nullptr) load_mask(key0 + kStep);
+    if (args.mask != nullptr) load_mask(key_of(number + kStep));
     // All reads of the slot are behind this point: the next turn fills it.
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
@@ -469,7 +521,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 }
 
 // Worker blockIdx.x's granules, item by item.
-template <Kv4Type T, int kDim, int kCols>
+template <Kv4Type T, int kDim, int kCols, bool kMore>
 __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
                                                                    Split split, float* __restrict__ partial) {
   if (__builtin_expect(blockIdx.x >= split.workers, 0)) {
@@ -477,8 +529,8 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
     return;
   }
   Deal deal;
-  Cursor at;
-  if (!find_work(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
+  Cursor<kMore> at;
+  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
@@ -488,7 +540,7 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
     const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
-    attend_item<T, kDim, kCols>(pool, batch, args, split, partial, at, from, upto);
+    attend_item<T, kDim, kCols, kMore>(pool, batch, args, split, partial, at, from, upto);
     granule = at.item_at + upto;
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
@@ -593,10 +645,10 @@ int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
 }
 
-Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, int num_cus) {
+Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents, int num_cus) {
   Split s;
   s.share = heads / pool.kv_heads;
-  if (kv4_prompt_takes(pool, batch, heads, type)) {
+  if (kv4_prompt_takes(pool, batch, heads, type, parents)) {
     s = kv4_prompt_split(num_cus);
   } else {
     const int columns = columns_for(pool, batch, heads);
@@ -631,7 +683,10 @@ template <Kv4Type T, int kDim, int kCols>
 hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                          float* partial, hipStream_t stream) {
   const dim3 grid(split.workers + loose_groups(batch)), block(kWaves * kWave);
-  kv4_attend_kernel<T, kDim, kCols><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+  if (args.sinks > 0 || args.parents != nullptr)
+    kv4_attend_kernel<T, kDim, kCols, true><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+  else
+    kv4_attend_kernel<T, kDim, kCols, false><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
   return hipGetLastError();
 }
 
@@ -639,7 +694,7 @@ template <Kv4Type T, int kDim>
 hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                       float* partial, hipStream_t stream) {
   hipError_t e = hipErrorInvalidValue;
-  if (kv4_prompt_takes(pool, batch, args.heads, T))
+  if (kv4_prompt_takes(pool, batch, args.heads, T, args.parents != nullptr))
     e = launch_kv4_prompt(pool, batch, args, T, split, partial, stream);
   else if (kDim > 128 || split.tile_shift == 4)
     e = launch_attend<T, kDim, 1>(pool, batch, args, split, partial, stream);
@@ -666,18 +721,19 @@ hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
 
 size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
   size_t bytes = 0;
-  for (Kv4Type type : {kKv4F32, kKv4BF16}) {  // f16 splits as bfloat16
-    const Split s = split_for(pool, batch, heads, type, num_cus);
-    if (s.one_launch) continue;
-    bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * sizeof(Unfinished));
-  }
+  for (Kv4Type type : {kKv4F32, kKv4BF16})  // f16 splits as bfloat16
+    for (bool parents : {false, true}) {
+      const Split s = split_for(pool, batch, heads, type, parents, num_cus);
+      if (s.one_launch) continue;
+      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * sizeof(Unfinished));
+    }
   return bytes;
 }
 
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              void* workspace, int num_cus, hipStream_t stream) {
   if (batch.rows <= 0) return hipSuccess;
-  const Split split = split_for(pool, batch, args.heads, type, num_cus);
+  const Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, num_cus);
   float* partial = static_cast<float*>(workspace);
   switch (type) {
     case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, stream);

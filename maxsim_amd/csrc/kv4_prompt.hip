@@ -138,9 +138,10 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
 
 __device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
-template <Kv4Type T, int kDim>
+// Keys are numbered as TileRange says in calls with sinks (kMore), else by themselves.
+template <Kv4Type T, int kDim, bool kMore>
 __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                            const Split& split, float* __restrict__ partial, const Cursor& at,
+                                            const Split& split, float* __restrict__ partial, const Cursor<kMore>& at,
                                             uint32_t from, uint32_t upto, char* s_raw) {
   typedef Buffer<kDim> B;
   constexpr int kChunks = kDim / 16, kTiles = kDim / 32;
@@ -148,10 +149,14 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   const SeqWork& u = at.work;
 
   // The first keys' way to registers.
-  const int begin = at.range.low + (int)(from << split.granule_shift);
-  const int end = (int)min((int64_t)at.range.low + ((int64_t)upto << split.granule_shift), (int64_t)at.range.high);
+  const int low = kMore ? 0 : at.range.low;
+  auto key_of = [&](int number) -> int { return kMore ? at.range.key_of(number) : number; };
+  auto number_of = [&](int key) -> int { return kMore ? at.range.number_of(key) : key; };
+  const int begin = low + (int)(from << split.granule_shift);
+  const int end = (int)min((int64_t)low + ((int64_t)upto << split.granule_shift), (int64_t)number_of(at.range.high));
   Staged<kDim> staged;
-  int key = begin + staged_key<kDim>(threadIdx.x);
+  int number = begin + staged_key<kDim>(threadIdx.x);
+  int key = key_of(number);
   stage<kDim>(pool, page_of(pool, batch, at.seq, u.length, key), at.head, key, staged);
 
   // This wave's query rows.
@@ -215,8 +220,9 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   }
   const int all_low = wave_reduce(see_low, [](int a, int b) { return max(a, b); });
   const int all_high = wave_reduce(see_high, [](int a, int b) { return min(a, b); });
-  const int any_low = wave_reduce(sees ? see_low : INT_MAX, [](int a, int b) { return min(a, b); });
-  const int any_high = wave_reduce(sees ? see_high : 0, [](int a, int b) { return max(a, b); });
+  const int window_low = wave_reduce(sees ? see_low : INT_MAX, [](int a, int b) { return min(a, b); });
+  const int any_low = kMore ? 0 : window_low;
+  const int any_high = number_of(wave_reduce(sees ? see_high : 0, [](int a, int b) { return max(a, b); }));
 
   float ref = kUnset, sum = 0.0f;
   v16f o[kTiles];
@@ -224,8 +230,9 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   for (int t = 0; t < kTiles; ++t) o[t] = (v16f)(0.0f);
 
   unstage<kDim>(staged, s_raw);
-  key += kKeys;
-  int page = page_of(pool, batch, at.seq, u.length, key + kKeys);
+  number += kKeys;
+  key = key_of(number);
+  int page = page_of(pool, batch, at.seq, u.length, key_of(number + kKeys));
   stage<kDim>(pool, page_of(pool, batch, at.seq, u.length, key), at.head, key, staged);
   __syncthreads();
   char* now = s_raw;
@@ -233,9 +240,10 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   for (int key0 = begin; key0 < end; key0 += kKeys) {
     if (key0 + kKeys < end) {
       unstage<kDim>(staged, other);
-      key += kKeys;
+      number += kKeys;
+      key = key_of(number);
       stage<kDim>(pool, page, at.head, key, staged);
-      page = page_of(pool, batch, at.seq, u.length, key + kKeys);
+      page = page_of(pool, batch, at.seq, u.length, key_of(number + kKeys));
     }
     const float* scales = reinterpret_cast<const float*>(now + B::kScales);
     const v8h* keys = reinterpret_cast<const v8h*>(now) + lane;
@@ -244,7 +252,8 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     const int step0 = max(0, any_low - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
 #pragma unroll 1
     for (int st = step0; st < step1; ++st) {
-      const int first = key0 + 32 * st;
+      const int first = key_of(key0 + 32 * st);
+      if (kMore && first >= args.sinks && first + 32 <= window_low) continue;
       v4f k4[4], v4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -265,7 +274,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
       float x[16], vs[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = s[i] * k4[i / 4][i % 4], vs[i] = v4[i / 4][i % 4];
-      if (!(first >= all_low && first + 32 <= all_high && args.mask == nullptr && first + 32 <= u.length) ||
+      if (!((first >= all_low || (kMore && first + 32 <= args.sinks)) && first + 32 <= all_high && args.mask == nullptr && first + 32 <= u.length) ||
           __ballot(scales[2 * kKeys + 32 * st + col] != 0.0f) != 0) {
         // A hidden key takes no part in the maxima, and its probability and
         // value scale are zeros whatever the cache holds there.
@@ -276,7 +285,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int local = 8 * (i / 4) + 4 * g + i % 4, k = first + local;
-          const bool see = k >= see_low && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f &&
+          const bool see = (k >= see_low || (kMore && k < args.sinks)) && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f &&
                            (seen[i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
@@ -359,7 +368,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   }
 }
 
-template <Kv4Type T, int kDim>
+template <Kv4Type T, int kDim, bool kMore>
 __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4Pool pool, Kv4Batch batch,
                                                                            Kv4AttendArgs args, Split split,
                                                                            float* __restrict__ partial) {
@@ -371,8 +380,8 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
     return;
   }
   Deal deal;
-  Cursor at;
-  if (!find_work(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
+  Cursor<kMore> at;
+  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
@@ -382,7 +391,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
     const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
-    prompt_item<T, kDim>(pool, batch, args, split, partial, at, from, upto, s_raw);
+    prompt_item<T, kDim, kMore>(pool, batch, args, split, partial, at, from, upto, s_raw);
     granule = at.item_at + upto;
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
@@ -391,14 +400,14 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   note_unfinished(partial, split, kDim, at, parts);
 }
 
-template <Kv4Type T>
+template <Kv4Type T, bool kMore>
 hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                   float* partial, hipStream_t stream) {
   const dim3 grid(split.workers + loose_groups(batch)), block(kPromptWaves * kWave);
   switch (pool.dim) {
-    case 64: kv4_prompt_kernel<T, 64><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 96: kv4_prompt_kernel<T, 96><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 128: kv4_prompt_kernel<T, 128><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 64: kv4_prompt_kernel<T, 64, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 96: kv4_prompt_kernel<T, 96, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 128: kv4_prompt_kernel<T, 128, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -406,7 +415,7 @@ hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArg
 
 }  // namespace
 
-bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type) {
+bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents) {
   // Two workgroups' rows per sequence and head on average, or one where the items
   // fill half the CUs: fewer leave CUs, or parts of them, without work. Heads of
   // 128, 32 on 8, this kernel against kv4_attend.hip's: 8 x 128 tokens behind 4,000
@@ -414,7 +423,7 @@ bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4
   // against 52; 2 x 128 behind 16,000 135 against 141; 32 x 256 behind 1,000, 8 heads
   // on 8, 71 against 114.
   const int64_t rows = (int64_t)batch.rows * (heads / pool.kv_heads), whole = (int64_t)batch.batch * kPromptRows;
-  return type != kKv4F32 && pool.dim <= 128 && batch.offsets != nullptr &&
+  return !parents && type != kKv4F32 && pool.dim <= 128 && batch.offsets != nullptr &&
          (rows >= 2 * whole || (rows >= whole && rows * pool.kv_heads >= 128 * kPromptRows));
 }
 
@@ -428,8 +437,11 @@ Split kv4_prompt_split(int num_cus) {
 
 hipError_t launch_kv4_prompt(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              const Split& split, float* partial, hipStream_t stream) {
-  return type == kKv4F16 ? launch<kKv4F16>(pool, batch, args, split, partial, stream)
-                         : launch<kKv4BF16>(pool, batch, args, split, partial, stream);
+  if (args.sinks > 0)
+    return type == kKv4F16 ? launch<kKv4F16, true>(pool, batch, args, split, partial, stream)
+                           : launch<kKv4BF16, true>(pool, batch, args, split, partial, stream);
+  return type == kKv4F16 ? launch<kKv4F16, false>(pool, batch, args, split, partial, stream)
+                         : launch<kKv4BF16, false>(pool, batch, args, split, partial, stream);
 }
 
 }  // namespace msim

@@ -64,12 +64,20 @@ __device__ __forceinline__ SeqWork seq_work(const Kv4Pool& pool, const Kv4Batch&
   return w;
 }
 
-// The keys that some row of a tile may see, by position alone.
+// The keys that some row of a tile may see, by position alone: low .. high, and of calls
+// with sinks `head` more from 0 on (a multiple of kKeyAlign, as low is).
 struct TileRange {
   int low, high;
   uint32_t granules;
+  int head;
+
+  // The keys of such calls are numbered without the gap between the two.
+  __device__ int key_of(int number) const { return number < head ? number : number - head + low; }
+  __device__ int number_of(int key) const { return key <= head ? key : max(head, key - low + head); }
 };
 
+// kMore: calls with sinks or parents.
+template <bool kMore>
 __device__ __forceinline__ TileRange tile_range(const Kv4AttendArgs& args, const Split& split, const SeqWork& w,
                                                 uint32_t tile) {
   TileRange r;
@@ -79,33 +87,23 @@ __device__ __forceinline__ TileRange tile_range(const Kv4AttendArgs& args, const
     const uint32_t rows = min((tile + 1) << split.tile_shift, (uint32_t)w.rows * split.share);
     r.high = max(0, min(w.length, w.length - w.rows + (int)((rows - 1) / split.share) + 1));
   }
-  const int first = w.length - w.rows + (int)((tile << split.tile_shift) / split.share);
+  // Positions of rows with parents begin anew at each that has none.
+  const int row = kMore && args.parents != nullptr ? 0 : (int)((tile << split.tile_shift) / split.share);
+  const int first = w.length - w.rows + row;
   if (first >= args.window) r.low = min(w.length, (first - args.window + 1)) / kKeyAlign * kKeyAlign;
+  r.head = 0;
+  if constexpr (kMore) r.head = min(r.low, (min(args.sinks, w.length) + kKeyAlign - 1) / kKeyAlign * kKeyAlign);
   r.granules =
-      max(1u, ((uint32_t)max(0, r.high - r.low) + (1u << split.granule_shift) - 1) >> split.granule_shift);
+      max(1u, ((uint32_t)(max(0, r.high - r.low) + r.head) + (1u << split.granule_shift) - 1) >> split.granule_shift);
   return r;
 }
 
+template <bool kMore>
 __device__ __forceinline__ uint32_t seq_granules(const Kv4Pool& pool, const Kv4AttendArgs& args, const Split& split,
                                                  const SeqWork& w) {
   uint32_t sum = 0;
-  for (uint32_t t = 0; t < w.tiles; ++t) sum += tile_range(args, split, w, t).granules;
+  for (uint32_t t = 0; t < w.tiles; ++t) sum += tile_range<kMore>(args, split, w, t).granules;
   return sum * pool.kv_heads;
-}
-
-// Inclusive sums over the lanes (DPP row shifts, then the rows' last lanes).
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  auto add = [&](auto ctrl, auto rows) {
-    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-  };
-  typedef std::integral_constant<int, 0xF> All;
-  add(std::integral_constant<int, 0x111>{}, All{});
-  add(std::integral_constant<int, 0x112>{}, All{});
-  add(std::integral_constant<int, 0x114>{}, All{});
-  add(std::integral_constant<int, 0x118>{}, All{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
-  return v;
 }
 
 // `total` granules among `workers`: the first `extra` have one more.
@@ -120,12 +118,13 @@ struct Deal {
 
 // By a wave together: the deal, and the sequence that holds the first granule
 // of worker `worker` with the granules before it.  False if the worker has none.
+template <bool kMore>
 __device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                           const Split& split, uint32_t worker, int& seq, uint32_t& before,
                                           Deal& deal) {
   const int lane = lane_id();
   auto granules = [&](int b) -> uint32_t {
-    return b < batch.batch ? seq_granules(pool, args, split, seq_work(pool, batch, split, b)) : 0;
+    return b < batch.batch ? seq_granules<kMore>(pool, args, split, seq_work(pool, batch, split, b)) : 0;
   };
   const uint32_t head = granules(lane);
   uint32_t total = head;
@@ -155,6 +154,7 @@ __device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& b
 }
 
 // Walks over the items of the call from a sequence's first one on.
+template <bool kMore>
 struct Cursor {
   int seq = 0;
   uint32_t before = 0;  // granules before the item group (sequence, tile)
@@ -174,7 +174,7 @@ struct Cursor {
     work.length = wave_uniform(w.length);
     work.tiles = wave_uniform(w.tiles);
     tile = 0;
-    range = tile_range(args, split, work, 0);
+    range = tile_range<kMore>(args, split, work, 0);
   }
   // To the item that holds `granule`; false past the last (offsets out of order).
   __device__ __forceinline__ bool seek(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
@@ -182,7 +182,7 @@ struct Cursor {
     while (tile >= work.tiles || granule - before >= range.granules * pool.kv_heads) {
       if (tile < work.tiles) before += range.granules * pool.kv_heads;
       if (tile + 1 < work.tiles) {
-        range = tile_range(args, split, work, ++tile);
+        range = tile_range<kMore>(args, split, work, ++tile);
       } else {
         if (++seq >= batch.batch) return false;
         enter(pool, batch, args, split);
@@ -341,7 +341,8 @@ struct Unfinished {
 __host__ __device__ inline int64_t partial_floats(const Split& split, int dim) {
   return ((int64_t)split.workers * 2 << split.tile_shift) * (dim + 2);
 }
-__device__ __forceinline__ void note_unfinished(float* partial, const Split& split, int dim, const Cursor& at,
+template <bool kMore>
+__device__ __forceinline__ void note_unfinished(float* partial, const Split& split, int dim, const Cursor<kMore>& at,
                                                 int parts) {
   if (threadIdx.x == 0 && blockIdx.x < split.workers && !split.one_launch)
     reinterpret_cast<Unfinished*>(partial + partial_floats(split, dim))[blockIdx.x] =
@@ -349,7 +350,7 @@ __device__ __forceinline__ void note_unfinished(float* partial, const Split& spl
 }
 
 // kv4_prompt.hip: many rows per sequence.
-bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type);
+bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents);
 Split kv4_prompt_split(int num_cus);
 hipError_t launch_kv4_prompt(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              const Split& split, float* partial, hipStream_t stream);

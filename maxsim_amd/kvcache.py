@@ -21,7 +21,7 @@ Every call enqueues its work on the current stream and returns; none copies
 anything to the host, and none records gradients.  Indices on the device are
 not visible to the checks here: lengths are cut to the table, and a page
 number outside the pool is a hole (not written, read back as zeros, taking no
-attention).  ``append`` and ``attend`` can be captured in a HIP graph.
+attention).  ``append``, ``attend`` and ``keep`` can be captured in a HIP graph.
 """
 from __future__ import annotations
 
@@ -134,15 +134,36 @@ class Int4KVCache:
             rows = lengths.shape[0] if offsets is None else int(offsets[-1])
         return self._calls.read(self._handle, page_table, lengths, offsets, rows, _type_number(dtype), None, None)
 
-    def attend(self, q, page_table, lengths, offsets=None, *, scale=None, causal=True, window=None, mask=None,
-               out=None, return_lse=False):
+    def keep(self, page_table, lengths, offsets, kept):
+        """Of the rows that a call added, some stay: ``kept`` int32 [batch, width] lists
+        the numbers of each sequence's rows that do, ascending; the list ends at the
+        first entry that is no such number (-1).  They move up to the end of what
+        the sequence held before, and the new lengths (int32 [batch]) are returned:
+        length - rows + rows kept, 0 at least.  Table, lengths and offsets are those of the call
+        that added the rows; pages that are spare now stay in the table.  A row that
+        lies in a hole is zeros.  At most 2^20 sequences."""
+        return self._calls.keep(self._handle, page_table, lengths, offsets, kept)
+
+    def attend(self, q, page_table, lengths, offsets=None, *, scale=None, causal=True, window=None, sinks=None,
+               mask=None, parents=None, out=None, return_lse=False):
         """Attention of queries [rows, heads, head_dim] over their sequences.
 
         ``heads`` is a multiple of kv_heads; query head h reads key/value head
         ``h // (heads // kv_heads)``.  Row i of a sequence's n stands at position
         p = length - n + i and sees the keys j < length with j <= p (``causal``),
-        j > p - window (``window``) and mask[row, j] (``mask`` bool
-        [rows, width]; keys past its width are hidden).  ``scale`` defaults to
+        j > p - window (``window``) or j < sinks (``sinks``: first tokens that
+        stay visible under a window), and mask[row, j] (``mask`` bool
+        [rows, width]; keys past its width are hidden).
+
+        ``parents`` int32 [rows] makes each sequence's rows a tree of drafted tokens:
+        parents[row] is the number, among the sequence's rows, of the earlier one
+        that the row comes after; any other number (-1): the last token before them.
+        A row then sees the tokens before the sequence's rows, the rows that it comes
+        after and itself, and stands at length - n + the number of rows that it comes
+        after (``sinks`` and ``window`` go by these positions).  A sequence may have 1,024
+        rows then; rows of a longer one see nothing.
+
+        ``scale`` defaults to
         head_dim ** -0.5.  Returns [rows, heads, head_dim] in q's dtype, rounded
         once from single precision sums, and with ``return_lse`` the logarithm
         of each softmax's sum, float32 [rows, heads].  A row that sees nothing
@@ -154,4 +175,4 @@ class Int4KVCache:
             raise ValueError("window must be positive")
         return self._calls.attend(self._handle, q, page_table, lengths, offsets,
                                   self.head_dim ** -0.5 if scale is None else scale, causal, window or 0, mask, out,
-                                  bool(return_lse))
+                                  bool(return_lse), sinks or 0, parents)
