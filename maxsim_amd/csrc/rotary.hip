@@ -89,7 +89,8 @@ struct Runs {
 // A wave has `split`-th parts of a row's heads.
 template <Kv4Type T, bool kAdjacent, bool kWide>
 __global__ __launch_bounds__(kWavesPerGroup* kWave) void rotary_kernel(RotaryPlan plan, RotaryRows q, RotaryRows k,
-                                                                       int64_t rows, const int32_t* __restrict__ positions,
+                                                                       int64_t rows,
+                                                                       const int32_t* __restrict__ positions,
                                                                        int64_t axis_stride, int split) {
   typedef typename Elem<T>::type E;
   constexpr int kGroup = Elem<T>::kGroup;
@@ -129,7 +130,8 @@ __global__ __launch_bounds__(kWavesPerGroup* kWave) void rotary_kernel(RotaryPla
   }
 
   const int heads = q.heads + k.heads, step = split * heads_at_once;
-  const E* in[2] = {static_cast<const E*>(q.in) + row * q.in_row_stride, static_cast<const E*>(k.in) + row * k.in_row_stride};
+  const E* in[2] = {static_cast<const E*>(q.in) + row * q.in_row_stride,
+                    static_cast<const E*>(k.in) + row * k.in_row_stride};
   E* out[2] = {static_cast<E*>(q.out) + row * q.out_row_stride, static_cast<E*>(k.out) + row * k.out_row_stride};
   for (int h0 = part * heads_at_once + lane / lanes; h0 < heads; h0 += kBatch * step) {
     Runs<E, kGroup, kWide> x[kBatch];
@@ -165,7 +167,8 @@ hipError_t launch_type(const RotaryPlan& plan, const RotaryRows rows[2], int64_t
   bool wide = plan.pairs % kGroup == 0 && (plan.dim - 2 * plan.pairs) % (2 * kGroup) == 0;
   for (int i = 0; i < 2; ++i) {
     if (rows[i].heads == 0) continue;
-    for (const void* p : {rows[i].in, (const void*)rows[i].out}) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    for (const void* p : {rows[i].in, static_cast<const void*>(rows[i].out)})
+      wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int64_t s : {rows[i].in_row_stride, rows[i].in_head_stride, rows[i].out_row_stride, rows[i].out_head_stride})
       wide = wide && s * kSize % 16 == 0;
   }

@@ -81,10 +81,9 @@ class CachePages:
         + place in the page; -1 behind the last.  ``rows`` is the capacity for them;
         without it a tensor's sum is fetched from the device.  Enqueued on the current
         stream; can be captured in a HIP graph."""
-        import torch
+        if isinstance(new, int):
+            import torch
 
-        if new is not None and not torch.is_tensor(new):
-            new = int(new)
             if new < 0:
                 raise ValueError("new must not be negative")
             if rows is None:
@@ -92,4 +91,4 @@ class CachePages:
             new = torch.full((self.batch,), min(new, 2**31 - 1), dtype=torch.int32, device=self.device)
         if rows is None:
             rows = 0 if new is None else int(new.clamp(min=0).sum())
-        return self._calls.update(self._handle, new, lengths, int(rows))
+        return self._calls.update(self._handle, new, lengths, rows)
