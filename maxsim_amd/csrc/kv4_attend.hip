@@ -155,35 +155,21 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   const uint32_t tile = at.tile;
   const int seq = at.seq, head = at.head;
 
-  // With parents: of each row of the tile the rows that it comes after and itself, a bit
-  // each (a word more is read than has any), and how many they are.
-  constexpr int kLineWords = kMostDrafts / 32, kLinePitch = kLineWords + 3;  // odd: rows spread over the banks
-  __shared__ uint32_t s_line[kMore ? kRows * kLinePitch : 1];
+  // With parents: of each row of the tile the rows that it comes after and itself, as bits
+  // of the words of 32 keys from first_word on, and how many it comes after.
+  constexpr int kLineWords = kMostDrafts / 32 + 1;  // odd: the lines spread over the banks
+  __shared__ uint32_t s_line[kMore ? kRows * kLineWords : 1];
   __shared__ int s_parent[kMore ? kMostDrafts : 1], s_depth[kMore ? kRows : 1];
   const bool tree = kMore && args.parents != nullptr;
   const int start = u.length - u.rows;  // the first row's position
+  const int first_word = start & -32, drafts = min(u.rows, kMostDrafts);
+  int parents[kMore ? kMostDrafts / (kWaves * kWave) : 1];
   if (tree) {
-    const int drafts = min(u.rows, kMostDrafts);
-    for (int i = threadIdx.x; i < drafts; i += kWaves * kWave) s_parent[i] = args.parents[u.first + i];
-    for (int i = threadIdx.x; i < kRows * kLinePitch; i += kWaves * kWave) s_line[i] = 0;
-    __syncthreads();
-    if (threadIdx.x < kRows) {
-      const int token = (int)((tile * kRows + threadIdx.x) / split.share);
-      auto up = [&](int row) -> int {  // -1 past the first
-        const int parent = s_parent[row];
-        return (uint32_t)parent < (uint32_t)row ? parent : -1;
-      };
-      int depth = 0;
-      if (token < drafts) {
-        for (int row = up(token); row >= 0; row = up(row)) ++depth;
-        int back = 0;
-        for (int row = token; row >= 0; row = up(row), ++back)
-          if (back < args.window || start + depth - back < args.sinks)
-            s_line[threadIdx.x * kLinePitch + row / 32] |= 1u << (row % 32);
-      }
-      s_depth[threadIdx.x] = depth;
+#pragma unroll
+    for (int i = 0; i < kMostDrafts / (kWaves * kWave); ++i) {
+      const int row = i * kWaves * kWave + (int)threadIdx.x;
+      if (row < drafts) parents[i] = args.parents[u.first + row];
     }
-    __syncthreads();
   }
 
   // Query rows of this tile: row r is new token r / share, head r % share.
@@ -201,9 +187,9 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     query[c] = have ? (int64_t)(u.first + token) * args.q_row_stride +
                           (int64_t)(head * split.share + sub) * args.q_head_stride
                     : -1;
-    const int own = start + token, pos = tree ? start + s_depth[16 * c + col] : own;
-    see_low[c] = pos >= args.window ? pos - args.window + 1 : 0;
-    see_high[c] = args.causal ? max(0, min(u.length, own + 1)) : u.length;
+    const int pos = start + token;
+    see_low[c] = !tree && pos >= args.window ? pos - args.window + 1 : 0;
+    see_high[c] = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
     if (tree && u.rows > kMostDrafts) see_high[c] = 0;
     mask[c] = nullptr;
     if (args.mask != nullptr) {
@@ -224,7 +210,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   all_high = wave_reduce(all_high, [](int a, int b) { return min(a, b); });
   any_low = wave_reduce(any_low, [](int a, int b) { return min(a, b); });
   any_high = wave_reduce(any_high, [](int a, int b) { return max(a, b); });
-  if (tree) all_high = min(all_high, max(0, start));
+  if (tree) all_high = min(all_high, max(0, start));  // up to where all rows see all that the window leaves
   // This worker's keys of the item, cut to what some row sees.
   const int low = kMore ? 0 : at.range.low;
   auto key_of = [&](int number) -> int { return kMore ? at.range.key_of(number) : number; };
@@ -241,17 +227,55 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   const int tiles = end > key_first ? (end - key_first + kStep - 1) / kStep : 0;
   const char* ring = s_raw + wave * kStages * L::kBytes;
   const uint32_t ring_lds = lds_address(ring);
+  // The lines are needed where the worker comes to the rows' own keys, and for a window.
+  const bool lines = tree && end > begin && (end > at.range.number_of(start) || args.window != INT_MAX);
   bool hole[kStages][2];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int key = key_of(key_first + i * kStep);
     const TilePages pages = tile_pages(pool, batch, seq, u.length, key);
+    if (kMore && i == 0 && lines) {  // before the tiles, or their arrival is waited for
+#pragma unroll
+      for (int j = 0; j < kMostDrafts / (kWaves * kWave); ++j) {
+        const int row = j * kWaves * kWave + (int)threadIdx.x;
+        if (row < drafts) s_parent[row] = parents[j];
+      }
+      for (int j = threadIdx.x; j < kRows * kLineWords; j += kWaves * kWave) s_line[j] = 0;
+    }
     if (i < tiles) load_tile<kDim>(pool, pages, head, key, ring_lds + i * L::kBytes);
     hole[i][0] = (uint32_t)pages.page[0] >= (uint32_t)pool.num_pages;
     hole[i][1] = (uint32_t)pages.page[1] >= (uint32_t)pool.num_pages;
   }
 
-  // The queries, while the first tiles come.
+  // The lines and the queries, while the first tiles come.
+  if (kMore && lines) {
+    group_sync_lds();
+    if (threadIdx.x < kRows) {
+      const int token = (int)((tile * kRows + threadIdx.x) / split.share);
+      int depth = 0;
+      if (token < drafts) {
+        if (args.window != INT_MAX)
+          for (int row = row_before(s_parent, token); row >= 0; row = row_before(s_parent, row)) ++depth;
+        int back = 0;
+        for (int row = token; row >= 0; row = row_before(s_parent, row), ++back) {
+          const int at = start + row - first_word;
+          if (back < args.window || start + depth - back < args.sinks)
+            s_line[threadIdx.x * kLineWords + at / 32] |= 1u << at % 32;
+        }
+      }
+      s_depth[threadIdx.x] = depth;
+    }
+    group_sync_lds();
+    if (args.window != INT_MAX) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const int pos = start + s_depth[16 * c + col];
+        see_low[c] = query[c] >= 0 && pos >= args.window ? pos - args.window + 1 : 0;
+        all_low = max(all_low, see_low[c]);
+      }
+      all_low = wave_reduce(all_low, [](int a, int b) { return max(a, b); });
+    }
+  }
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
     float x[S::kKeyWords][8];
@@ -373,21 +397,14 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
       if (!whole) {
         // A hidden key takes no part in the maxima, and its probability and
         // value scale are zeros whatever the cache holds there.
-        uint32_t line[2] = {};  // bits of the lane's keys among the sequence's rows
-        if (tree && key0 + kTileKeys > start) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = key0 + 16 * h + 4 * g - start;
-            const uint32_t* words = s_line + (16 * c + col) * kLinePitch + max(row, 0) / 32;
-            line[h] = row >= 0 ? __builtin_amdgcn_alignbit(words[1], words[0], row % 32)
-                               : (row > -4 ? words[0] << -row : 0);
-          }
-        }
+        const bool own = tree && key0 >= first_word;  // some keys of the tile are the sequence's rows
+        const uint32_t line = own ? s_line[(16 * c + col) * kLineWords + (key0 - first_word) / 32] : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int key = key0 + 16 * (i / 4) + 4 * g + i % 4;
-          bool see = (key >= see_low[c] || (kMore && key < args.sinks)) && key < see_high[c] && !hole[0][i / 4];
-          if (tree && key >= start) see = key < see_high[c] && !hole[0][i / 4] && (line[i / 4] >> (i % 4) & 1u) != 0;
+          const int local = 16 * (i / 4) + 4 * g + i % 4, key = key0 + local;
+          bool see = key >= see_low[c] || (kMore && key < args.sinks);
+          if (own && key >= start) see = (line >> local & 1u) != 0;
+          see = see && key < see_high[c] && !hole[0][i / 4];
           if (args.mask != nullptr) see = see && (seen[c][i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
@@ -530,13 +547,12 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   }
   Deal deal;
   Cursor<kMore> at;
-  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
+  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at, deal)) {
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
   uint32_t granule = deal.begin(blockIdx.x);
   const uint32_t last = deal.begin(blockIdx.x + 1);
-  at.enter(pool, batch, args, split);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
     const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
@@ -549,29 +565,77 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   note_unfinished(partial, split, kDim, at, parts);
 }
 
-// Joins the parts of split items: workgroup (i, y) has rows y, y + gridDim.y, ...
-// of the item that worker i left unfinished.
+// Joins the parts of split items. Of an item of up to kDirect parts each wave joins a row
+// by itself, and a workgroup has four rows of it; of more, each wave adds up every
+// kWaves-th part and the waves' sums are joined, and a workgroup has one row. Where many
+// workgroups would find nothing to do, fewer count the pieces of work in the list of parts
+// and take them in turn (`counted`).
 template <Kv4Type T, int kDim>
-__global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split,
-                                                                 float* __restrict__ partial) {
+__global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split, uint32_t rows,
+                                                                 bool counted, float* __restrict__ partial) {
   constexpr int kRegs = (kDim + 63) / 64;
-  __shared__ float s_part[kWaves][kDim + 1];
-  const int wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
-  const uint32_t first = blockIdx.x;
-  const Unfinished item = reinterpret_cast<const Unfinished*>(partial + partial_floats(split, kDim))[first];
-  const int parts = min(item.parts, (int)(split.workers - first));
-  const uint32_t rows = 1u << split.tile_shift;
-  // Up to kDirect parts a wave joins a row by itself; of more, each wave adds up
-  // every kWaves-th part and the waves' sums are joined.
   constexpr int kDirect = kWave / kWaves;
-  const bool direct = parts <= kDirect;
-  const int start = direct ? 0 : wave, stride = direct ? 1 : kWaves;
-  const uint32_t row_step = gridDim.y * (direct ? kWaves : 1);
-  for (uint32_t local = direct ? blockIdx.y * kWaves + wave : blockIdx.y; parts > 0 && local < rows;
-       local += row_step) {
+  __shared__ float s_part[kWaves][kDim + 1];
+  __shared__ uint32_t s_end[kWaves], s_worker, s_piece;
+  __shared__ int s_parts;
+  const int wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
+  const Unfinished* items = reinterpret_cast<const Unfinished*>(partial + partial_floats(split, kDim));
+  const int* counts = reinterpret_cast<const int*>(items + split.workers);
+  auto pieces = [&](int parts) -> uint32_t {
+    return parts == 0 ? 0 : (parts <= kDirect ? (rows + kWaves - 1) / kWaves : rows);
+  };
+  // A thread counts the pieces of kEach workers.
+  constexpr uint32_t kEach = kMostWorkers / (kWaves * kWave);
+  int have_parts[kEach] = {};
+  uint32_t mine = 0, before = 0, all_pieces = 0;
+  if (counted) {
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+      const uint32_t worker = threadIdx.x * kEach + i;
+      have_parts[i] = worker < split.workers ? counts[worker] : 0;
+      mine += pieces(have_parts[i]);
+    }
+    const uint32_t upto = wave_scan(mine);
+    if (lane == kWave - 1) s_end[wave] = upto;
+    __syncthreads();
+    before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) before += s_end[w];
+      all_pieces += s_end[w];
+    }
+  }
+  // Without counting, workgroup (i, y) has the pieces y, y + gridDim.y, ... of worker i.
+  const int own_parts = counted ? 0 : counts[blockIdx.x];
+  const uint32_t step = counted ? gridDim.x : gridDim.y;
+  for (uint32_t work = counted ? blockIdx.x : blockIdx.y; work < (counted ? all_pieces : pieces(own_parts)); work += step) {
+    if (counted && work >= before && work < before + mine) {
+      uint32_t piece = work - before;
+      bool found = false;
+#pragma unroll
+      for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t n = pieces(have_parts[i]);
+        if (!found && piece < n) {
+          found = true;
+          s_worker = threadIdx.x * kEach + i;
+          s_parts = have_parts[i];
+          s_piece = piece;
+        }
+        piece -= found ? 0 : n;
+      }
+    }
+    if (counted) __syncthreads();
+    const uint32_t first = counted ? wave_uniform(s_worker) : blockIdx.x, piece = counted ? wave_uniform(s_piece) : work;
+    const int parts = min(counted ? wave_uniform(s_parts) : own_parts, (int)(split.workers - first));
+    const Unfinished item = items[first];
+    const bool direct = parts <= kDirect;
+    const int start = direct ? 0 : wave, stride = direct ? 1 : kWaves;
+    const uint32_t local = direct ? piece * kWaves + wave : piece;
     const uint32_t r = (item.tile << split.tile_shift) + local;
     const int token = (int)(r / split.share), qh = item.head * split.share + (int)(r - token * split.share);
-    if (token >= item.rows) return;
+    if (counted) __syncthreads();  // the next piece may be written
+    // Without barriers in them for single waves: a row is a wave's, or all waves agree on it.
+    if (local >= rows || token >= item.rows) continue;
     float all = kUnset, total = 0.0f, o[kRegs] = {};
     for (int p0 = 0; p0 < parts; p0 += kWave) {
       const int count = min(kWave, parts - p0);
@@ -579,8 +643,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
         return partial_slot(partial, split, kDim, first + p0 + p, p0 + p == 0);
       };
       const bool have = lane < count;
-      const float* mine = slot(have ? lane : 0) + rows * kDim + 2 * local;
-      const float ref = have ? mine[0] : kUnset, share = have ? mine[1] : 0.0f;
+      const float* sums = slot(have ? lane : 0) + ((int64_t)kDim << split.tile_shift) + 2 * local;
+      const float ref = have ? sums[0] : kUnset, share = have ? sums[1] : 0.0f;
       // All loads of the wave's parts go out before the weights are known.
       float part[kDirect][kRegs];
 #pragma unroll
@@ -659,6 +723,7 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     s.few = num_cus;
   }
   s.share = heads / pool.kv_heads;
+  s.workers = std::min(s.workers, kMostWorkers);
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
   s.one_launch = longest <= kShort;
   if (s.one_launch) s.few = s.workers;
@@ -669,13 +734,16 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
 }
 
 template <Kv4Type T, int kDim>
-hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial,
+hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial, int num_cus,
                        hipStream_t stream) {
-  // One row of a tile per workgroup, or a share of them; without offsets a tile
-  // has as many rows as heads share a key/value head.
+  // Without offsets a tile has as many rows as heads share a key/value head.
   const uint32_t rows = std::min(1u << split.tile_shift, batch.offsets == nullptr ? split.share : UINT32_MAX);
-  kv4_join_kernel<T, kDim><<<dim3(split.workers, std::min(32u, rows)), dim3(kWaves * kWave), 0, stream>>>(args, split,
-                                                                                                      partial);
+  // Up to 4,096 workgroups, where most have nothing to do, cost less than the counting
+  // (3,072 for 32 tokens behind 100 to 8,000 keys: 43.3 us against 44.7; 12,288 for 7 x 5 tokens of
+  // 12 heads 20.4 against 19.7).
+  const bool counted = (uint64_t)split.workers * rows > 4096;
+  const dim3 grid = counted ? dim3(num_cus * 4) : dim3(split.workers, rows);
+  kv4_join_kernel<T, kDim><<<grid, dim3(kWaves * kWave), 0, stream>>>(args, split, rows, counted, partial);
   return hipGetLastError();
 }
 
@@ -692,7 +760,7 @@ hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4At
 
 template <Kv4Type T, int kDim>
 hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
-                      float* partial, hipStream_t stream) {
+                      float* partial, int num_cus, hipStream_t stream) {
   hipError_t e = hipErrorInvalidValue;
   if (kv4_prompt_takes(pool, batch, args.heads, T, args.parents != nullptr))
     e = launch_kv4_prompt(pool, batch, args, T, split, partial, stream);
@@ -701,18 +769,18 @@ hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atten
   else if constexpr (kDim <= 128)
     e = launch_attend<T, kDim, 2>(pool, batch, args, split, partial, stream);
   if (e != hipSuccess || split.one_launch) return e;
-  return launch_join<T, kDim>(batch, args, split, partial, stream);
+  return launch_join<T, kDim>(batch, args, split, partial, num_cus, stream);
 }
 
 template <Kv4Type T>
 hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
-                       float* partial, hipStream_t stream) {
+                       float* partial, int num_cus, hipStream_t stream) {
   switch (pool.dim) {
-    case 64: return launch_dim<T, 64>(pool, batch, args, split, partial, stream);
-    case 96: return launch_dim<T, 96>(pool, batch, args, split, partial, stream);
-    case 128: return launch_dim<T, 128>(pool, batch, args, split, partial, stream);
-    case 192: return launch_dim<T, 192>(pool, batch, args, split, partial, stream);
-    case 256: return launch_dim<T, 256>(pool, batch, args, split, partial, stream);
+    case 64: return launch_dim<T, 64>(pool, batch, args, split, partial, num_cus, stream);
+    case 96: return launch_dim<T, 96>(pool, batch, args, split, partial, num_cus, stream);
+    case 128: return launch_dim<T, 128>(pool, batch, args, split, partial, num_cus, stream);
+    case 192: return launch_dim<T, 192>(pool, batch, args, split, partial, num_cus, stream);
+    case 256: return launch_dim<T, 256>(pool, batch, args, split, partial, num_cus, stream);
   }
   return hipErrorInvalidValue;
 }
@@ -725,7 +793,7 @@ size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int head
     for (bool parents : {false, true}) {
       const Split s = split_for(pool, batch, heads, type, parents, num_cus);
       if (s.one_launch) continue;
-      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * sizeof(Unfinished));
+      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * (sizeof(Unfinished) + sizeof(int)));
     }
   return bytes;
 }
@@ -736,9 +804,9 @@ hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const K
   const Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, num_cus);
   float* partial = static_cast<float*>(workspace);
   switch (type) {
-    case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, stream);
-    case kKv4F16: return launch_type<kKv4F16>(pool, batch, args, split, partial, stream);
-    case kKv4BF16: return launch_type<kKv4BF16>(pool, batch, args, split, partial, stream);
+    case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, num_cus, stream);
+    case kKv4F16: return launch_type<kKv4F16>(pool, batch, args, split, partial, num_cus, stream);
+    case kKv4BF16: return launch_type<kKv4BF16>(pool, batch, args, split, partial, num_cus, stream);
   }
   return hipErrorInvalidValue;
 }

@@ -138,8 +138,9 @@ __device__ __forceinline__ void unstage(const Staged<kDim>& s, char* buffer) {
 
 __device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 
-// Keys are numbered as TileRange says in calls with sinks (kMore), else by themselves.
-template <Kv4Type T, int kDim, bool kMore>
+// Keys are numbered as TileRange says in calls with sinks or parents (kMore; with parents
+// kTree too), else by themselves.
+template <Kv4Type T, int kDim, bool kMore, bool kTree>
 __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                             const Split& split, float* __restrict__ partial, const Cursor<kMore>& at,
                                             uint32_t from, uint32_t upto, char* s_raw) {
@@ -158,6 +159,19 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   int number = begin + staged_key<kDim>(threadIdx.x);
   int key = key_of(number);
   stage<kDim>(pool, page_of(pool, batch, at.seq, u.length, key), at.head, key, staged);
+
+  // With parents: the lines of the wave's rows as in kv4_attend.hip, eight words of them at a
+  // time (of all 1,024 rows they do not fit LDS beside the buffers), made by the wave when it
+  // comes to them.
+  constexpr int kLineWords = 8, kLinePitch = kLineWords + 1;  // odd: the lines spread over the banks
+  __shared__ int s_parent[kTree ? kMostDrafts : 1];
+  __shared__ uint32_t s_line[kTree ? kPromptRows * kLinePitch : 1];
+  const int start = u.length - u.rows;  // the first row's position
+  const int first_word = start & -32, drafts = min(u.rows, kMostDrafts);
+  if constexpr (kTree) {
+    for (int i = threadIdx.x; i < drafts; i += kPromptWaves * kWave) s_parent[i] = args.parents[u.first + i];
+    __syncthreads();
+  }
 
   // This wave's query rows.
   v8h q[kChunks];
@@ -205,26 +219,35 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
       }
     factor = score_factor(args.scale_log2, shift);
   }
-  const int pos = u.length - u.rows + token;
-  int see_low = pos >= args.window ? pos - args.window + 1 : 0;
+  int pos = start + token;
   int see_high = args.causal ? max(0, min(u.length, pos + 1)) : u.length;
+  int depth = 0;
+  if constexpr (kTree) {
+    if (u.rows > kMostDrafts) see_high = 0;
+    if (args.window != INT_MAX && token < drafts)
+      for (int row = row_before(s_parent, token); row >= 0; row = row_before(s_parent, row)) ++depth;
+    pos = start + depth;
+  }
+  int see_low = pos >= args.window ? pos - args.window + 1 : 0;
   const uint8_t* mask = nullptr;
   if (args.mask != nullptr) {
     see_high = (int)min((int64_t)see_high, args.mask_width);
     mask = args.mask + (have ? (int64_t)(u.first + token) * args.mask_row_stride : 0);
   }
-  const bool sees = have && see_high > see_low;
+  const bool sees = have && (kMore ? see_high > 0 : see_high > see_low);
   if (!have) {  // a row of padding: nothing depends on what it sees
     see_low = 0;
     see_high = args.mask != nullptr ? 0 : INT_MAX;
   }
   const int all_low = wave_reduce(see_low, [](int a, int b) { return max(a, b); });
-  const int all_high = wave_reduce(see_high, [](int a, int b) { return min(a, b); });
+  int all_high = wave_reduce(see_high, [](int a, int b) { return min(a, b); });
+  if (kTree) all_high = min(all_high, max(0, start));
   const int window_low = wave_reduce(sees ? see_low : INT_MAX, [](int a, int b) { return min(a, b); });
-  const int any_low = kMore ? 0 : window_low;
+  const int any_low = number_of(window_low);
   const int any_high = number_of(wave_reduce(sees ? see_high : 0, [](int a, int b) { return max(a, b); }));
 
   float ref = kUnset, sum = 0.0f;
+  int words_from = -1;  // of the lines at hand
   v16f o[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) o[t] = (v16f)(0.0f);
@@ -249,11 +272,10 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     const v8h* keys = reinterpret_cast<const v8h*>(now) + lane;
     const v8b* values = reinterpret_cast<const v8b*>(now + B::kKeyBytes) + lane;
     // The 32-key steps that this wave's rows see something of.
-    const int step0 = max(0, any_low - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
+    const int step0 = max(0, (kMore && key_of(key0) < args.sinks ? 0 : any_low) - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
 #pragma unroll 1
     for (int st = step0; st < step1; ++st) {
       const int first = key_of(key0 + 32 * st);
-      if (kMore && first >= args.sinks && first + 32 <= window_low) continue;
       v4f k4[4], v4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -278,6 +300,29 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
           __ballot(scales[2 * kKeys + 32 * st + col] != 0.0f) != 0) {
         // A hidden key takes no part in the maxima, and its probability and
         // value scale are zeros whatever the cache holds there.
+        const bool own = kTree && first >= first_word;  // some keys of the step are the sequence's rows
+        uint32_t line = 0;
+        if (own) {
+          const int word = (first - first_word) / 32, base = word / kLineWords * kLineWords;
+          uint32_t* mine = s_line + (wave * 32 + col) * kLinePitch;
+          if (base != words_from) {
+            words_from = base;
+            wave_sync_lds();
+            if (g == 0) {
+#pragma unroll
+              for (int i = 0; i < kLineWords; ++i) mine[i] = 0;
+              int back = 0;
+              for (int row = token < drafts ? token : -1; row >= 0; row = row_before(s_parent, row), ++back) {
+                const int at = start + row - first_word - 32 * base;
+                if (at < 0) break;
+                if (at < 32 * kLineWords && (back < args.window || start + depth - back < args.sinks))
+                  mine[at / 32] |= 1u << at % 32;
+              }
+            }
+            wave_sync_lds();
+          }
+          line = mine[word - base];
+        }
         uint32_t seen[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -285,8 +330,10 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int local = 8 * (i / 4) + 4 * g + i % 4, k = first + local;
-          const bool see = (k >= see_low || (kMore && k < args.sinks)) && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f &&
-                           (seen[i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
+          bool see = k >= see_low || (kMore && k < args.sinks);
+          if (own && k >= start) see = (line >> local & 1u) != 0;
+          see = see && k < see_high && scales[2 * kKeys + 32 * st + local] == 0.0f &&
+                (seen[i / 4] >> (8 * (i % 4)) & 0xFFu) != 0;
           x[i] = see ? x[i] : kNegInf;
           vs[i] = see ? vs[i] : 0.0f;
         }
@@ -368,7 +415,7 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   }
 }
 
-template <Kv4Type T, int kDim, bool kMore>
+template <Kv4Type T, int kDim, bool kMore, bool kTree>
 __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4Pool pool, Kv4Batch batch,
                                                                            Kv4AttendArgs args, Split split,
                                                                            float* __restrict__ partial) {
@@ -381,17 +428,16 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   }
   Deal deal;
   Cursor<kMore> at;
-  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at.seq, at.before, deal)) {
+  if (!find_work<kMore>(pool, batch, args, split, blockIdx.x, at, deal)) {
     note_unfinished(partial, split, kDim, at, 0);
     return;
   }
   uint32_t granule = deal.begin(blockIdx.x);
   const uint32_t last = deal.begin(blockIdx.x + 1);
-  at.enter(pool, batch, args, split);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
     const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
-    prompt_item<T, kDim, kMore>(pool, batch, args, split, partial, at, from, upto, s_raw);
+    prompt_item<T, kDim, kMore, kTree>(pool, batch, args, split, partial, at, from, upto, s_raw);
     granule = at.item_at + upto;
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
@@ -400,14 +446,14 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   note_unfinished(partial, split, kDim, at, parts);
 }
 
-template <Kv4Type T, bool kMore>
+template <Kv4Type T, bool kMore, bool kTree>
 hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                   float* partial, hipStream_t stream) {
   const dim3 grid(split.workers + loose_groups(batch)), block(kPromptWaves * kWave);
   switch (pool.dim) {
-    case 64: kv4_prompt_kernel<T, 64, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 96: kv4_prompt_kernel<T, 96, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 128: kv4_prompt_kernel<T, 128, kMore><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 64: kv4_prompt_kernel<T, 64, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 96: kv4_prompt_kernel<T, 96, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 128: kv4_prompt_kernel<T, 128, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -423,8 +469,20 @@ bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4
   // against 52; 2 x 128 behind 16,000 135 against 141; 32 x 256 behind 1,000, 8 heads
   // on 8, 71 against 114.
   const int64_t rows = (int64_t)batch.rows * (heads / pool.kv_heads), whole = (int64_t)batch.batch * kPromptRows;
-  return !parents && type != kKv4F32 && pool.dim <= 128 && batch.offsets != nullptr &&
-         (rows >= 2 * whole || (rows >= whole && rows * pool.kv_heads >= 128 * kPromptRows));
+  if (type == kKv4F32 || pool.dim > 128 || batch.offsets == nullptr) return false;
+  // Trees have few rows behind long contexts: where tiles are full to 7 / 8 and there are six
+  // granules of 128 keys for each CU, this kernel's longer way in and out (partial results
+  // of 256 rows) is worth it. Heads of 128, 32 on 8, this kernel against the other: 4 x 64 drafts
+  // behind 20,000 to 65,000 keys 310 us against 395 (41 granules), 1 x 64 behind 60,000 134
+  // against 150 (15), 8 x 64 behind 4,000 81 against 98 (8), 1 x 64 behind 8,000 52 against 44 (2);
+  // tiles full to 3 / 4: 2 x 48 behind 30,000 129 against 120 (15).
+  if (parents) {
+    const int64_t each = rows / std::max(1, batch.batch);
+    const int64_t tiles = (each + kPromptRows - 1) / kPromptRows * batch.batch;
+    const int64_t keys = (int64_t)batch.max_pages << pool.page_shift;
+    return rows * 8 >= tiles * kPromptRows * 7 && tiles * pool.kv_heads * keys >= 6 * kGranule * 256;
+  }
+  return (rows >= 2 * whole || (rows >= whole && rows * pool.kv_heads >= 128 * kPromptRows));
 }
 
 Split kv4_prompt_split(int num_cus) {
@@ -437,11 +495,14 @@ Split kv4_prompt_split(int num_cus) {
 
 hipError_t launch_kv4_prompt(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              const Split& split, float* partial, hipStream_t stream) {
-  if (args.sinks > 0)
-    return type == kKv4F16 ? launch<kKv4F16, true>(pool, batch, args, split, partial, stream)
-                           : launch<kKv4BF16, true>(pool, batch, args, split, partial, stream);
-  return type == kKv4F16 ? launch<kKv4F16, false>(pool, batch, args, split, partial, stream)
-                         : launch<kKv4BF16, false>(pool, batch, args, split, partial, stream);
+  auto run = [&](auto more, auto tree) -> hipError_t {
+    constexpr bool kMore = decltype(more)::value, kTree = decltype(tree)::value;
+    return type == kKv4F16 ? launch<kKv4F16, kMore, kTree>(pool, batch, args, split, partial, stream)
+                           : launch<kKv4BF16, kMore, kTree>(pool, batch, args, split, partial, stream);
+  };
+  if (args.parents != nullptr) return run(std::true_type{}, std::true_type{});
+  if (args.sinks > 0) return run(std::true_type{}, std::false_type{});
+  return run(std::false_type{}, std::false_type{});
 }
 
 }  // namespace msim

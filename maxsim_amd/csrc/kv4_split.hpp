@@ -50,6 +50,8 @@ struct Split {
   uint32_t one_launch;  // no item is split
 };
 
+constexpr uint32_t kMostWorkers = 1024;
+
 struct SeqWork {
   int first, rows, length;
   uint32_t tiles;
@@ -116,43 +118,6 @@ struct Deal {
   }
 };
 
-// By a wave together: the deal, and the sequence that holds the first granule
-// of worker `worker` with the granules before it.  False if the worker has none.
-template <bool kMore>
-__device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                          const Split& split, uint32_t worker, int& seq, uint32_t& before,
-                                          Deal& deal) {
-  const int lane = lane_id();
-  auto granules = [&](int b) -> uint32_t {
-    return b < batch.batch ? seq_granules<kMore>(pool, args, split, seq_work(pool, batch, split, b)) : 0;
-  };
-  const uint32_t head = granules(lane);
-  uint32_t total = head;
-  for (int b0 = kWave; b0 < batch.batch; b0 += kWave) total += granules(b0 + lane);
-  const uint32_t head_scan = wave_scan(head);
-  deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
-                                    : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
-  deal.workers = min(split.workers, max(max(1u, min(deal.total, split.few)), deal.total / 2));
-  deal.each = deal.total / deal.workers;
-  deal.extra = deal.total - deal.each * deal.workers;
-  if (deal.total == 0 || worker >= deal.workers) return false;
-  const uint32_t target = deal.begin(worker);
-  uint32_t done = 0;
-  for (int b0 = 0; b0 < batch.batch; b0 += kWave) {
-    const uint32_t mine = b0 == 0 ? head : granules(b0 + lane);
-    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine)), first = upto - mine;
-    const uint64_t here = __ballot(first <= target && target < upto);
-    if (here != 0) {
-      const int at = __builtin_ctzll(here);
-      seq = wave_uniform(b0 + at);
-      before = __builtin_amdgcn_readlane(first, at);
-      return true;
-    }
-    done = __builtin_amdgcn_readlane(upto, kWave - 1);
-  }
-  return false;
-}
-
 // Walks over the items of the call from a sequence's first one on.
 template <bool kMore>
 struct Cursor {
@@ -166,13 +131,12 @@ struct Cursor {
   int head = 0;
   uint32_t item_at = 0;  // its first granule
 
-  __device__ __forceinline__ void enter(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
-                                        const Split& split) {
-    const SeqWork w = seq_work(pool, batch, split, seq);
-    work.first = wave_uniform(w.first);
-    work.rows = wave_uniform(w.rows);
-    work.length = wave_uniform(w.length);
-    work.tiles = wave_uniform(w.tiles);
+  // The work of sequence `seq` as lane `lane` has it.
+  __device__ __forceinline__ void enter(const Kv4AttendArgs& args, const Split& split, const SeqWork& w, int lane) {
+    work.first = __builtin_amdgcn_readlane(w.first, lane);
+    work.rows = __builtin_amdgcn_readlane(w.rows, lane);
+    work.length = __builtin_amdgcn_readlane(w.length, lane);
+    work.tiles = __builtin_amdgcn_readlane(w.tiles, lane);
     tile = 0;
     range = tile_range<kMore>(args, split, work, 0);
   }
@@ -185,7 +149,7 @@ struct Cursor {
         range = tile_range<kMore>(args, split, work, ++tile);
       } else {
         if (++seq >= batch.batch) return false;
-        enter(pool, batch, args, split);
+        enter(args, split, seq_work(pool, batch, split, seq), 0);
       }
     }
     head = wave_uniform((granule - before) / range.granules);
@@ -193,6 +157,46 @@ struct Cursor {
     return true;
   }
 };
+
+// By a wave together: the deal, and the cursor on the sequence that holds the first
+// granule of worker `worker`.  False if the worker has none.
+template <bool kMore>
+__device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
+                                          const Split& split, uint32_t worker, Cursor<kMore>& cursor, Deal& deal) {
+  const int lane = lane_id();
+  auto work_of = [&](int b) -> SeqWork {
+    return b < batch.batch ? seq_work(pool, batch, split, b) : SeqWork{0, 0, 0, 0};
+  };
+  auto granules = [&](const SeqWork& w) -> uint32_t { return seq_granules<kMore>(pool, args, split, w); };
+  const SeqWork head_work = work_of(lane);
+  const uint32_t head = granules(head_work);
+  uint32_t total = head;
+  for (int b0 = kWave; b0 < batch.batch; b0 += kWave) total += granules(work_of(b0 + lane));
+  const uint32_t head_scan = wave_scan(head);
+  deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
+                                    : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
+  deal.workers = min(split.workers, max(max(1u, min(deal.total, split.few)), deal.total / 2));
+  deal.each = deal.total / deal.workers;
+  deal.extra = deal.total - deal.each * deal.workers;
+  if (deal.total == 0 || worker >= deal.workers) return false;
+  const uint32_t target = deal.begin(worker);
+  uint32_t done = 0;
+  for (int b0 = 0; b0 < batch.batch; b0 += kWave) {
+    const SeqWork work = b0 == 0 ? head_work : work_of(b0 + lane);
+    const uint32_t mine = b0 == 0 ? head : granules(work);
+    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine)), first = upto - mine;
+    const uint64_t here = __ballot(first <= target && target < upto);
+    if (here != 0) {
+      const int at = __builtin_ctzll(here);
+      cursor.seq = wave_uniform(b0 + at);
+      cursor.before = __builtin_amdgcn_readlane(first, at);
+      cursor.enter(args, split, work, at);
+      return true;
+    }
+    done = __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
 
 // -------------------------------------------------------- queries and outputs
 
@@ -324,19 +328,23 @@ __device__ __forceinline__ void loose_rows(const Kv4Batch& batch, const Kv4Atten
   }
 }
 
+// The row that a row with parents comes right after; -1 where it is the context's last.
+__device__ __forceinline__ int row_before(const int* parents, int row) {
+  const int p = parents[row];
+  return (uint32_t)p < (uint32_t)row ? p : -1;
+}
+
 // A worker's slot of partial results: [rows][dim], then [rows][reference, sum].
 __device__ __forceinline__ float* partial_slot(float* partial, const Split& split, int dim, uint32_t worker, bool begins) {
   return partial + (((int64_t)worker * 2 + begins) << split.tile_shift) * (dim + 2);
 }
 
-// Behind the slots: of each worker the item that it begins and leaves to others,
-// for the join.
+// Behind the slots, for the join: of each worker the item that it begins and leaves to
+// others, and behind those in how many parts the item is (0: no such item).
 struct Unfinished {
-  int parts;  // 0: no such item
   int first, rows;  // of its sequence
   uint32_t tile;
   int head;
-  int pad[3];
 };
 __host__ __device__ inline int64_t partial_floats(const Split& split, int dim) {
   return ((int64_t)split.workers * 2 << split.tile_shift) * (dim + 2);
@@ -344,9 +352,11 @@ __host__ __device__ inline int64_t partial_floats(const Split& split, int dim) {
 template <bool kMore>
 __device__ __forceinline__ void note_unfinished(float* partial, const Split& split, int dim, const Cursor<kMore>& at,
                                                 int parts) {
-  if (threadIdx.x == 0 && blockIdx.x < split.workers && !split.one_launch)
-    reinterpret_cast<Unfinished*>(partial + partial_floats(split, dim))[blockIdx.x] =
-        Unfinished{parts, at.work.first, at.work.rows, at.tile, at.head, {}};
+  if (threadIdx.x == 0 && blockIdx.x < split.workers && !split.one_launch) {
+    Unfinished* items = reinterpret_cast<Unfinished*>(partial + partial_floats(split, dim));
+    if (parts > 0) items[blockIdx.x] = Unfinished{at.work.first, at.work.rows, at.tile, at.head};
+    reinterpret_cast<int*>(items + split.workers)[blockIdx.x] = parts;
+  }
 }
 
 // kv4_prompt.hip: many rows per sequence.
