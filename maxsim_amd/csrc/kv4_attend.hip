@@ -555,11 +555,13 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   const uint32_t last = deal.begin(blockIdx.x + 1);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
-    const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
+    const uint32_t size = at.range.granules + split.lead, stop = min(size, last - at.item_at);
+    const uint32_t from = at.own(split, granule - at.item_at), upto = at.own(split, stop);
+    granule = at.item_at + stop;
+    if (from == upto) continue;
     attend_item<T, kDim, kCols, kMore>(pool, batch, args, split, partial, at, from, upto);
-    granule = at.item_at + upto;
     if (from == 0 && upto < at.range.granules)
-      parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
+      parts = (int)(deal.worker_of(at.item_at + size - 1) - blockIdx.x) + 1;
     __syncthreads();
   }
   note_unfinished(partial, split, kDim, at, parts);
@@ -709,10 +711,12 @@ int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
 }
 
-Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents, int num_cus) {
-  Split s;
-  s.share = heads / pool.kv_heads;
-  if (kv4_prompt_takes(pool, batch, heads, type, parents)) {
+// `args` nullptr: any call with or without parents, of those that need a workspace.
+Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents,
+                const Kv4AttendArgs* args, int num_cus) {
+  Split s{};
+  const bool prompt = kv4_prompt_takes(pool, batch, heads, type, parents);
+  if (prompt) {
     s = kv4_prompt_split(num_cus);
   } else {
     const int columns = columns_for(pool, batch, heads);
@@ -725,11 +729,31 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   s.share = heads / pool.kv_heads;
   s.workers = std::min(s.workers, kMostWorkers);
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
-  s.one_launch = longest <= kShort;
-  if (s.one_launch) s.few = s.workers;
-  s.granule_shift = __builtin_ctz(s.one_launch ? kShort : kGranule);
   const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
-  while (items * ((longest >> s.granule_shift) + 1) >= (int64_t)1 << 31) ++s.granule_shift;
+  s.one_launch = longest <= kShort;
+  int64_t whole = kShort;  // keys of a granule that is an item
+  const bool more = args != nullptr && (args->sinks > 0 || parents);
+  if (more && !prompt) {
+    // Of these calls, whose keys a window may count, items of up to 17 granules stay whole
+    // where there are 16 for each granule of one. 32 heads of 128 on 8, one token each of 64
+    // sequences, window 1,024: 24 us against 32 split, 2,048: 37 against 43; of 32 sequences 20
+    // against 24, and 29 against 28; of 8, 19 against 16; 8 tokens of 32: 27 against 35. At windows
+    // of 4,096 sequences of 100 to 4,200 keys took 54 us against 46.
+    int64_t keys = longest;
+    if (args->causal && !parents)
+      keys = std::min(keys, (int64_t)args->window + (1 << s.tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
+    const int64_t granules = (keys + kGranule - 1) / kGranule;
+    const int64_t tiles = ((int64_t)batch.rows * s.share / std::max(1, batch.batch) + (1 << s.tile_shift) - 1) >> s.tile_shift;
+    s.one_launch = keys <= kShort || (granules <= 17 && tiles * batch.batch * pool.kv_heads >= 16 * granules);
+    while (whole < keys && s.one_launch) whole *= 2;
+  }
+  // An item costs its worker as much as four granules besides its own (queries, the waves' join):
+  // 32 x 16 drafts behind 100 to 4,000 keys take 74 us, dealt out by granules alone 134; 4 x 500
+  // tokens behind 100 to 9,000, window 4,096, 221 and 349.
+  if (more && !s.one_launch) s.lead = 4;
+  if (s.one_launch) s.few = s.workers;
+  s.granule_shift = __builtin_ctzll(s.one_launch ? whole : kGranule);
+  while (items * ((longest >> s.granule_shift) + 1 + s.lead) >= (int64_t)1 << 31) ++s.granule_shift;
   return s;
 }
 
@@ -791,7 +815,7 @@ size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int head
   size_t bytes = 0;
   for (Kv4Type type : {kKv4F32, kKv4BF16})  // f16 splits as bfloat16
     for (bool parents : {false, true}) {
-      const Split s = split_for(pool, batch, heads, type, parents, num_cus);
+      const Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
       if (s.one_launch) continue;
       bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * (sizeof(Unfinished) + sizeof(int)));
     }
@@ -801,7 +825,7 @@ size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int head
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              void* workspace, int num_cus, hipStream_t stream) {
   if (batch.rows <= 0) return hipSuccess;
-  const Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, num_cus);
+  const Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, &args, num_cus);
   float* partial = static_cast<float*>(workspace);
   switch (type) {
     case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, num_cus, stream);

@@ -436,11 +436,13 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   const uint32_t last = deal.begin(blockIdx.x + 1);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
-    const uint32_t from = granule - at.item_at, upto = min(at.range.granules, last - at.item_at);
+    const uint32_t size = at.range.granules + split.lead, stop = min(size, last - at.item_at);
+    const uint32_t from = at.own(split, granule - at.item_at), upto = at.own(split, stop);
+    granule = at.item_at + stop;
+    if (from == upto) continue;
     prompt_item<T, kDim, kMore, kTree>(pool, batch, args, split, partial, at, from, upto, s_raw);
-    granule = at.item_at + upto;
     if (from == 0 && upto < at.range.granules)
-      parts = (int)(deal.worker_of(at.item_at + at.range.granules - 1) - blockIdx.x) + 1;
+      parts = (int)(deal.worker_of(at.item_at + size - 1) - blockIdx.x) + 1;
     __syncthreads();
   }
   note_unfinished(partial, split, kDim, at, parts);

@@ -48,6 +48,7 @@ struct Split {
   uint32_t granule_shift;
   uint32_t few;         // workers may have a single granule while there are no more of them
   uint32_t one_launch;  // no item is split
+  uint32_t lead;        // granules that an item is dealt out as, besides its own
 };
 
 constexpr uint32_t kMostWorkers = 1024;
@@ -104,7 +105,7 @@ template <bool kMore>
 __device__ __forceinline__ uint32_t seq_granules(const Kv4Pool& pool, const Kv4AttendArgs& args, const Split& split,
                                                  const SeqWork& w) {
   uint32_t sum = 0;
-  for (uint32_t t = 0; t < w.tiles; ++t) sum += tile_range<kMore>(args, split, w, t).granules;
+  for (uint32_t t = 0; t < w.tiles; ++t) sum += tile_range<kMore>(args, split, w, t).granules + split.lead;
   return sum * pool.kv_heads;
 }
 
@@ -129,7 +130,7 @@ struct Cursor {
 
   // The item at hand.
   int head = 0;
-  uint32_t item_at = 0;  // its first granule
+  uint32_t item_at = 0;  // where it begins
 
   // The work of sequence `seq` as lane `lane` has it.
   __device__ __forceinline__ void enter(const Kv4AttendArgs& args, const Split& split, const SeqWork& w, int lane) {
@@ -143,8 +144,8 @@ struct Cursor {
   // To the item that holds `granule`; false past the last (offsets out of order).
   __device__ __forceinline__ bool seek(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                        const Split& split, uint32_t granule) {
-    while (tile >= work.tiles || granule - before >= range.granules * pool.kv_heads) {
-      if (tile < work.tiles) before += range.granules * pool.kv_heads;
+    while (tile >= work.tiles || granule - before >= (range.granules + split.lead) * pool.kv_heads) {
+      if (tile < work.tiles) before += (range.granules + split.lead) * pool.kv_heads;
       if (tile + 1 < work.tiles) {
         range = tile_range<kMore>(args, split, work, ++tile);
       } else {
@@ -152,9 +153,13 @@ struct Cursor {
         enter(args, split, seq_work(pool, batch, split, seq), 0);
       }
     }
-    head = wave_uniform((granule - before) / range.granules);
-    item_at = before + head * range.granules;
+    head = wave_uniform((granule - before) / (range.granules + split.lead));
+    item_at = before + head * (range.granules + split.lead);
     return true;
+  }
+  // Of what is dealt out from `from` to `upto` (counted from item_at) the item's own granules.
+  __device__ __forceinline__ uint32_t own(const Split& split, uint32_t at) const {
+    return min(range.granules, at - min(at, split.lead));
   }
 };
 
