@@ -17,6 +17,7 @@
 #include <cstdlib>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -102,6 +103,11 @@ struct Launch {
     stream = c10::hip::getCurrentHIPStream(device.index()).stream();
   }
 };
+
+// Memory of a GPU: at::empty without the way through the dispatcher.
+at::Tensor allocate(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  return at::detail::empty_cuda(sizes, type, device, std::nullopt);
+}
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   TORCH_CHECK_VALUE(THPVariable_Check(o), name, " must be a tensor");
@@ -301,10 +307,9 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[6] == Py_None) {
     const int64_t rows = integer(a[4]), type = integer(a[5]);
     TORCH_CHECK_VALUE(rows >= 0, "rows must not be negative");
-    const auto options = at::TensorOptions().device(c.device).dtype(
-        type == MSIM_F32 ? at::kFloat : (type == MSIM_F16 ? at::kHalf : at::kBFloat16));
-    k = at::empty({rows, c.pool.kv_heads, c.pool.dim}, options);
-    v = at::empty({rows, c.pool.kv_heads, c.pool.dim}, options);
+    const at::ScalarType dtype = type == MSIM_F32 ? at::kFloat : (type == MSIM_F16 ? at::kHalf : at::kBFloat16);
+    k = allocate({rows, c.pool.kv_heads, c.pool.dim}, dtype, c.device);
+    v = allocate({rows, c.pool.kv_heads, c.pool.dim}, dtype, c.device);
   } else {
     k = row_tensor(c, a[6], "out[0]", c.pool.kv_heads);
     v = row_tensor(c, a[7], "out[1]", c.pool.kv_heads);
@@ -356,7 +361,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   at::Tensor out, lse, work;
   if (a[9] == Py_None) {
-    out = at::empty({rows, heads, c.pool.dim}, q.options().requires_grad(false));
+    out = allocate({rows, heads, c.pool.dim}, q.scalar_type(), c.device);
   } else {
     out = row_tensor(c, a[9], "out", heads);
     TORCH_CHECK_VALUE(out.scalar_type() == q.scalar_type() && out.size(0) == rows, "out must have q's shape and dtype");
@@ -365,11 +370,11 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(!share_memory(out, q, true), "out must not overlap q, unless it is q");
   }
   const bool want_lse = a[10] == Py_True;
-  if (want_lse) lse = at::empty({rows, heads}, at::TensorOptions().device(c.device).dtype(at::kFloat));
+  if (want_lse) lse = allocate({rows, heads}, at::kFloat, c.device);
   const Launch launch(c.device);
   uint64_t need = 0;
   check(abi.attend_workspace(&c.pool, b.batch, b.max_pages, rows, heads, &need));
-  if (need > 0) work = at::empty({(int64_t)need}, at::TensorOptions().device(c.device).dtype(at::kByte));
+  if (need > 0) work = allocate({(int64_t)need}, at::kByte, c.device);
   check(abi.attend(&c.pool, b.table, b.lengths, b.offsets, b.batch, b.max_pages, rows, q.const_data_ptr(), q.stride(0),
                    q.stride(1), heads, type_of(q.scalar_type()), scale, causal, integer(a[7]), mask, mask_stride,
                    mask_width, integer(a[11]), parents, out.data_ptr(), out.stride(0), out.stride(1),
@@ -389,7 +394,7 @@ PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Batch b = read_batch(c, a[1], a[2], a[3], a[3] == Py_None ? batch : kMostRows);
   const at::Tensor& kept = index_tensor(a[4], "kept", 2, c.device);
   TORCH_CHECK_VALUE(kept.size(0) == b.batch, "kept must have shape [batch, width]");
-  const at::Tensor out = at::empty({b.batch}, kept.options());
+  const at::Tensor out = allocate({b.batch}, at::kInt, c.device);
   const Launch launch(c.device);
   check(abi.keep(&c.pool, b.table, b.lengths, b.offsets, b.batch, b.max_pages, b.rows, ints(kept), kept.size(1),
                  static_cast<int32_t*>(out.data_ptr()), launch.stream));
@@ -424,8 +429,9 @@ PyObject* update(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t rows = integer(a[3]);
   TORCH_CHECK_VALUE(rows >= 0, "rows must not be negative");
   TORCH_CHECK_NOT_IMPLEMENTED(rows <= kMostRows, "a call takes at most 2^26 rows");
-  const at::Tensor offsets = at::empty({batch + 1}, p.table.options()), positions = at::empty({rows}, p.table.options());
-  const at::Tensor slots = at::empty({rows}, p.table.options().dtype(at::kLong));
+  const at::Device device = p.table.device();
+  const at::Tensor offsets = allocate({batch + 1}, at::kInt, device), positions = allocate({rows}, at::kInt, device);
+  const at::Tensor slots = allocate({rows}, at::kLong, device);
   const Launch launch(p.table.device());
   auto address = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
   check(abi.pages(address(p.table), address(p.lengths), address(p.free_pages), address(p.free_count), batch,
@@ -475,8 +481,8 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor out[2];
   if (a[4] == Py_None) {
     TORCH_CHECK_VALUE(a[5] == Py_None, "out must hold a tensor for q");
-    out[0] = at::empty(q.sizes(), q.options().requires_grad(false));
-    if (two) out[1] = at::empty(k.sizes(), k.options().requires_grad(false));
+    out[0] = allocate(q.sizes(), q.scalar_type(), device);
+    if (two) out[1] = allocate(k.sizes(), k.scalar_type(), device);
   } else {
     TORCH_CHECK_VALUE((a[5] != Py_None) == two, "out must hold a tensor for each of q and k");
     for (int i = 0; i < 1 + two; ++i) {
@@ -542,7 +548,7 @@ PyObject* multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
   sizes.back() = w.n;
   at::Tensor out;
   if (a[2] == Py_None) {
-    out = at::empty(sizes, x.options().requires_grad(false));
+    out = allocate(sizes, x.scalar_type(), x.device());
   } else {
     out = tensor(a[2], "out");
     TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(sizes) && out.scalar_type() == x.scalar_type() &&

@@ -60,7 +60,7 @@ def binding_command(out: str) -> list[str]:
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
             *(f"-I{path}" for path in includes), BINDING_SRC, "-o", out, f"-L{os.path.join(home, 'lib')}", "-ltorch",
-            "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python"]
+            "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python"]
 
 
 def _binding_command_or_none(out: str) -> list[str] | None:
