@@ -2,8 +2,8 @@
 
 A MaxSim search finds passages for a batch of queries; one attention layer of a
 reader takes the passages' tokens into its key/value cache and decodes a few
-tokens over them: projections by ``Int4Linear``, keys and values into
-``Int4KVCache``, attention over it.  Synthetic corpus, random weights; the passages'
+tokens over them: pages by ``CachePages``, projections by ``Int4Linear``, positions by
+``Rotary``, keys and values into ``Int4KVCache``, attention over it.  Synthetic corpus, random weights; the passages'
 token embeddings stand for the hidden states that a reader's lower layers would make
 of their text.
 
@@ -40,26 +40,40 @@ class ReaderLayer:
         self.linear = {name: maxsim.Int4Linear.from_float(w, group_size=32) for name, w in self.weights.items()}
         pages = -(-tokens // page_size)  # of a sequence, at most
         self.cache = maxsim.Int4KVCache(batch * pages, KV_HEADS, HEAD_DIM, page_size=page_size)
-        self.table = torch.arange(batch * pages, dtype=torch.int32, device="cuda").view(batch, pages)
-        self.lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
+        self.pages = maxsim.CachePages(batch * pages, batch, pages, page_size=page_size)
+        self.rotary = maxsim.Rotary(HEAD_DIM)
+        self.ones = torch.ones(batch, dtype=torch.int32, device="cuda")
 
     def __call__(self, x, offsets=None):
         """New tokens x [rows, WIDTH] of every sequence (offsets; without: one each)
         attend to what the cache holds and to themselves."""
-        self.lengths += 1 if offsets is None else offsets[1:] - offsets[:-1]
+        new = self.ones if offsets is None else offsets[1:] - offsets[:-1]
+        offsets, positions, _ = self.pages.update(new, rows=x.shape[0])
         q = self.linear["q"](x).view(-1, HEADS, HEAD_DIM)
         k = self.linear["k"](x).view(-1, KV_HEADS, HEAD_DIM)
         v = self.linear["v"](x).view(-1, KV_HEADS, HEAD_DIM)
-        self.cache.append(k, v, self.table, self.lengths, offsets)
-        out = self.cache.attend(q, self.table, self.lengths, offsets)
+        q, k = self.rotary(q, k, positions)
+        self.cache.append(k, v, self.pages.table, self.pages.lengths, offsets)
+        out = self.cache.attend(q, self.pages.table, self.pages.lengths, offsets)
         return self.linear["o"](out.view(-1, HEADS * HEAD_DIM))
+
+
+def plain_rotary(x):
+    """Rows [tokens, heads, HEAD_DIM] turned by their places."""
+    pairs = HEAD_DIM // 2
+    frequencies = 10000.0 ** (-torch.arange(pairs, dtype=torch.float64, device=x.device) / pairs)
+    angle = torch.arange(x.shape[0], device=x.device)[:, None, None] * frequencies
+    cos, sin = angle.cos().to(x.dtype), angle.sin().to(x.dtype)
+    a, b = x[..., :pairs], x[..., pairs:]
+    return torch.cat((a * cos - b * sin, a * sin + b * cos), -1)
 
 
 def plain_layer(weights, sequence):
     """The same layer on one whole sequence [tokens, WIDTH], unquantised."""
     q, k, v = (sequence @ weights[name].t() for name in "qkv")
-    q = q.view(-1, HEADS, HEAD_DIM).transpose(0, 1)
-    k, v = (t.view(-1, KV_HEADS, HEAD_DIM).transpose(0, 1).repeat_interleave(HEADS // KV_HEADS, 0) for t in (k, v))
+    q = plain_rotary(q.view(-1, HEADS, HEAD_DIM)).transpose(0, 1)
+    k, v = plain_rotary(k.view(-1, KV_HEADS, HEAD_DIM)), v.view(-1, KV_HEADS, HEAD_DIM)
+    k, v = (t.transpose(0, 1).repeat_interleave(HEADS // KV_HEADS, 0) for t in (k, v))
     s = q @ k.transpose(1, 2).contiguous() / HEAD_DIM**0.5
     s = s.masked_fill(torch.ones(s.shape[1:], dtype=torch.bool, device=s.device).triu(1), -torch.inf)
     out = torch.softmax(s, -1) @ v

@@ -53,7 +53,8 @@ class Rotary:
         if min(axes) < 0 or max(axes) >= pairs:
             raise ValueError("axes must be numbered from 0, and be no more than the pairs")
         self.device = _cuda_device(device)
-        self.head_dim, self.rotary_dim, self.num_axes, self.adjacent = head_dim, rotary_dim, max(axes) + 1, bool(adjacent)
+        self.head_dim, self.rotary_dim = head_dim, rotary_dim
+        self.num_axes, self.adjacent = max(axes) + 1, bool(adjacent)
         # Turns per position, in 2^-64, whole turns dropped (as two's complement numbers).
         turns = [round(Fraction(f) / _TURN * 2**64) % 2**64 for f in frequencies]
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64,

@@ -291,6 +291,111 @@ def test_drafts_that_a_row_does_not_come_after_have_no_effect(gpu):
         assert torch.equal(got[row], clean[row])
 
 
+# A table as wide as for long contexts sends trees that fill tiles of 256 query rows
+# through the kernel for prompts.
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 64), (128, 32)])
+@pytest.mark.parametrize("window,sinks", [(None, None), (3, 2), (40, 130), (300, 5)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_large_trees(gpu, kind, dim, page, window, sinks, masked):
+    cache = Int4KVCache(2400 // page, 2, dim, page_size=page)
+    _fill(cache, page)
+    new = [60, 64, 58, 63]
+    batch = Batch(cache, [275, 64, 900, 131], new, seed=1, spare=40000 // page)
+    parents = _tree(new, dim, lean=0.4)
+    q = _queries(batch.rows, 8, dim, kind, 3)
+    mask = (torch.rand((batch.rows, 880), generator=_rng(4)) < 0.7).cuda() if masked else None
+    got, lse = cache.attend(q, *batch.args, parents=parents.cuda(), window=window, sinks=sinks, mask=mask,
+                            return_lse=True)
+    _check(cache, batch, q, got, lse, parents=parents, window=window, sinks=sinks, mask=mask)
+
+
+@pytest.mark.parametrize("chain", [False, True])
+@pytest.mark.parametrize("lengths", [[1300, 1024], [1057, 2000], [1025, 900]])
+def test_trees_of_many_words(gpu, chain, lengths):
+    """A thousand rows of a sequence, more of them than it holds too, and of one too many."""
+    cache = Int4KVCache(300, 2, 64, page_size=16)
+    _fill(cache, 6)
+    for new in ([1024, 1000], [1025, 1020]):
+        batch = Batch(cache, lengths, new, seed=1, spare=3000)
+        parents = torch.cat([torch.arange(n) - 1 for n in new]).to(torch.int32) if chain else _tree(new, 5, lean=0.7)
+        q = _queries(batch.rows, 2, 64, BF16, 3)
+        for kw in ({}, {"window": 200, "sinks": 1100}):
+            got, lse = cache.attend(q, *batch.args, parents=parents.cuda(), return_lse=True, **kw)
+            _check(cache, batch, q, got, lse, parents=parents, **kw)
+
+
+# Many sequences, whose items stay whole in one launch.
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("share,new", [(1, 1), (4, 1), (4, 7), (1, 40), (40, 2)])
+@pytest.mark.parametrize("window,sinks", [(700, 40), (1500, 3), (95, 260)])
+def test_many_sequences_with_sinks(gpu, kind, share, new, window, sinks):
+    g = _rng(new)
+    lengths = torch.randint(1, 1900, (40,), generator=g).tolist()
+    lengths[:3] = [1900, 2, 0]
+    cache = Int4KVCache(sum(-(-n // 32) for n in lengths), 4, 64, page_size=32)
+    _fill(cache, 8)
+    rows = [min(n, new) for n in lengths]
+    batch = Batch(cache, lengths, rows, seed=3, spare=200)
+    q = _queries(batch.rows, 4 * share, 64, kind, 3)
+    got, lse = cache.attend(q, *batch.args, window=window, sinks=sinks, return_lse=True)
+    _check(cache, batch, q, got, lse, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("share,new", [(1, 3), (4, 12)])
+def test_many_sequences_with_trees(gpu, kind, share, new):
+    g = _rng(new)
+    lengths = torch.randint(1, 1000, (70,), generator=g).tolist()
+    lengths[:3] = [1000, 2, 0]
+    cache = Int4KVCache(sum(-(-n // 32) for n in lengths), 4, 64, page_size=32)
+    _fill(cache, 8)
+    rows = [min(n, new) for n in lengths]
+    batch = Batch(cache, lengths, rows, seed=3)
+    parents = _tree(rows, 5)
+    q = _queries(batch.rows, 4 * share, 64, kind, 3)
+    for kw in ({}, {"window": 100, "sinks": 20}):
+        got, lse = cache.attend(q, *batch.args, parents=parents.cuda(), return_lse=True, **kw)
+        _check(cache, batch, q, got, lse, parents=parents, **kw)
+
+
+@pytest.mark.parametrize("lo,hi,new", [(1, 2500, 9), (1, 700, 33), (2000, 6000, 2)])
+def test_ragged_split_items(gpu, lo, hi, new):
+    """Short and long sequences dealt out together."""
+    lengths = torch.randint(lo, hi, (24,), generator=_rng(hi)).tolist()
+    cache = Int4KVCache(sum(-(-n // 16) for n in lengths), 2, 64, page_size=16)
+    _fill(cache, 8)
+    rows = [min(n, new) for n in lengths]
+    batch = Batch(cache, lengths, rows, seed=3, spare=200)
+    parents = _tree(rows, 5)
+    q = _queries(batch.rows, 4, 64, BF16, 3)
+    got, lse = cache.attend(q, *batch.args, parents=parents.cuda(), return_lse=True)
+    _check(cache, batch, q, got, lse, parents=parents)
+    got, lse = cache.attend(q, *batch.args, window=4000, sinks=9, return_lse=True)
+    _check(cache, batch, q, got, lse, window=4000, sinks=9)
+
+
+def test_another_stream(gpu):
+    cache = Int4KVCache(300, 2, 128, page_size=16)
+    _fill(cache, 3)
+    new = [20, 9]
+    batch = Batch(cache, [3001, 1500], new, seed=2)
+    parents = _tree(new, 8).cuda()
+    kept = torch.tensor([[1, 4, 9], [0, 2, -1]], dtype=torch.int32, device="cuda")
+    q = _queries(batch.rows, 8, 128, BF16, 3)
+    want = cache.attend(q, *batch.args, parents=parents, window=900, sinks=7)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            assert torch.equal(cache.attend(q, *batch.args, parents=parents, window=900, sinks=7), want)
+        assert cache.keep(*batch.args, kept).tolist() == [2984, 1493]
+
+
 # ------------------------------------------------------------------ kept rows
 
 
@@ -352,6 +457,23 @@ def test_kept_rows_and_bad_indices(gpu):
     # Sequence 2: rows 0 and 1 stand before its first token; row 4 at 2 goes to 0.
     assert torch.equal(cache.k_codes[t[2, 0], :, 0], codes[t[2, 0], :, 2])
     assert torch.equal(cache.k_scales[t[2, 0], :, 1:], scales[t[2, 0], :, 1:])
+
+
+def test_kept_rows_past_32_bits(gpu):
+    """Pages whose codes begin past 2^32 bytes."""
+    cache = Int4KVCache(132000, 8, 128, page_size=64)
+    table = torch.tensor([[131999, 131072], [3, 131998]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([70, 100], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")
+    x = [torch.randn((50, 8, 128), generator=_rng(i)).cuda() for i in (1, 2)]
+    cache.append(*x, table, lengths, offsets)
+    before = cache.read(table, lengths, offsets, rows=50, dtype=F32)
+    kept = torch.tensor([[3, 13, 19], [2, 28, -1]], dtype=torch.int32, device="cuda")
+    after = cache.keep(table, lengths, offsets, kept)
+    ends = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    index = torch.tensor([3, 13, 19, 22, 48], device="cuda")
+    for a, b in zip(cache.read(table, after, ends, rows=5, dtype=F32), before):
+        assert torch.equal(a, b[index])
 
 
 def test_kept_rows_of_single_tokens_and_empty_calls(gpu):

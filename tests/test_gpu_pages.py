@@ -86,8 +86,10 @@ def test_steps(gpu, batch, max_pages, page, num_pages):
         kind = step % 4
         new = [rng.choice([0, 1, rng.randint(0, most)]) if kind == 0 else rng.randint(0, 9) if kind == 1
                else rng.choice([1, 1, -3, most + 1, 2**31 - 1]) if kind == 2 else 1 for _ in range(batch)]
-        cut = None if step % 3 == 0 else [rng.choice([n, n - rng.randint(0, 20), 0, 2**31 - 1, -5]) if rng.random() < 0.5
-                                          else n for n in lists.lengths]
+        cut = None
+        if step % 3:
+            cut = [rng.choice([n, n - rng.randint(0, 20), 0, 2**31 - 1, -5]) if rng.random() < 0.5 else n
+                   for n in lists.lengths]
         total = sum(min(max(n, 0), most) for n in new)
         rows = rng.choice([total, total + 7, total // 2, total])
         _step(pages, lists, new, cut, rows)

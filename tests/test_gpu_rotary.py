@@ -133,6 +133,19 @@ def test_values_at_the_ends(gpu):
     assert rotary(x, x[:, :0], positions)[1].shape == (3, 0, 8)
 
 
+def test_rows_past_32_bits(gpu):
+    """Rows that begin past 2^31 elements."""
+    wide = torch.zeros(2**31 + 2**20, dtype=F16, device="cuda")
+    q = wide[:2**31 + 1024].as_strided((3, 4, 64), (2**30, 64, 1))
+    q.copy_(_inputs(3, 4, 64, F16, 8))
+    positions = _positions(1, 3, 900, 3)
+    rotary = Rotary(64)
+    want = rotary(q.contiguous(), None, positions)[0]
+    assert torch.equal(rotary(q, None, positions)[0], want)
+    rotary(q, None, positions, out=(q, None))
+    assert torch.equal(q, want)
+
+
 def test_graph_replays(gpu):
     rotary = Rotary(64, axes=[0] * 16 + [1] * 16)
     q, k, positions = _inputs(5, 4, 64, BF16, 1), _inputs(5, 2, 64, BF16, 2), _positions(2, 5, 900, 3)
@@ -162,8 +175,8 @@ def test_refusals(gpu):
     rotary, two = Rotary(8), Rotary(8, axes=[0, 0, 1, 1])
     q, p = torch.zeros((3, 2, 8), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
     wide = torch.zeros((3, 4, 8), device="cuda")
-    for r, args, kw in ((rotary, (q[..., :6], None, p), {}), (rotary, (q, q.half(), p), {}), (rotary, (q, q[:2], p), {}),
-                        (rotary, (q, None, p.long()), {}), (rotary, (q, None, p[:2]), {}), (two, (q, None, p), {}),
+    for r, args, kw in ((rotary, (q[..., :6], None, p), {}), (rotary, (q, q.half(), p), {}),
+                        (rotary, (q, q[:2], p), {}), (rotary, (q, None, p.long()), {}), (rotary, (q, None, p[:2]), {}), (two, (q, None, p), {}),
                         (two, (q, None, p.expand(3, 3)), {}), (rotary, (q, None, p.cpu()), {}),
                         (rotary, (q.double(), None, p), {}), (rotary, (q.cpu(), None, p), {}),
                         (rotary, (q.transpose(1, 2).contiguous().transpose(1, 2), None, p), {}),

@@ -73,7 +73,8 @@ def test_rotary_checks(change, status, text):
 
 def test_calls_of_no_rows_do_nothing():
     pool = _pool()
-    assert _status("msim_kv4_keep_async", ctypes.addressof(pool), None, None, None, 0, 0, 0, None, 4, None, None)[0] == 0
+    args = [ctypes.addressof(pool), None, None, None, 0, 0, 0, None, 4, None, None]
+    assert _status("msim_kv4_keep_async", *args)[0] == 0
     args = list(ROTARY)
     args[8] = 0
     assert _status("msim_rotary_async", *args)[0] == 0
