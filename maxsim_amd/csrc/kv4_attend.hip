@@ -45,13 +45,13 @@ namespace msim {
 namespace {
 
 constexpr int kTileKeys = kKeyAlign;
-constexpr int kWaves = 4;
+constexpr int kFewWaves = 4;  // of a workgroup, where a CU has several
 constexpr int kStages = 2;  // of a wave's ring: three or four, with as many or fewer waves, gained nothing
 
 // Rings of tiles, and in their place the join of the waves.
-constexpr int attend_lds(int dim, int cols) {
-  const int rings = kWaves * kStages * (32 * dim + 256);
-  const int join = 16 * cols * 4 * kWaves * (2 + dim + 4);
+constexpr int attend_lds(int dim, int cols, int waves) {
+  const int rings = waves * kStages * (32 * dim + 256);
+  const int join = 16 * cols * 4 * waves * (2 + dim + 4);
   return rings > join ? rings : join;
 }
 
@@ -141,7 +141,7 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 //
 // kMore: calls with sinks or parents. Keys are numbered as TileRange says then, else by
 // themselves.
-template <Kv4Type T, int kDim, int kCols, bool kMore>
+template <Kv4Type T, int kDim, int kCols, bool kMore, int kWaves>
 __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                             const Split& split, float* __restrict__ partial, const Cursor<kMore>& at,
                                             uint32_t from, uint32_t upto) {
@@ -149,7 +149,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   constexpr int kParts = T == kKv4F32 ? 2 : 1;      // of a query
   constexpr int kProbParts = T == kKv4F32 ? 3 : 2;  // of a probability times its value scale
   constexpr int kRows = 16 * kCols;
-  __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols)];
+  __shared__ __attribute__((aligned(16))) char s_raw[attend_lds(kDim, kCols, kWaves)];
   const int lane = lane_id(), col = lane % 16, g = lane / 16, wave = wave_uniform(threadIdx.x / kWave);
   const SeqWork& u = at.work;
   const uint32_t tile = at.tile;
@@ -163,10 +163,11 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
   const bool tree = kMore && args.parents != nullptr;
   const int start = u.length - u.rows;  // the first row's position
   const int first_word = start & -32, drafts = min(u.rows, kMostDrafts);
-  int parents[kMore ? kMostDrafts / (kWaves * kWave) : 1];
+  constexpr int kTurns = (kMostDrafts + kWaves * kWave - 1) / (kWaves * kWave);
+  int parents[kMore ? kTurns : 1];
   if (tree) {
 #pragma unroll
-    for (int i = 0; i < kMostDrafts / (kWaves * kWave); ++i) {
+    for (int i = 0; i < kTurns; ++i) {
       const int row = i * kWaves * kWave + (int)threadIdx.x;
       if (row < drafts) parents[i] = args.parents[u.first + row];
     }
@@ -236,7 +237,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
     const TilePages pages = tile_pages(pool, batch, seq, u.length, key);
     if (kMore && i == 0 && lines) {  // before the tiles, or their arrival is waited for
 #pragma unroll
-      for (int j = 0; j < kMostDrafts / (kWaves * kWave); ++j) {
+      for (int j = 0; j < kTurns; ++j) {
         const int row = j * kWaves * kWave + (int)threadIdx.x;
         if (row < drafts) s_parent[row] = parents[j];
       }
@@ -538,7 +539,7 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 }
 
 // Worker blockIdx.x's granules, item by item.
-template <Kv4Type T, int kDim, int kCols, bool kMore>
+template <Kv4Type T, int kDim, int kCols, bool kMore, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
                                                                    Split split, float* __restrict__ partial) {
   if (__builtin_expect(blockIdx.x >= split.workers, 0)) {
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
     const uint32_t from = at.own(split, granule - at.item_at), upto = at.own(split, stop);
     granule = at.item_at + stop;
     if (from == upto) continue;
-    attend_item<T, kDim, kCols, kMore>(pool, batch, args, split, partial, at, from, upto);
+    attend_item<T, kDim, kCols, kMore, kWaves>(pool, batch, args, split, partial, at, from, upto);
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + size - 1) - blockIdx.x) + 1;
     __syncthreads();
@@ -567,27 +568,29 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   note_unfinished(partial, split, kDim, at, parts);
 }
 
+constexpr int kJoinWaves = 4;
+
 // Joins the parts of split items. Of an item of up to kDirect parts each wave joins a row
 // by itself, and a workgroup has four rows of it; of more, each wave adds up every
-// kWaves-th part and the waves' sums are joined, and a workgroup has one row. Where many
+// kJoinWaves-th part and the waves' sums are joined, and a workgroup has one row. Where many
 // workgroups would find nothing to do, fewer count the pieces of work in the list of parts
 // and take them in turn (`counted`).
 template <Kv4Type T, int kDim>
-__global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split, uint32_t rows,
+__global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split, uint32_t rows,
                                                                  bool counted, float* __restrict__ partial) {
   constexpr int kRegs = (kDim + 63) / 64;
-  constexpr int kDirect = kWave / kWaves;
-  __shared__ float s_part[kWaves][kDim + 1];
-  __shared__ uint32_t s_end[kWaves], s_worker, s_piece;
+  constexpr int kDirect = kWave / kJoinWaves;
+  __shared__ float s_part[kJoinWaves][kDim + 1];
+  __shared__ uint32_t s_end[kJoinWaves], s_worker, s_piece;
   __shared__ int s_parts;
   const int wave = wave_uniform(threadIdx.x / kWave), lane = lane_id();
   const Unfinished* items = reinterpret_cast<const Unfinished*>(partial + partial_floats(split, kDim));
   const int* counts = reinterpret_cast<const int*>(items + split.workers);
   auto pieces = [&](int parts) -> uint32_t {
-    return parts == 0 ? 0 : (parts <= kDirect ? (rows + kWaves - 1) / kWaves : rows);
+    return parts == 0 ? 0 : (parts <= kDirect ? (rows + kJoinWaves - 1) / kJoinWaves : rows);
   };
   // A thread counts the pieces of kEach workers.
-  constexpr uint32_t kEach = kMostWorkers / (kWaves * kWave);
+  constexpr uint32_t kEach = kMostWorkers / (kJoinWaves * kWave);
   int have_parts[kEach] = {};
   uint32_t mine = 0, before = 0, all_pieces = 0;
   if (counted) {
@@ -602,7 +605,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
     __syncthreads();
     before = upto - mine;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
       if (w < wave) before += s_end[w];
       all_pieces += s_end[w];
     }
@@ -631,8 +634,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
     const int parts = min(counted ? wave_uniform(s_parts) : own_parts, (int)(split.workers - first));
     const Unfinished item = items[first];
     const bool direct = parts <= kDirect;
-    const int start = direct ? 0 : wave, stride = direct ? 1 : kWaves;
-    const uint32_t local = direct ? piece * kWaves + wave : piece;
+    const int start = direct ? 0 : wave, stride = direct ? 1 : kJoinWaves;
+    const uint32_t local = direct ? piece * kJoinWaves + wave : piece;
     const uint32_t r = (item.tile << split.tile_shift) + local;
     const int token = (int)(r / split.share), qh = item.head * split.share + (int)(r - token * split.share);
     if (counted) __syncthreads();  // the next piece may be written
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
       const float now = fmaxf(all, wave_reduce(ref, [](float a, float b) { return fmaxf(a, b); }));
       const float old = exp2_hw(all - now), alpha = exp2_hw(ref - now);
       all = now;
-      const float weighed = direct || lane % kWaves == wave ? share * alpha : 0.0f;
+      const float weighed = direct || lane % kJoinWaves == wave ? share * alpha : 0.0f;
       total = total * old + wave_reduce(weighed, [](float a, float b) { return a + b; });
 #pragma unroll
       for (int k = 0; k < kRegs; ++k) o[k] *= old;
@@ -683,7 +686,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_join_kernel(Kv4AttendArgs a
 #pragma unroll
       for (int k = 0; k < kRegs; ++k) o[k] = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < kJoinWaves; ++w) {
         total += s_part[w][kDim];
 #pragma unroll
         for (int k = 0; k < kRegs; ++k) o[k] += s_part[w][min(k * 64 + lane, kDim - 1)];
@@ -734,17 +737,25 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   int64_t whole = kShort;  // keys of a granule that is an item
   const bool more = args != nullptr && (args->sinks > 0 || parents);
   if (more && !prompt) {
-    // Of these calls, whose keys a window may count, items of up to 17 granules stay whole
-    // where there are 16 for each granule of one. 32 heads of 128 on 8, one token each of 64
-    // sequences, window 1,024: 24 us against 32 split, 2,048: 37 against 43; of 32 sequences 20
-    // against 24, and 29 against 28; of 8, 19 against 16; 8 tokens of 32: 27 against 35. At windows
-    // of 4,096 sequences of 100 to 4,200 keys took 54 us against 46.
+    // Of these calls, whose keys a window may count, items stay whole where there are many for
+    // their length. 32 heads of 128 on 8, one token of a sequence, by the window:
+    //   up to 512 keys always: of 4 sequences 11.6 us against 12.8 split, of 64 14.4 against 21;
+    //   a workgroup for each CU, with all the waves it holds, from 7 items for each granule of one:
+    //     1,024 keys of 8 sequences 16.5 against 15.6, of 16 16.5 against 18.2, of 32 17.5 against 23;
+    //     2,048 of 16 21.8 against 21.9, of 32 22.6 against 27.7; 4,096 of 32 35 against 41, but of
+    //     100 to 4,200 tokens 34.5 against 30; 8 tokens of 32, 2,048, 31 against 45;
+    //   more items than CUs from 16 on, the usual workgroups: 1,024 of 64 25 against 32, 2,048
+    //     38 against 42, 4,096 of 100 to 4,200 tokens 54 against 46.
     int64_t keys = longest;
     if (args->causal && !parents)
       keys = std::min(keys, (int64_t)args->window + (1 << s.tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
     const int64_t granules = (keys + kGranule - 1) / kGranule;
     const int64_t tiles = ((int64_t)batch.rows * s.share / std::max(1, batch.batch) + (1 << s.tile_shift) - 1) >> s.tile_shift;
-    s.one_launch = keys <= kShort || (granules <= 17 && tiles * batch.batch * pool.kv_heads >= 16 * granules);
+    const int64_t whole_items = tiles * batch.batch * pool.kv_heads;
+    const int per_simd = waves_per_simd(type, pool.dim, s.tile_shift == 5 ? 2 : 1);
+    s.whole_cu = keys > kShort && per_simd > 1 && whole_items <= num_cus && whole_items >= 7 * granules && granules <= 33;
+    if (s.whole_cu) s.workers = num_cus;
+    s.one_launch = keys <= kShort || s.whole_cu || (granules <= 17 && whole_items >= 16 * granules);
     while (whole < keys && s.one_launch) whole *= 2;
   }
   // An item costs its worker as much as four granules besides its own (queries, the waves' join):
@@ -767,18 +778,26 @@ hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const S
   // 12 heads 20.4 against 19.7).
   const bool counted = (uint64_t)split.workers * rows > 4096;
   const dim3 grid = counted ? dim3(num_cus * 4) : dim3(split.workers, rows);
-  kv4_join_kernel<T, kDim><<<grid, dim3(kWaves * kWave), 0, stream>>>(args, split, rows, counted, partial);
+  kv4_join_kernel<T, kDim><<<grid, dim3(kJoinWaves * kWave), 0, stream>>>(args, split, rows, counted, partial);
   return hipGetLastError();
 }
 
 template <Kv4Type T, int kDim, int kCols>
 hipError_t launch_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                          float* partial, hipStream_t stream) {
-  const dim3 grid(split.workers + loose_groups(batch)), block(kWaves * kWave);
-  if (args.sinks > 0 || args.parents != nullptr)
-    kv4_attend_kernel<T, kDim, kCols, true><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+  const dim3 grid(split.workers + loose_groups(batch));
+  auto run = [&](auto more, auto waves) {
+    constexpr int kWaves = decltype(waves)::value;
+    kv4_attend_kernel<T, kDim, kCols, decltype(more)::value, kWaves>
+        <<<grid, dim3(kWaves * kWave), 0, stream>>>(pool, batch, args, split, partial);
+  };
+  typedef std::integral_constant<int, kFewWaves> Few;
+  if (split.whole_cu)
+    run(std::true_type{}, std::integral_constant<int, 4 * waves_per_simd(T, kDim, kCols)>{});
+  else if (args.sinks > 0 || args.parents != nullptr)
+    run(std::true_type{}, Few{});
   else
-    kv4_attend_kernel<T, kDim, kCols, false><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+    run(std::false_type{}, Few{});
   return hipGetLastError();
 }
 
