@@ -38,6 +38,15 @@
 // 32 heads of 128 on 8: three tokens behind 100,000 to 131,072 keys (f16) take
 // 89 us, 4.3 TB/s, of which the main launch has 84 and the join 5; 32 behind 100 to
 // 8,000 (bfloat16) 43 to 44 us, 3.5 TB/s (38 and 5).
+//
+// Windows with sinks, trees of drafts: instances of their own (kMore), so that the other
+// calls keep their registers. The keys between the sinks and the window are left out of the
+// tiles' count. A row of a tree sees, of its sequence's own rows, those whose bits are set in
+// its line: a walk over the parents makes it, in LDS, while the first tiles come; a tile of
+// 32 keys is a word of it. The walk and its barriers cost 1.5 us at 8 drafts behind 700 keys (16.3 us
+// against 14.7 for a causal call). 32 tokens, window 1,024 and 4 sinks 17.6 us (2.1 TB/s of the keys
+// they see); three times three, window 16,384 and 300 sinks, pages of 16, 29.5 us; 7 x 27 drafts
+// behind 133 to 3,001 keys, 12 heads of 64, single precision 23 us.
 #include "kv4_split.hpp"
 
 namespace msim {

@@ -11,6 +11,9 @@
 //
 // Bytes bound it: every element is read and written once.  A lane has one group of
 // pairs and meets it in every head of a row, so that its angles are computed once.
+// 9,216 rows of 32 + 8 heads of 128 in bfloat16, 189 MB: 34 us over and over, 42 with other inputs
+// each time (4.5 TB/s).  16 rows: 4.4 us.  Loads of the first heads before the angles took
+// 114 registers, and 44 us.
 #include "rotary.hpp"
 
 namespace msim {
@@ -175,6 +178,7 @@ hipError_t launch_type(const RotaryPlan& plan, const RotaryRows rows[2], int64_t
   const int turning = (plan.pairs + kGroup - 1) / kGroup;
   const int lanes = turning + (plan.dim - 2 * plan.pairs + 2 * kGroup - 1) / (2 * kGroup);
   const int heads = rows[0].heads + rows[1].heads, at_once = kWave / lanes;
+  // Waves for a row, while they are fewer than the CUs' 16 each.
   int split = 1;
   while (split * at_once < heads && num_rows * split < 4096) split *= 2;
   const int64_t groups = (num_rows * split + kWavesPerGroup - 1) / kWavesPerGroup;
