@@ -474,7 +474,8 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& p = tensor(a[3], "positions");
   const int64_t rows = q.size(0);
   TORCH_CHECK_VALUE(p.scalar_type() == at::kInt && p.device() == device &&
-                        (p.dim() == 2 ? p.size(0) == r.num_axes : p.dim() == 1 && r.num_axes == 1) && p.size(-1) == rows,
+                        (p.dim() == 2 ? p.size(0) == r.num_axes : p.dim() == 1 && r.num_axes == 1) &&
+                        p.size(-1) == rows,
                     "positions must be an int32 tensor of shape ", r.num_axes == 1 ? "[rows] or " : "", "[", r.num_axes,
                     ", rows] on ", device);
   TORCH_CHECK_VALUE(rows <= 1 || p.stride(-1) == 1, "positions must be dense in their last dimension");

@@ -622,7 +622,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
   // Without counting, workgroup (i, y) has the pieces y, y + gridDim.y, ... of worker i.
   const int own_parts = counted ? 0 : counts[blockIdx.x];
   const uint32_t step = counted ? gridDim.x : gridDim.y;
-  for (uint32_t work = counted ? blockIdx.x : blockIdx.y; work < (counted ? all_pieces : pieces(own_parts)); work += step) {
+  if (!counted) all_pieces = pieces(own_parts);
+  for (uint32_t work = counted ? blockIdx.x : blockIdx.y; work < all_pieces; work += step) {
     if (counted && work >= before && work < before + mine) {
       uint32_t piece = work - before;
       bool found = false;
@@ -639,7 +640,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
       }
     }
     if (counted) __syncthreads();
-    const uint32_t first = counted ? wave_uniform(s_worker) : blockIdx.x, piece = counted ? wave_uniform(s_piece) : work;
+    const uint32_t first = counted ? wave_uniform(s_worker) : blockIdx.x;
+    const uint32_t piece = counted ? wave_uniform(s_piece) : work;
     const int parts = min(counted ? wave_uniform(s_parts) : own_parts, (int)(split.workers - first));
     const Unfinished item = items[first];
     const bool direct = parts <= kDirect;
@@ -759,10 +761,11 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     if (args->causal && !parents)
       keys = std::min(keys, (int64_t)args->window + (1 << s.tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
     const int64_t granules = (keys + kGranule - 1) / kGranule;
-    const int64_t tiles = ((int64_t)batch.rows * s.share / std::max(1, batch.batch) + (1 << s.tile_shift) - 1) >> s.tile_shift;
-    const int64_t whole_items = tiles * batch.batch * pool.kv_heads;
+    const int64_t each = (int64_t)batch.rows * s.share / std::max(1, batch.batch);
+    const int64_t whole_items = ((each + (1 << s.tile_shift) - 1) >> s.tile_shift) * batch.batch * pool.kv_heads;
     const int per_simd = waves_per_simd(type, pool.dim, s.tile_shift == 5 ? 2 : 1);
-    s.whole_cu = keys > kShort && per_simd > 1 && whole_items <= num_cus && whole_items >= 7 * granules && granules <= 33;
+    s.whole_cu = keys > kShort && granules <= 33 && per_simd > 1 && whole_items <= num_cus &&
+                 whole_items >= 7 * granules;
     if (s.whole_cu) s.workers = num_cus;
     s.one_launch = keys <= kShort || s.whole_cu || (granules <= 17 && whole_items >= 16 * granules);
     while (whole < keys && s.one_launch) whole *= 2;
@@ -778,8 +781,8 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
 }
 
 template <Kv4Type T, int kDim>
-hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial, int num_cus,
-                       hipStream_t stream) {
+hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial,
+                       int num_cus, hipStream_t stream) {
   // Without offsets a tile has as many rows as heads share a key/value head.
   const uint32_t rows = std::min(1u << split.tile_shift, batch.offsets == nullptr ? split.share : UINT32_MAX);
   // Up to 4,096 workgroups, where most have nothing to do, cost less than the counting
@@ -845,7 +848,8 @@ size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int head
     for (bool parents : {false, true}) {
       const Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
       if (s.one_launch) continue;
-      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) + s.workers * (sizeof(Unfinished) + sizeof(int)));
+      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) +
+                                  s.workers * (sizeof(Unfinished) + sizeof(int)));
     }
   return bytes;
 }

@@ -274,7 +274,8 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
     const v8h* keys = reinterpret_cast<const v8h*>(now) + lane;
     const v8b* values = reinterpret_cast<const v8b*>(now + B::kKeyBytes) + lane;
     // The 32-key steps that this wave's rows see something of.
-    const int step0 = max(0, (kMore && key_of(key0) < args.sinks ? 0 : any_low) - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
+    const int from_key = kMore && key_of(key0) < args.sinks ? 0 : any_low;
+    const int step0 = max(0, from_key - key0) / 32, step1 = min(kKeys, any_high - key0 + 31) / 32;
 #pragma unroll 1
     for (int st = step0; st < step1; ++st) {
       const int first = key_of(key0 + 32 * st);
@@ -455,9 +456,15 @@ hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArg
                   float* partial, hipStream_t stream) {
   const dim3 grid(split.workers + loose_groups(batch)), block(kPromptWaves * kWave);
   switch (pool.dim) {
-    case 64: kv4_prompt_kernel<T, 64, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 96: kv4_prompt_kernel<T, 96, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
-    case 128: kv4_prompt_kernel<T, 128, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial); break;
+    case 64:
+      kv4_prompt_kernel<T, 64, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+      break;
+    case 96:
+      kv4_prompt_kernel<T, 96, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+      break;
+    case 128:
+      kv4_prompt_kernel<T, 128, kMore, kTree><<<grid, block, 0, stream>>>(pool, batch, args, split, partial);
+      break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

@@ -27,7 +27,7 @@ namespace msim {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kFewRows = 4096;
+constexpr int kFewRows = 4096;  // of 64 sequences: 7.9 us in one launch, 8.7 for 8,192 in two
 constexpr uint32_t kNoCap = ~0u;
 
 // Inclusive scans of N sums over the workgroup's threads, each kept at its cap at most;
@@ -136,8 +136,8 @@ __global__ __launch_bounds__(kThreads) void pages_update_kernel(PagesState st, P
   // Scans of the first sequences: pages that come back, rows and pages asked for.
   const int had = min(max(*st.free_count, 0), st.num_pages);
   const Sequence head = sequence_of(st, up, tid);
-  const Scans<3> first({(uint32_t)head.back, (uint32_t)min(head.fresh, (int64_t)cap), (uint32_t)need_of(head, head.fresh)},
-                       {kNoCap, cap, kNoCap}, s_three);
+  const uint32_t head_rows = (uint32_t)min(head.fresh, (int64_t)cap), head_need = (uint32_t)need_of(head, head.fresh);
+  const Scans<3> first({(uint32_t)head.back, head_rows, head_need}, {kNoCap, cap, kNoCap}, s_three);
 
   // What comes back: never past the stack, whatever the lengths and the count were set to.
   uint32_t all_back = first.all[0];

@@ -178,9 +178,10 @@ hipError_t launch_type(const RotaryPlan& plan, const RotaryRows rows[2], int64_t
   const int turning = (plan.pairs + kGroup - 1) / kGroup;
   const int lanes = turning + (plan.dim - 2 * plan.pairs + 2 * kGroup - 1) / (2 * kGroup);
   const int heads = rows[0].heads + rows[1].heads, at_once = kWave / lanes;
-  // Waves for a row, while they are fewer than the CUs' 16 each.
+  // Waves for a row, while they are fewer than 1,024: more compute angles that one would
+  // share (512 rows of 32 + 8 heads 5.6 us, 6.1 with one for each, 8.0 up to 4,096 waves).
   int split = 1;
-  while (split * at_once < heads && num_rows * split < 4096) split *= 2;
+  while (split * at_once < heads && num_rows * split < 1024) split *= 2;
   const int64_t groups = (num_rows * split + kWavesPerGroup - 1) / kWavesPerGroup;
   const dim3 grid((unsigned)groups), block(kWavesPerGroup * kWave);
   auto run = [&](auto adjacent, auto w) {

@@ -90,5 +90,7 @@ class CachePages:
                 rows = self.batch * new
             new = torch.full((self.batch,), min(new, 2**31 - 1), dtype=torch.int32, device=self.device)
         if rows is None:
+            if new is not None and not hasattr(new, "clamp"):
+                raise ValueError("new must be a tensor or a number")
             rows = 0 if new is None else int(new.clamp(min=0).sum())
         return self._calls.update(self._handle, new, lengths, rows)

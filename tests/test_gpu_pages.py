@@ -186,7 +186,7 @@ def test_refusals(gpu):
             CachePages(*args, **kw)
     pages = CachePages(8, 3, 4, page_size=16)
     three = torch.ones(3, dtype=torch.int32, device="cuda")
-    for new, kw in ((three.long(), {"rows": 3}), (three[:2], {"rows": 2}), (three.cpu(), {"rows": 3}), (-1, {}),
+    for new, kw in (([1, 1, 1], {}), ([1, 1, 1], {"rows": 3}), (three.long(), {"rows": 3}), (three[:2], {"rows": 2}), (three.cpu(), {"rows": 3}), (-1, {}),
                     (three, {"rows": -1}), (three, {"lengths": three.long(), "rows": 3}),
                     (three, {"lengths": three[:1], "rows": 3}), (three.repeat(2)[::2], {"rows": 3})):
         with pytest.raises(ValueError):
