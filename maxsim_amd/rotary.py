@@ -6,13 +6,20 @@ column, each of which turns its own part of a head's dims.
 from __future__ import annotations
 
 import math
-from fractions import Fraction
 
 from maxsim_amd import _native
 from maxsim_amd.kvcache import _cuda_device
 
 
-_TURN = 2 * Fraction("3.14159265358979323846264338327950288419716939937511")
+# A turn, 2 pi, over 10^-49.
+_TURN = 2 * 31415926535897932384626433832795028841971693993751
+
+
+def _fixed_turns(frequency: float) -> int:
+    """Turns per position, in 2^-64, whole turns dropped: the exact quotient rounded once."""
+    numerator, denominator = frequency.as_integer_ratio()
+    numerator, denominator = numerator * 10**49 << 64, denominator * _TURN
+    return (2 * numerator + denominator) // (2 * denominator) % 2**64
 
 
 class Rotary:
@@ -55,8 +62,7 @@ class Rotary:
         self.device = _cuda_device(device)
         self.head_dim, self.rotary_dim = head_dim, rotary_dim
         self.num_axes, self.adjacent = max(axes) + 1, bool(adjacent)
-        # Turns per position, in 2^-64, whole turns dropped (as two's complement numbers).
-        turns = [round(Fraction(f) / _TURN * 2**64) % 2**64 for f in frequencies]
+        turns = [_fixed_turns(f) for f in frequencies]  # kept as two's complement numbers
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64,
                                    device=self.device)
         self._axes = torch.tensor(axes, dtype=torch.int32, device=self.device)
