@@ -102,12 +102,12 @@ __device__ __forceinline__ TileRange tile_range(const Kv4AttendArgs& args, const
   return r;
 }
 
+// What tile `tile` of a sequence is dealt out as, for all heads; 0 past the last.
 template <bool kMore>
-__device__ __forceinline__ uint32_t seq_granules(const Kv4Pool& pool, const Kv4AttendArgs& args, const Split& split,
-                                                 const SeqWork& w) {
-  uint32_t sum = 0;
-  for (uint32_t t = 0; t < w.tiles; ++t) sum += tile_range<kMore>(args, split, w, t).granules + split.lead;
-  return sum * pool.kv_heads;
+__device__ __forceinline__ uint32_t tile_share(const Kv4Pool& pool, const Kv4AttendArgs& args, const Split& split,
+                                               const SeqWork& w, uint32_t tile) {
+  if (tile >= w.tiles) return 0;
+  return (tile_range<kMore>(args, split, w, tile).granules + split.lead) * pool.kv_heads;
 }
 
 // `total` granules among `workers`: the first `extra` have one more.
@@ -142,13 +142,32 @@ struct Cursor {
     tile = 0;
     range = tile_range<kMore>(args, split, work, 0);
   }
-  // To the item that holds `granule`; false past the last (offsets out of order).
+  // To the item that holds `granule`; false past the last (offsets out of order).  By a wave
+  // together: of a sequence's tiles it looks through 64 at a time (2 x 40 tokens, 20 tiles of 16
+  // rows: one after another they cost 1 us more).
   __device__ __forceinline__ bool seek(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                        const Split& split, uint32_t granule) {
-    while (tile >= work.tiles || granule - before >= (range.granules + split.lead) * pool.kv_heads) {
-      if (tile < work.tiles) before += (range.granules + split.lead) * pool.kv_heads;
-      if (tile + 1 < work.tiles) {
-        range = tile_range<kMore>(args, split, work, ++tile);
+    for (int hops = 0;; ++hops) {
+      if (tile < work.tiles) {
+        const uint32_t size = (range.granules + split.lead) * pool.kv_heads;
+        if (granule - before < size) break;
+        before += size;
+        ++tile;
+      }
+      while (hops > 0 && tile < work.tiles) {
+        const uint32_t mine = tile_share<kMore>(pool, args, split, work, tile + lane_id()), upto = wave_scan(mine);
+        const uint64_t beyond = __ballot(granule - before < upto);
+        if (beyond != 0) {
+          const int at = __builtin_ctzll(beyond);
+          before += __builtin_amdgcn_readlane(upto - mine, at);
+          tile += at;
+          break;
+        }
+        before += __builtin_amdgcn_readlane(upto, kWave - 1);
+        tile = min(tile + kWave, work.tiles);
+      }
+      if (tile < work.tiles) {
+        range = tile_range<kMore>(args, split, work, tile);
       } else {
         if (++seq >= batch.batch) return false;
         enter(args, split, seq_work(pool, batch, split, seq), 0);
@@ -170,32 +189,40 @@ template <bool kMore>
 __device__ __forceinline__ bool find_work(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args,
                                           const Split& split, uint32_t worker, Cursor<kMore>& cursor, Deal& deal) {
   const int lane = lane_id();
+  // Where there are few sequences, 2^shift lanes share the tiles of each (2 x 2,048 fp32 tokens,
+  // window 1,024: 265 us for 382 with a lane each).
+  const int shift = batch.batch <= 1 ? 6 : max(0, __builtin_clz(batch.batch - 1) - 26);
+  const int each = kWave >> shift, stripes = 1 << shift, stripe = lane & (stripes - 1);
   auto work_of = [&](int b) -> SeqWork {
     return b < batch.batch ? seq_work(pool, batch, split, b) : SeqWork{0, 0, 0, 0};
   };
-  auto granules = [&](const SeqWork& w) -> uint32_t { return seq_granules<kMore>(pool, args, split, w); };
-  const SeqWork head_work = work_of(lane);
+  auto granules = [&](const SeqWork& w) -> uint32_t {
+    uint32_t sum = 0;
+    for (uint32_t t = stripe; t < w.tiles; t += stripes) sum += tile_share<kMore>(pool, args, split, w, t);
+    return sum;
+  };
+  const SeqWork head_work = work_of(lane >> shift);
   const uint32_t head = granules(head_work);
   uint32_t total = head;
-  for (int b0 = kWave; b0 < batch.batch; b0 += kWave) total += granules(work_of(b0 + lane));
+  for (int b0 = each; b0 < batch.batch; b0 += each) total += granules(work_of(b0 + (lane >> shift)));
   const uint32_t head_scan = wave_scan(head);
-  deal.total = batch.batch <= kWave ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
-                                    : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
+  deal.total = batch.batch <= each ? __builtin_amdgcn_readlane(head_scan, kWave - 1)
+                                   : __builtin_amdgcn_readlane(wave_scan(total), kWave - 1);
   deal.workers = min(split.workers, max(max(1u, min(deal.total, split.few)), deal.total / 2));
   deal.each = deal.total / deal.workers;
   deal.extra = deal.total - deal.each * deal.workers;
   if (deal.total == 0 || worker >= deal.workers) return false;
   const uint32_t target = deal.begin(worker);
   uint32_t done = 0;
-  for (int b0 = 0; b0 < batch.batch; b0 += kWave) {
-    const SeqWork work = b0 == 0 ? head_work : work_of(b0 + lane);
+  for (int b0 = 0; b0 < batch.batch; b0 += each) {
+    const SeqWork work = b0 == 0 ? head_work : work_of(b0 + (lane >> shift));
     const uint32_t mine = b0 == 0 ? head : granules(work);
-    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine)), first = upto - mine;
-    const uint64_t here = __ballot(first <= target && target < upto);
-    if (here != 0) {
-      const int at = __builtin_ctzll(here);
-      cursor.seq = wave_uniform(b0 + at);
-      cursor.before = __builtin_amdgcn_readlane(first, at);
+    const uint32_t upto = done + (b0 == 0 ? head_scan : wave_scan(mine));
+    const uint64_t beyond = __ballot(target < upto);
+    if (beyond != 0) {
+      const int at = __builtin_ctzll(beyond) & -stripes;  // the sequence's first lane
+      cursor.seq = wave_uniform(b0 + (at >> shift));
+      cursor.before = __builtin_amdgcn_readlane(upto - mine, at);
       cursor.enter(args, split, work, at);
       return true;
     }
