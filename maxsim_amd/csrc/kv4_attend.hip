@@ -549,8 +549,8 @@ __device__ __forceinline__ void attend_item(const Kv4Pool& pool, const Kv4Batch&
 
 // Worker blockIdx.x's granules, item by item.
 template <Kv4Type T, int kDim, int kCols, bool kMore, int kWaves>
-__global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args,
-                                                                   Split split, float* __restrict__ partial) {
+__global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void kv4_attend_kernel(
+    Kv4Pool pool, Kv4Batch batch, Kv4AttendArgs args, Split split, float* __restrict__ partial) {
   if (__builtin_expect(blockIdx.x >= split.workers, 0)) {
     loose_rows<T, kDim>(batch, args, split);
     return;
@@ -743,7 +743,6 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   s.share = heads / pool.kv_heads;
   s.workers = std::min(s.workers, kMostWorkers);
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
-  const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
   s.one_launch = longest <= kShort;
   int64_t whole = kShort;  // keys of a granule that is an item
   const bool more = args != nullptr && (args->sinks > 0 || parents);
@@ -751,22 +750,37 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     // Of these calls, whose keys a window may count, items stay whole where there are many for
     // their length. 32 heads of 128 on 8, one token of a sequence, by the window:
     //   up to 512 keys always: of 4 sequences 11.6 us against 12.8 split, of 64 14.4 against 21;
-    //   a workgroup for each CU, with all the waves it holds, from 7 items for each granule of one:
+    //   a workgroup for each CU, with all the waves it holds, from 7 items for each granule of one,
+    //   and 10 where the longest sequence alone bounds them, others being shorter:
     //     1,024 keys of 8 sequences 16.5 against 15.6, of 16 16.5 against 18.2, of 32 17.5 against 23;
     //     2,048 of 16 21.8 against 21.9, of 32 22.6 against 27.7; 4,096 of 32 35 against 41, but of
     //     100 to 4,200 tokens 34.5 against 30; 8 tokens of 32, 2,048, 31 against 45;
+    //   their tiles have 16 rows if that gives no more items than CUs, for the more items and waves
+    //     (32 rows in brackets): 8 drafts of 8 sequences, 1,400 keys, 19.2 (23.6), of 16 at 500 to
+    //     2,000 23.0 (29.7), 64 of one at 1,400 20.4 (24.8); 16 tokens of 8, 2,048, 23.3 (29.6);
+    //     8 drafts of 16 behind 100 to 2,500, 3,000 and 3,500 keys, 12.8, 10.7 and 9.1 items for a
+    //     granule, 25.4, 29.3 and 31.7 against 28.5, 29.5 and 30.6 split;
     //   more items than CUs from 16 on, the usual workgroups: 1,024 of 64 25 against 32, 2,048
     //     38 against 42, 4,096 of 100 to 4,200 tokens 54 against 46.
-    int64_t keys = longest;
-    if (args->causal && !parents)
-      keys = std::min(keys, (int64_t)args->window + (1 << s.tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
-    const int64_t granules = (keys + kGranule - 1) / kGranule;
-    const int64_t each = (int64_t)batch.rows * s.share / std::max(1, batch.batch);
-    const int64_t whole_items = ((each + (1 << s.tile_shift) - 1) >> s.tile_shift) * batch.batch * pool.kv_heads;
-    const int per_simd = waves_per_simd(type, pool.dim, s.tile_shift == 5 ? 2 : 1);
-    s.whole_cu = keys > kShort && granules <= 33 && per_simd > 1 && whole_items <= num_cus &&
-                 whole_items >= 7 * granules;
-    if (s.whole_cu) s.workers = num_cus;
+    int64_t keys = 0, granules = 0, whole_items = 0;
+    auto for_whole_cus = [&](uint32_t tile_shift) {
+      keys = longest;
+      if (args->causal && !parents)
+        keys = std::min(keys, (int64_t)args->window + (1 << tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
+      granules = (keys + kGranule - 1) / kGranule;
+      const int64_t each = (int64_t)batch.rows * s.share / std::max(1, batch.batch);
+      whole_items = ((each + (1 << tile_shift) - 1) >> tile_shift) * batch.batch * pool.kv_heads;
+      return keys > kShort && granules <= 33 && waves_per_simd(type, pool.dim, tile_shift == 5 ? 2 : 1) > 1 &&
+             whole_items <= num_cus && whole_items >= (keys == longest ? 10 : 7) * granules;
+    };
+    s.whole_cu = for_whole_cus(4);
+    if (s.whole_cu) {
+      s.tile_shift = 4;
+      s.workers = num_cus;
+    } else if (s.tile_shift == 5) {
+      s.whole_cu = for_whole_cus(5);
+      if (s.whole_cu) s.workers = num_cus;
+    }
     s.one_launch = keys <= kShort || s.whole_cu || (granules <= 17 && whole_items >= 16 * granules);
     while (whole < keys && s.one_launch) whole *= 2;
   }
@@ -776,6 +790,7 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   if (more && !s.one_launch) s.lead = 4;
   if (s.one_launch) s.few = s.workers;
   s.granule_shift = __builtin_ctzll(s.one_launch ? whole : kGranule);
+  const int64_t items = (((int64_t)batch.rows * s.share >> s.tile_shift) + batch.batch) * pool.kv_heads;
   while (items * ((longest >> s.granule_shift) + 1 + s.lead) >= (int64_t)1 << 31) ++s.granule_shift;
   return s;
 }
@@ -786,8 +801,8 @@ hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const S
   // Without offsets a tile has as many rows as heads share a key/value head.
   const uint32_t rows = std::min(1u << split.tile_shift, batch.offsets == nullptr ? split.share : UINT32_MAX);
   // Up to 4,096 workgroups, where most have nothing to do, cost less than the counting
-  // (3,072 for 32 tokens behind 100 to 8,000 keys: 43.3 us against 44.7; 12,288 for 7 x 5 tokens of
-  // 12 heads 20.4 against 19.7).
+  // (32 tokens behind 100 to 8,000 keys: 43.3 us against 44.7; with three times as many, 7 x 5 tokens
+  // of 12 heads, 20.4 against 19.7).
   const bool counted = (uint64_t)split.workers * rows > 4096;
   const dim3 grid = counted ? dim3(num_cus * 4) : dim3(split.workers, rows);
   kv4_join_kernel<T, kDim><<<grid, dim3(kJoinWaves * kWave), 0, stream>>>(args, split, rows, counted, partial);

@@ -363,6 +363,25 @@ def test_many_sequences_with_trees(gpu, kind, share, new):
         _check(cache, batch, q, got, lse, parents=parents, **kw)
 
 
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("lengths,new", [([700], 64), ([0, 1, 900, 513, 130, 31, 800, 24], 24), ([1040, 1023], 39)])
+def test_few_sequences_in_small_tiles(gpu, kind, dim, lengths, new):
+    """Whole items of 16 rows, several for a sequence, some of them ragged or empty."""
+    cache = Int4KVCache(sum(-(-n // 16) for n in lengths), 4, dim, page_size=16)
+    _fill(cache, 8)
+    rows = [min(n, new) for n in lengths]
+    batch = Batch(cache, lengths, rows, seed=3, spare=150)
+    parents = _tree(rows, 5)
+    q = _queries(batch.rows, 16, dim, kind, 3)
+    for kw in ({}, {"window": 60, "sinks": 33}):
+        got, lse = cache.attend(q, *batch.args, parents=parents.cuda(), return_lse=True, **kw)
+        _check(cache, batch, q, got, lse, parents=parents, **kw)
+    for window, sinks in ((600, 4), (513, 100)):
+        got, lse = cache.attend(q, *batch.args, window=window, sinks=sinks, return_lse=True)
+        _check(cache, batch, q, got, lse, window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("lo,hi,new", [(1, 2500, 9), (1, 700, 33), (2000, 6000, 2)])
 def test_ragged_split_items(gpu, lo, hi, new):
     """Short and long sequences dealt out together."""
