@@ -725,6 +725,11 @@ int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
 }
 
+// Workgroups that the CUs hold at once.
+uint32_t workers_for(Kv4Type type, int dim, int columns, int num_cus) {
+  return std::min<uint32_t>(num_cus * waves_per_simd(type, dim, columns), kMostWorkers);
+}
+
 // `args` nullptr: any call with or without parents, of those that need a workspace.
 Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents,
                 const Kv4AttendArgs* args, int num_cus) {
@@ -735,13 +740,12 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   } else {
     const int columns = columns_for(pool, batch, heads);
     s.tile_shift = columns == 2 ? 5 : 4;
-    s.workers = num_cus * waves_per_simd(type, pool.dim, columns);
+    s.workers = workers_for(type, pool.dim, columns, num_cus);
     // A granule each is the shortest way while every CU has one workgroup (one token
     // behind 1,000 keys: 12.2 us against 13.2).
     s.few = num_cus;
   }
   s.share = heads / pool.kv_heads;
-  s.workers = std::min(s.workers, kMostWorkers);
   const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
   s.one_launch = longest <= kShort;
   int64_t whole = kShort;  // keys of a granule that is an item
@@ -760,27 +764,31 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     //     2,000 23.0 (29.7), 64 of one at 1,400 20.4 (24.8); 16 tokens of 8, 2,048, 23.3 (29.6);
     //     8 drafts of 16 behind 100 to 2,500, 3,000 and 3,500 keys, 12.8, 10.7 and 9.1 items for a
     //     granule, 25.4, 29.3 and 31.7 against 28.5, 29.5 and 30.6 split;
+    //   16 rows too where every granule, or short item, then has a workgroup at once: 8 drafts of one
+    //     sequence, 100 keys, 10.1 (12.3), 400 13.6 (17.2), 700 14.6 (16.7), 3,500 16.6 (17.3), of four
+    //     at 1,400 18.6 (19.6);
     //   more items than CUs from 16 on, the usual workgroups: 1,024 of 64 25 against 32, 2,048
     //     38 against 42, 4,096 of 100 to 4,200 tokens 54 against 46.
     int64_t keys = 0, granules = 0, whole_items = 0;
-    auto for_whole_cus = [&](uint32_t tile_shift) {
+    auto count = [&](uint32_t tile_shift) {
       keys = longest;
       if (args->causal && !parents)
         keys = std::min(keys, (int64_t)args->window + (1 << tile_shift) / s.share + 2 + args->sinks + 2 * kKeyAlign);
       granules = (keys + kGranule - 1) / kGranule;
       const int64_t each = (int64_t)batch.rows * s.share / std::max(1, batch.batch);
       whole_items = ((each + (1 << tile_shift) - 1) >> tile_shift) * batch.batch * pool.kv_heads;
-      return keys > kShort && granules <= 33 && waves_per_simd(type, pool.dim, tile_shift == 5 ? 2 : 1) > 1 &&
-             whole_items <= num_cus && whole_items >= (keys == longest ? 10 : 7) * granules;
+      s.whole_cu = keys > kShort && granules <= 33 && waves_per_simd(type, pool.dim, tile_shift == 5 ? 2 : 1) > 1 &&
+                   whole_items <= num_cus && whole_items >= (keys == longest ? 10 : 7) * granules;
+      return s.whole_cu;
     };
-    s.whole_cu = for_whole_cus(4);
-    if (s.whole_cu) {
+    const int at_once = workers_for(type, pool.dim, 1, num_cus);
+    if (count(4) || (s.tile_shift == 5 && whole_items * (keys <= kShort ? 1 : granules) <= at_once)) {
       s.tile_shift = 4;
-      s.workers = num_cus;
+      s.workers = at_once;
     } else if (s.tile_shift == 5) {
-      s.whole_cu = for_whole_cus(5);
-      if (s.whole_cu) s.workers = num_cus;
+      count(5);
     }
+    if (s.whole_cu) s.workers = num_cus;
     s.one_launch = keys <= kShort || s.whole_cu || (granules <= 17 && whole_items >= 16 * granules);
     while (whole < keys && s.one_launch) whole *= 2;
   }
@@ -859,12 +867,19 @@ hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
 
 size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
   size_t bytes = 0;
+  auto add = [&](const Split& s) {
+    bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) +
+                                s.workers * (sizeof(Unfinished) + sizeof(int)));
+  };
   for (Kv4Type type : {kKv4F32, kKv4BF16})  // f16 splits as bfloat16
     for (bool parents : {false, true}) {
-      const Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
+      Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
       if (s.one_launch) continue;
-      bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) +
-                                  s.workers * (sizeof(Unfinished) + sizeof(int)));
+      add(s);
+      if (s.tile_shift != 5) continue;  // else a call may take tiles of 16 rows
+      s.tile_shift = 4;
+      s.workers = workers_for(type, pool.dim, 1, num_cus);
+      add(s);
     }
   return bytes;
 }
