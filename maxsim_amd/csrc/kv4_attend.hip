@@ -43,10 +43,11 @@
 // calls keep their registers. The keys between the sinks and the window are left out of the
 // tiles' count. A row of a tree sees, of its sequence's own rows, those whose bits are set in
 // its line: a walk over the parents makes it, in LDS, while the first tiles come; a tile of
-// 32 keys is a word of it. The walk and its barriers cost 1.5 us at 8 drafts behind 700 keys (16.3 us
-// against 14.7 for a causal call). 32 tokens, window 1,024 and 4 sinks 17.6 us (2.1 TB/s of the keys
-// they see); three times three, window 16,384 and 300 sinks, pages of 16, 29.5 us; 7 x 27 drafts
-// behind 133 to 3,001 keys, 12 heads of 64, single precision 23 us.
+// 32 keys is a word of it. The walk and its barriers cost 1.5 us at 8 drafts behind 700 keys (in tiles
+// of 32 rows 16.3 us against 14.7 for a causal call; of 16, as they have there, 14.4). 32 tokens,
+// window 1,024 and 4 sinks 17.6 us (2.1 TB/s of the keys they see); three times three, window
+// 16,384 and 300 sinks, pages of 16, 29.5 us; 7 x 27 drafts behind 133 to 3,001 keys, 12 heads
+// of 64, single precision 23 us.
 #include "kv4_split.hpp"
 
 namespace msim {
@@ -719,7 +720,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
 // Column tiles per workgroup: as many as a sequence's rows fill on average (one
 // for wide heads, whose outputs take the registers). At 8 sequences of 4,000 keys,
 // 32 heads of 128 on 8, two took 30.2 us for 5 tokens each and one 32.0; 32.7 and
-// 33.3 for 8; 38.2 and 41.7 for 16.
+// 33.3 for 8; 38.2 and 41.7 for 16.  With sinks or parents split_for takes one for
+// shorter work.
 int columns_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads) {
   const int64_t rows = (int64_t)batch.rows * (heads / pool.kv_heads) / std::max(1, batch.batch);
   return rows <= 16 || pool.dim > 128 ? 1 : 2;
