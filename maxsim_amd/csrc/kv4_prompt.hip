@@ -245,7 +245,9 @@ __device__ __forceinline__ void prompt_item(const Kv4Pool& pool, const Kv4Batch&
   int all_high = wave_reduce(see_high, [](int a, int b) { return min(a, b); });
   if (kTree) all_high = min(all_high, max(0, start));
   const int window_low = wave_reduce(sees ? see_low : INT_MAX, [](int a, int b) { return min(a, b); });
-  const int any_low = number_of(window_low);
+  // Where the sinks reach past the context, rows of a tree are first tokens by their depths,
+  // wherever their keys lie: no step is left out.
+  const int any_low = kTree && start < args.sinks ? 0 : number_of(window_low);
   const int any_high = number_of(wave_reduce(sees ? see_high : 0, [](int a, int b) { return max(a, b); }));
 
   float ref = kUnset, sum = 0.0f;
