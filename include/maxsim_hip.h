@@ -445,6 +445,12 @@ int msim_kv4_read_async(const msim_kv4_pool* pool, const int32_t* page_table, co
  * none, NULL will do). */
 int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
                               int64_t heads, uint64_t* bytes);
+/* Bytes that msim_kv4_attend_ex_async makes use of: the same without parents, others with
+ * them (parents != 0), up to four times as many.  A tree does with the lesser of both, and
+ * goes a slower way then where there are many rows behind long contexts; the two ways'
+ * results differ by their roundings. */
+int msim_kv4_attend_ex_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
+                                 int64_t heads, int parents, uint64_t* bytes);
 /* Attention of queries [rows, heads, dim] over the cache: head h reads key/value
  * head h / (heads / kv_heads).  A row at position p = length - rows + i sees keys
  * j < length with, if causal, j <= p; j > p - window (window 0: all); mask[row, j]

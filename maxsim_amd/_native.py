@@ -100,6 +100,7 @@ SIGNATURES: dict[str, list] = {
     "msim_kv4_read_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
                             c_int, c_vp],
     "msim_kv4_attend_workspace": [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp],
+    "msim_kv4_attend_ex_workspace": [c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp],
     "msim_kv4_attend_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_dbl,
                               c_int, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_u64, c_vp],
     "msim_kv4_attend_ex_async": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_dbl,
@@ -206,7 +207,7 @@ def tensor_calls():
         path = os.path.join(HERE, "_tensor_calls.so")
         why = f"cannot be loaded beside torch {torch.__version__} ({exc})" if os.path.exists(path) else "is not built"
         raise NativeLibraryMissing(f"{path} {why}; run `python -m maxsim_amd.build`") from exc
-    names = ("msim_last_error", "msim_kv4_append_async", "msim_kv4_read_async", "msim_kv4_attend_workspace",
+    names = ("msim_last_error", "msim_kv4_append_async", "msim_kv4_read_async", "msim_kv4_attend_ex_workspace",
              "msim_kv4_attend_ex_async", "msim_linear4_async", "msim_kv4_keep_async", "msim_pages_update_async",
              "msim_rotary_async")
     _tensor_calls.setup(*(ctypes.cast(getattr(lib, name), c_vp).value for name in names))

@@ -31,7 +31,7 @@ struct {
   const char* (*last_error)() = nullptr;
   decltype(&msim_kv4_append_async) append = nullptr;
   decltype(&msim_kv4_read_async) read = nullptr;
-  decltype(&msim_kv4_attend_workspace) attend_workspace = nullptr;
+  decltype(&msim_kv4_attend_ex_workspace) attend_workspace = nullptr;
   decltype(&msim_kv4_attend_ex_async) attend = nullptr;
   decltype(&msim_linear4_async) linear = nullptr;
   decltype(&msim_kv4_keep_async) keep = nullptr;
@@ -373,7 +373,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (want_lse) lse = allocate({rows, heads}, at::kFloat, c.device);
   const Launch launch(c.device);
   uint64_t need = 0;
-  check(abi.attend_workspace(&c.pool, b.batch, b.max_pages, rows, heads, &need));
+  check(abi.attend_workspace(&c.pool, b.batch, b.max_pages, rows, heads, parents != nullptr, &need));
   if (need > 0) work = allocate({(int64_t)need}, at::kByte, c.device);
   check(abi.attend(&c.pool, b.table, b.lengths, b.offsets, b.batch, b.max_pages, rows, q.const_data_ptr(), q.stride(0),
                    q.stride(1), heads, type_of(q.scalar_type()), scale, causal, integer(a[7]), mask, mask_stride,

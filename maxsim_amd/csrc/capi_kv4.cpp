@@ -1,6 +1,7 @@
 // capi_kv4.cpp -- C ABI of the 4-bit key/value cache (kv4_rows.hip,
 // kv4_attend.hip, kv4_keep.hip): argument checks and launches.  The pool, the batch and the
 // workspace are the caller's device memory.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -109,13 +110,18 @@ extern "C" int msim_kv4_read_async(const msim_kv4_pool* pool, const int32_t* pag
 
 extern "C" int msim_kv4_attend_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
                                          int64_t heads, uint64_t* bytes) {
+  return msim_kv4_attend_ex_workspace(pool, batch, max_pages, rows, heads, 0, bytes);
+}
+
+extern "C" int msim_kv4_attend_ex_workspace(const msim_kv4_pool* pool, int64_t batch, int64_t max_pages, int64_t rows,
+                                            int64_t heads, int parents, uint64_t* bytes) {
   return guarded([&] {
     if (bytes == nullptr) throw InvalidArgument("bytes must not be NULL");
     const Kv4Pool p = check_pool(pool);
     static const int32_t present = 0;  // only the sizes count here
     const Kv4Batch b = check_batch(p, &present, &present, &present, batch, max_pages, rows);
     check_heads(p, b, heads);
-    *bytes = kv4_attend_workspace(p, b, (int)heads, device_cu_count());
+    *bytes = kv4_attend_workspace(p, b, (int)heads, parents != 0, device_cu_count());
   });
 }
 
@@ -155,7 +161,8 @@ extern "C" int msim_kv4_attend_ex_async(const msim_kv4_pool* pool, const int32_t
     check_rows(q, t, "q");
     check_rows(out, t, "out");
     const int cus = device_cu_count();
-    const size_t need = kv4_attend_workspace(p, b, (int)heads, cus);
+    size_t need = kv4_attend_workspace(p, b, (int)heads, false, cus);
+    if (parents != nullptr) need = std::min(need, kv4_attend_workspace(p, b, (int)heads, true, cus));
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need))
       throw InvalidArgument("workspace is smaller than msim_kv4_attend_workspace asks for, or not 16-byte aligned");
     Kv4AttendArgs a{};
@@ -178,7 +185,7 @@ extern "C" int msim_kv4_attend_ex_async(const msim_kv4_pool* pool, const int32_t
     a.sinks = a.window == INT_MAX ? 0 : (int32_t)std::min<int64_t>(sinks, INT_MAX);
     a.parents = parents;
     a.scale_log2 = scale_log2;
-    check_hip(launch_kv4_attend(p, b, a, t, workspace, cus, as_stream(stream)), "launch cache attention kernels");
+    check_hip(launch_kv4_attend(p, b, a, t, workspace, workspace_bytes, cus, as_stream(stream)), "launch cache attention kernels");
   });
 }
 

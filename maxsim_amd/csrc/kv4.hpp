@@ -140,8 +140,9 @@ struct Kv4AttendArgs {
 // Rows of a sequence in a call with parents, at most: rows of a longer one see nothing.
 constexpr int kMostDrafts = 1024;
 
-size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus);
+// Bytes for a call of any type; one with parents does with the lesser of both.
+size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, bool parents, int num_cus);
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
-                             void* workspace, int num_cus, hipStream_t stream);
+                             void* workspace, size_t workspace_bytes, int num_cus, hipStream_t stream);
 
 }  // namespace msim

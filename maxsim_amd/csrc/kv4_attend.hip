@@ -732,11 +732,12 @@ uint32_t workers_for(Kv4Type type, int dim, int columns, int num_cus) {
   return std::min<uint32_t>(num_cus * waves_per_simd(type, dim, columns), kMostWorkers);
 }
 
-// `args` nullptr: any call with or without parents, of those that need a workspace.
+// `args` nullptr: any call with or without parents, of those that need a workspace. `prompts`
+// false: not by kv4_prompt.hip.
 Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents,
-                const Kv4AttendArgs* args, int num_cus) {
+                const Kv4AttendArgs* args, int num_cus, bool prompts = true) {
   Split s{};
-  const bool prompt = kv4_prompt_takes(pool, batch, heads, type, parents);
+  const bool prompt = prompts && kv4_prompt_takes(pool, batch, heads, type, parents);
   if (prompt) {
     s = kv4_prompt_split(num_cus);
   } else {
@@ -805,6 +806,11 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   return s;
 }
 
+// What a call of such a split leaves for the join.
+size_t split_bytes(const Split& s, int dim) {
+  return s.one_launch ? 0 : partial_floats(s, dim) * sizeof(float) + s.workers * (sizeof(Unfinished) + sizeof(int));
+}
+
 template <Kv4Type T, int kDim>
 hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial,
                        int num_cus, hipStream_t stream) {
@@ -842,7 +848,7 @@ template <Kv4Type T, int kDim>
 hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
                       float* partial, int num_cus, hipStream_t stream) {
   hipError_t e = hipErrorInvalidValue;
-  if (kv4_prompt_takes(pool, batch, args.heads, T, args.parents != nullptr))
+  if (split.prompt)
     e = launch_kv4_prompt(pool, batch, args, T, split, partial, stream);
   else if (kDim > 128 || split.tile_shift == 4)
     e = launch_attend<T, kDim, 1>(pool, batch, args, split, partial, stream);
@@ -867,29 +873,27 @@ hipError_t launch_type(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
 
 }  // namespace
 
-size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, int num_cus) {
+size_t kv4_attend_workspace(const Kv4Pool& pool, const Kv4Batch& batch, int heads, bool parents, int num_cus) {
   size_t bytes = 0;
-  auto add = [&](const Split& s) {
-    bytes = std::max(bytes, (size_t)partial_floats(s, pool.dim) * sizeof(float) +
-                                s.workers * (sizeof(Unfinished) + sizeof(int)));
-  };
-  for (Kv4Type type : {kKv4F32, kKv4BF16})  // f16 splits as bfloat16
-    for (bool parents : {false, true}) {
-      Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
-      if (s.one_launch) continue;
-      add(s);
-      if (s.tile_shift != 5) continue;  // else a call may take tiles of 16 rows
-      s.tile_shift = 4;
-      s.workers = workers_for(type, pool.dim, 1, num_cus);
-      add(s);
-    }
+  for (Kv4Type type : {kKv4F32, kKv4BF16}) {  // f16 splits as bfloat16
+    Split s = split_for(pool, batch, heads, type, parents, nullptr, num_cus);
+    bytes = std::max(bytes, split_bytes(s, pool.dim));
+    if (s.tile_shift != 5) continue;  // else a call may take tiles of 16 rows
+    s.tile_shift = 4;
+    s.workers = workers_for(type, pool.dim, 1, num_cus);
+    bytes = std::max(bytes, split_bytes(s, pool.dim));
+  }
   return bytes;
 }
 
 hipError_t launch_kv4_attend(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
-                             void* workspace, int num_cus, hipStream_t stream) {
+                             void* workspace, size_t workspace_bytes, int num_cus, hipStream_t stream) {
   if (batch.rows <= 0) return hipSuccess;
-  const Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, &args, num_cus);
+  Split split = split_for(pool, batch, args.heads, type, args.parents != nullptr, &args, num_cus);
+  // Trees in tiles of 256 rows may leave larger partial results than other calls of their sizes,
+  // whose workspace suffices: with that alone their tiles are smaller.
+  if (split_bytes(split, pool.dim) > workspace_bytes)
+    split = split_for(pool, batch, args.heads, type, args.parents != nullptr, &args, num_cus, false);
   float* partial = static_cast<float*>(workspace);
   switch (type) {
     case kKv4F32: return launch_type<kKv4F32>(pool, batch, args, split, partial, num_cus, stream);

@@ -500,6 +500,7 @@ bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4
 
 Split kv4_prompt_split(int num_cus) {
   Split s{};
+  s.prompt = 1;
   s.tile_shift = __builtin_ctz(kPromptRows);
   s.workers = num_cus;  // LDS holds one workgroup per CU
   s.few = 0;

@@ -49,6 +49,7 @@ struct Split {
   uint32_t few;         // workers may have a single granule while there are no more of them
   uint32_t one_launch;  // no item is split
   uint32_t whole_cu;    // a workgroup has as many waves as a CU holds
+  uint32_t prompt;      // kv4_prompt.hip's kernel
   uint32_t lead;        // granules that an item is dealt out as, besides its own
 };
 
