@@ -737,7 +737,7 @@ uint32_t workers_for(Kv4Type type, int dim, int columns, int num_cus) {
 Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents,
                 const Kv4AttendArgs* args, int num_cus, bool prompts = true) {
   Split s{};
-  const bool prompt = prompts && kv4_prompt_takes(pool, batch, heads, type, parents);
+  const bool prompt = prompts && kv4_prompt_takes(pool, batch, heads, type, parents, num_cus);
   if (prompt) {
     s = kv4_prompt_split(num_cus);
   } else {

@@ -474,7 +474,7 @@ hipError_t launch(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArg
 
 }  // namespace
 
-bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents) {
+bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents, int num_cus) {
   // Two workgroups' rows per sequence and head on average, or one where the items
   // fill half the CUs: fewer leave CUs, or parts of them, without work. Heads of
   // 128, 32 on 8, this kernel against kv4_attend.hip's: 8 x 128 tokens behind 4,000
@@ -493,9 +493,9 @@ bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4
     const int64_t each = rows / std::max(1, batch.batch);
     const int64_t tiles = (each + kPromptRows - 1) / kPromptRows * batch.batch;
     const int64_t keys = (int64_t)batch.max_pages << pool.page_shift;
-    return rows * 8 >= tiles * kPromptRows * 7 && tiles * pool.kv_heads * keys >= 6 * kGranule * 256;
+    return rows * 8 >= tiles * kPromptRows * 7 && tiles * pool.kv_heads * keys >= 6 * kGranule * (int64_t)num_cus;
   }
-  return (rows >= 2 * whole || (rows >= whole && rows * pool.kv_heads >= 128 * kPromptRows));
+  return rows >= 2 * whole || (rows >= whole && 2 * rows * pool.kv_heads >= (int64_t)num_cus * kPromptRows);
 }
 
 Split kv4_prompt_split(int num_cus) {

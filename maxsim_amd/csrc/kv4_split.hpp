@@ -394,7 +394,7 @@ __device__ __forceinline__ void note_unfinished(float* partial, const Split& spl
 }
 
 // kv4_prompt.hip: many rows per sequence.
-bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents);
+bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type type, bool parents, int num_cus);
 Split kv4_prompt_split(int num_cus);
 hipError_t launch_kv4_prompt(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, Kv4Type type,
                              const Split& split, float* partial, hipStream_t stream);

@@ -4,6 +4,8 @@ import ctypes
 import pytest
 from test_operators_host import P, _pool, _status
 
+from maxsim_amd import _native
+
 
 def _bytes(call, pool, *sizes):
     need = ctypes.c_uint64(0)
@@ -45,3 +47,42 @@ def test_less_than_a_tree_needs(tokens, batch, rows, heads):
                 bytes_, None]
         got = _status("msim_kv4_attend_ex_async", ctypes.addressof(pool), *args)
         assert got[0] == 1 and "workspace" in got[1]
+
+
+class _Pool(ctypes.Structure):
+    """csrc/kv4.hpp's Kv4Pool."""
+
+    _fields_ = [("arrays", ctypes.c_void_p * 4), ("num_pages", ctypes.c_int32), ("page_shift", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class _Batch(ctypes.Structure):
+    """Its Kv4Batch."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("batch", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("rows", ctypes.c_int32)]
+
+
+def _slots(cus, batch, pages, rows, parents):
+    """Rows of partial results in the library's own answer for a device of `cus` CUs: 32 heads of 128 on
+    8, pages of 16."""
+    call = getattr(_native.load(), "_ZN4msim20kv4_attend_workspaceERKNS_7Kv4PoolERKNS_8Kv4BatchEibi")
+    call.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_bool, ctypes.c_int]
+    call.restype = ctypes.c_size_t
+    pool = _Pool((ctypes.c_void_p * 4)(), 4, 4, 8, 128)
+    sizes = _Batch(P, P, P, batch, pages, rows)
+    return call(ctypes.addressof(pool), ctypes.addressof(sizes), 32, parents, cus) // (130 * 4)
+
+
+@pytest.mark.parametrize("cus", [32, 64, 256, 304])
+def test_tiles_of_256_rows_by_the_number_of_cus(cus):
+    """A workgroup of them for each CU, in two slots; smaller tiles have less than half of that."""
+    large = 2 * 256 * cus
+    # Trees: 4 x 64 rows with six granules of 128 keys for each CU, and fewer.
+    pages = 6 * 128 * cus // (4 * 8) // 16
+    assert _slots(cus, 4, pages, 256, True) >= large
+    assert _slots(cus, 4, pages - 1, 256, True) < large // 2
+    # Other calls: one tile a sequence and head, for half the CUs, and for fewer.
+    assert _slots(cus, cus // 16, 1000, cus // 16 * 64, False) >= large
+    if cus > 32:
+        assert _slots(cus, cus // 32, 1000, cus // 32 * 64, False) < large // 2
