@@ -16,6 +16,8 @@ with the next step's call: ``pages.update(new, lengths=cache.keep(...), rows=row
 """
 from __future__ import annotations
 
+import numbers
+
 from maxsim_amd import _native
 from maxsim_amd.kvcache import _cuda_device
 
@@ -81,9 +83,10 @@ class CachePages:
         + place in the page; -1 behind the last.  ``rows`` is the capacity for them;
         without it a tensor's sum is fetched from the device.  Enqueued on the current
         stream; can be captured in a HIP graph."""
-        if isinstance(new, int):
+        if isinstance(new, numbers.Integral):
             import torch
 
+            new = int(new)
             if new < 0:
                 raise ValueError("new must not be negative")
             if rows is None:
