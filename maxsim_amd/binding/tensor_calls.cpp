@@ -18,7 +18,9 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <ATen/record_function.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -104,8 +106,11 @@ struct Launch {
   }
 };
 
-// Memory of a GPU: at::empty without the way through the dispatcher.
+// Memory of a GPU: at::empty, without the way through the dispatcher (0.6 us of a call) where
+// neither a dispatch mode nor a profiler looks on.
 at::Tensor allocate(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() || at::hasCallbacks())
+    return at::empty(sizes, at::TensorOptions().device(device).dtype(type));
   return at::detail::empty_cuda(sizes, type, device, std::nullopt);
 }
 
