@@ -566,10 +566,10 @@ __global__ __launch_bounds__(kWaves* kWave, waves_per_simd(T, kDim, kCols)) void
   const uint32_t last = deal.begin(blockIdx.x + 1);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
-    const uint32_t size = at.range.granules + split.lead, stop = min(size, last - at.item_at);
+    const uint32_t size = at.range.granules + lead_of<kMore>(split), stop = min(size, last - at.item_at);
     const uint32_t from = at.own(split, granule - at.item_at), upto = at.own(split, stop);
     granule = at.item_at + stop;
-    if (from == upto) continue;
+    if (kMore && from == upto) continue;
     attend_item<T, kDim, kCols, kMore, kWaves>(pool, batch, args, split, partial, at, from, upto);
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + size - 1) - blockIdx.x) + 1;
@@ -585,9 +585,9 @@ constexpr int kJoinWaves = 4;
 // kJoinWaves-th part and the waves' sums are joined, and a workgroup has one row. Where many
 // workgroups would find nothing to do, fewer count the pieces of work in the list of parts
 // and take them in turn (`counted`).
-template <Kv4Type T, int kDim>
+template <Kv4Type T, int kDim, bool kCounted>
 __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split, uint32_t rows,
-                                                                 bool counted, float* __restrict__ partial) {
+                                                                 float* __restrict__ partial) {
   constexpr int kRegs = (kDim + 63) / 64;
   constexpr int kDirect = kWave / kJoinWaves;
   __shared__ float s_part[kJoinWaves][kDim + 1];
@@ -603,7 +603,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
   constexpr uint32_t kEach = kMostWorkers / (kJoinWaves * kWave);
   int have_parts[kEach] = {};
   uint32_t mine = 0, before = 0, all_pieces = 0;
-  if (counted) {
+  if constexpr (kCounted) {
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
       const uint32_t worker = threadIdx.x * kEach + i;
@@ -621,11 +621,11 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
     }
   }
   // Without counting, workgroup (i, y) has the pieces y, y + gridDim.y, ... of worker i.
-  const int own_parts = counted ? 0 : counts[blockIdx.x];
-  const uint32_t step = counted ? gridDim.x : gridDim.y;
-  if (!counted) all_pieces = pieces(own_parts);
-  for (uint32_t work = counted ? blockIdx.x : blockIdx.y; work < all_pieces; work += step) {
-    if (counted && work >= before && work < before + mine) {
+  const int own_parts = kCounted ? 0 : counts[blockIdx.x];
+  const uint32_t step = kCounted ? gridDim.x : gridDim.y;
+  if (!kCounted) all_pieces = pieces(own_parts);
+  for (uint32_t work = kCounted ? blockIdx.x : blockIdx.y; work < all_pieces; work += step) {
+    if (kCounted && work >= before && work < before + mine) {
       uint32_t piece = work - before;
       bool found = false;
 #pragma unroll
@@ -640,17 +640,17 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendAr
         piece -= found ? 0 : n;
       }
     }
-    if (counted) __syncthreads();
-    const uint32_t first = counted ? wave_uniform(s_worker) : blockIdx.x;
-    const uint32_t piece = counted ? wave_uniform(s_piece) : work;
-    const int parts = min(counted ? wave_uniform(s_parts) : own_parts, (int)(split.workers - first));
+    if (kCounted) __syncthreads();
+    const uint32_t first = kCounted ? wave_uniform(s_worker) : blockIdx.x;
+    const uint32_t piece = kCounted ? wave_uniform(s_piece) : work;
+    const int parts = min(kCounted ? wave_uniform(s_parts) : own_parts, (int)(split.workers - first));
     const Unfinished item = items[first];
     const bool direct = parts <= kDirect;
     const int start = direct ? 0 : wave, stride = direct ? 1 : kJoinWaves;
     const uint32_t local = direct ? piece * kJoinWaves + wave : piece;
     const uint32_t r = (item.tile << split.tile_shift) + local;
     const int token = (int)(r / split.share), qh = item.head * split.share + (int)(r - token * split.share);
-    if (counted) __syncthreads();  // the next piece may be written
+    if (kCounted) __syncthreads();  // the next piece may be written
     // Without barriers in them for single waves: a row is a wave's, or all waves agree on it.
     if (local >= rows || token >= item.rows) continue;
     float all = kUnset, total = 0.0f, o[kRegs] = {};
@@ -812,16 +812,28 @@ size_t split_bytes(const Split& s, int dim) {
 }
 
 template <Kv4Type T, int kDim>
-hipError_t launch_join(const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split, float* partial,
-                       int num_cus, hipStream_t stream) {
+hipError_t launch_join(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4AttendArgs& args, const Split& split,
+                       float* partial, int num_cus, hipStream_t stream) {
   // Without offsets a tile has as many rows as heads share a key/value head.
   const uint32_t rows = std::min(1u << split.tile_shift, batch.offsets == nullptr ? split.share : UINT32_MAX);
-  // Up to 4,096 workgroups, where most have nothing to do, cost less than the counting
-  // (32 tokens behind 100 to 8,000 keys: 43.3 us against 44.7; with three times as many, 7 x 5 tokens
-  // of 12 heads, 20.4 against 19.7).
-  const bool counted = (uint64_t)split.workers * rows > 4096;
-  const dim3 grid = counted ? dim3(num_cus * 4) : dim3(split.workers, rows);
-  kv4_join_kernel<T, kDim><<<grid, dim3(kJoinWaves * kWave), 0, stream>>>(args, split, rows, counted, partial);
+  // A few workgroups for each worker, or four for each CU that count the pieces of work. Counting
+  // costs 0.7 us (768 workers with 1 row 10.5 us against 11.2, with 6 rows 10.4 against 11.1) and
+  // saves workgroups that would find nothing: 512 with 16 rows, 14 items, 18.1 us against 15.7; 512
+  // with 32, up to 128 items, 2.5 us; 256 with 32 each of 256, up to 128 items, 5. It saves none
+  // where there may be a piece for each (4 x 400 tokens behind 2,100, 32 heads of 128: 141 us, counted
+  // 151), and under a window, where fewer items than workers are short and all of them split, few
+  // (32 x 5 tokens, window 300: 28.3, counted 29.8). The workgroups of a single long item
+  // would all be on one XCD (8 heads of 256 on 1, single precision, 30,000 keys: 31.3, counted 20.0).
+  const uint32_t y = std::min(32u, rows);
+  const uint64_t groups = (uint64_t)split.workers * y;
+  const uint64_t items = (((uint64_t)batch.rows * split.share >> split.tile_shift) + batch.batch) * pool.kv_heads;
+  const uint64_t pieces = std::min<uint64_t>(items, split.workers) * ((rows + kJoinWaves - 1) / kJoinWaves);
+  const dim3 block(kJoinWaves * kWave);
+  const bool all_split = args.window != INT_MAX && items < split.workers;
+  if ((groups > 6144 && pieces < (all_split ? groups / 12 : groups)) || items < 4)
+    kv4_join_kernel<T, kDim, true><<<dim3(num_cus * 4), block, 0, stream>>>(args, split, rows, partial);
+  else
+    kv4_join_kernel<T, kDim, false><<<dim3(split.workers, y), block, 0, stream>>>(args, split, rows, partial);
   return hipGetLastError();
 }
 
@@ -855,7 +867,7 @@ hipError_t launch_dim(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atten
   else if constexpr (kDim <= 128)
     e = launch_attend<T, kDim, 2>(pool, batch, args, split, partial, stream);
   if (e != hipSuccess || split.one_launch) return e;
-  return launch_join<T, kDim>(batch, args, split, partial, num_cus, stream);
+  return launch_join<T, kDim>(pool, batch, args, split, partial, num_cus, stream);
 }
 
 template <Kv4Type T>

@@ -441,10 +441,10 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 2) void kv4_prompt_kernel(Kv4P
   const uint32_t last = deal.begin(blockIdx.x + 1);
   int parts = 0;
   while (granule < last && at.seek(pool, batch, args, split, granule)) {
-    const uint32_t size = at.range.granules + split.lead, stop = min(size, last - at.item_at);
+    const uint32_t size = at.range.granules + lead_of<kMore>(split), stop = min(size, last - at.item_at);
     const uint32_t from = at.own(split, granule - at.item_at), upto = at.own(split, stop);
     granule = at.item_at + stop;
-    if (from == upto) continue;
+    if (kMore && from == upto) continue;
     prompt_item<T, kDim, kMore, kTree>(pool, batch, args, split, partial, at, from, upto, s_raw);
     if (from == 0 && upto < at.range.granules)
       parts = (int)(deal.worker_of(at.item_at + size - 1) - blockIdx.x) + 1;

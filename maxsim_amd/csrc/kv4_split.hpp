@@ -103,12 +103,18 @@ __device__ __forceinline__ TileRange tile_range(const Kv4AttendArgs& args, const
   return r;
 }
 
+// Granules that an item is dealt out as, besides its own.
+template <bool kMore>
+__device__ __forceinline__ uint32_t lead_of(const Split& split) {
+  return kMore ? split.lead : 0;
+}
+
 // What tile `tile` of a sequence is dealt out as, for all heads; 0 past the last.
 template <bool kMore>
 __device__ __forceinline__ uint32_t tile_share(const Kv4Pool& pool, const Kv4AttendArgs& args, const Split& split,
                                                const SeqWork& w, uint32_t tile) {
   if (tile >= w.tiles) return 0;
-  return (tile_range<kMore>(args, split, w, tile).granules + split.lead) * pool.kv_heads;
+  return (tile_range<kMore>(args, split, w, tile).granules + lead_of<kMore>(split)) * pool.kv_heads;
 }
 
 // `total` granules among `workers`: the first `extra` have one more.
@@ -150,7 +156,7 @@ struct Cursor {
                                        const Split& split, uint32_t granule) {
     for (int hops = 0;; ++hops) {
       if (tile < work.tiles) {
-        const uint32_t size = (range.granules + split.lead) * pool.kv_heads;
+        const uint32_t size = (range.granules + lead_of<kMore>(split)) * pool.kv_heads;
         if (granule - before < size) break;
         before += size;
         ++tile;
@@ -174,13 +180,13 @@ struct Cursor {
         enter(args, split, seq_work(pool, batch, split, seq), 0);
       }
     }
-    head = wave_uniform((granule - before) / (range.granules + split.lead));
-    item_at = before + head * (range.granules + split.lead);
+    head = wave_uniform((granule - before) / (range.granules + lead_of<kMore>(split)));
+    item_at = before + head * (range.granules + lead_of<kMore>(split));
     return true;
   }
   // Of what is dealt out from `from` to `upto` (counted from item_at) the item's own granules.
   __device__ __forceinline__ uint32_t own(const Split& split, uint32_t at) const {
-    return min(range.granules, at - min(at, split.lead));
+    return min(range.granules, at - min(at, lead_of<kMore>(split)));
   }
 };
 
