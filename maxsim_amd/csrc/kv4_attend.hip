@@ -44,9 +44,9 @@
 // tiles' count. A row of a tree sees, of its sequence's own rows, those whose bits are set in
 // its line: a walk over the parents makes it, in LDS, while the first tiles come; a tile of
 // 32 keys is a word of it. The walk and its barriers cost 1.5 us at 8 drafts behind 700 keys (in tiles
-// of 32 rows 16.3 us against 14.7 for a causal call; of 16, as they have there, 14.4). 32 tokens,
-// window 1,024 and 4 sinks 17.6 us (2.1 TB/s of the keys they see); three times three, window
-// 16,384 and 300 sinks, pages of 16, 29.5 us; 7 x 27 drafts behind 133 to 3,001 keys, 12 heads
+// of 32 rows 16.1 us against 14.3 for a causal call; of 16, as they have there, 13.9). 32 tokens,
+// window 1,024 and 4 sinks 17.5 us (2.1 TB/s of the keys they see); three times three, window
+// 16,384 and 300 sinks, pages of 16, 29.2 us; 7 x 27 drafts behind 133 to 3,001 keys, 12 heads
 // of 64, single precision 23 us.
 #include "kv4_split.hpp"
 
@@ -584,7 +584,7 @@ constexpr int kJoinWaves = 4;
 // by itself, and a workgroup has four rows of it; of more, each wave adds up every
 // kJoinWaves-th part and the waves' sums are joined, and a workgroup has one row. Where many
 // workgroups would find nothing to do, fewer count the pieces of work in the list of parts
-// and take them in turn (`counted`).
+// and take them in turn (kCounted).
 template <Kv4Type T, int kDim, bool kCounted>
 __global__ __launch_bounds__(kJoinWaves* kWave) void kv4_join_kernel(Kv4AttendArgs args, Split split, uint32_t rows,
                                                                  float* __restrict__ partial) {
@@ -755,7 +755,9 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
   const bool more = args != nullptr && (args->sinks > 0 || parents);
   if (more && !prompt) {
     // Of these calls, whose keys a window may count, items stay whole where there are many for
-    // their length. 32 heads of 128 on 8, one token of a sequence, by the window:
+    // their length. A tree's keys are the table's, so the rules hold where tables are as wide as
+    // the sequences; behind wider ones trees go the way of longer contexts (8 x 8 drafts behind 1,400
+    // keys, table for 131,072 tokens, 23.4 us, trimmed 19.3). 32 heads of 128 on 8, one token of a sequence, by the window:
     //   up to 512 keys always: of 4 sequences 11.6 us against 12.8 split, of 64 14.4 against 21;
     //   a workgroup for each CU, with all the waves it holds, from 7 items for each granule of one,
     //   and 10 where the longest sequence alone bounds them, others being shorter:

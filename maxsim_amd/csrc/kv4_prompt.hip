@@ -30,7 +30,7 @@
 // beside 144 vector operations of 480 ns took 727.
 // 2 x 2048 tokens behind up to 15,000, 32 heads of 128 on 8, bfloat16: 0.83 TFLOP
 // (4 dim per row and key that it sees) in 1.20 to 1.30 ms, by the card, 0.64 to 0.69
-// PFLOP/s. The same with a window of 4,096 and 64 sinks 0.28 TFLOP in 440 to 470 us, 0.59 to 0.63;
+// PFLOP/s. The same with a window of 4,096 and 64 sinks 0.28 TFLOP in 437 to 470 us, 0.59 to 0.64;
 // trees of 4 x 64 drafts behind 20,000 to 65,000 keys 0.18 in 275 to 295 us, 0.62 to 0.67 (an
 // instance without trees, another without sinks: together they spill).
 #include "kv4_split.hpp"
@@ -488,7 +488,9 @@ bool kv4_prompt_takes(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4
   // of 256 rows) is worth it. Heads of 128, 32 on 8, this kernel against the other: 4 x 64 drafts
   // behind 20,000 to 65,000 keys 310 us against 395 (41 granules), 1 x 64 behind 60,000 134
   // against 150 (15), 8 x 64 behind 4,000 81 against 98 (8), 1 x 64 behind 8,000 52 against 44 (2);
-  // tiles full to 3 / 4: 2 x 48 behind 30,000 129 against 120 (15).
+  // tiles full to 3 / 4: 2 x 48 behind 30,000 129 against 120 (15). The keys are the table's, there as
+  // wide as the sequences: behind a wider one short trees lose (1 x 64 behind 700 keys, table for
+  // 131,072 tokens, 36.9 us against 22.3 with one for 16,384).
   if (parents) {
     const int64_t each = rows / std::max(1, batch.batch);
     const int64_t tiles = (each + kPromptRows - 1) / kPromptRows * batch.batch;

@@ -7,12 +7,15 @@
 // turns per position, whose product mod 2^64 drops the whole turns, so far positions
 // lose nothing (an error of p 2^-65 turns).  Its upper 32 bits, less the nearest
 // quarter, are an angle within pi / 4 in single precision, and sine and cosine its
-// Taylor polynomials, up to 2^-28.
+// Taylor polynomials, up to 2^-28.  32 bits place the angle within 2^-30: small ones lose
+// relative bits, but a result moves by 2^-30 of its pair, beside the 2^-24 of what is
+// added up in single precision.
 //
 // Bytes bound it: every element is read and written once.  A lane has one group of
 // pairs and meets it in every head of a row, so that its angles are computed once.
 // 9,216 rows of 32 + 8 heads of 128 in bfloat16, 189 MB: 34 us over and over, 42 with other inputs
-// each time (4.5 TB/s).  16 rows: 4.4 us.  Loads of the first heads before the angles took
+// each time (4.5 TB/s); over and over in f32 75 (5.0), in f16 36, adjacent pairs 1 to 3 more.  16
+// rows: 4.4 us.  Loads of the first heads before the angles took
 // 114 registers, and 44 us.
 #include "rotary.hpp"
 

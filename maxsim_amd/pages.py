@@ -79,8 +79,9 @@ class CachePages:
         there are; its length tells.
 
         Returns (offsets int32 [batch + 1], positions int32 [rows], slots int64 [rows])
-        of the tokens given, packed by sequence: their positions, and page * page_size
-        + place in the page; -1 behind the last.  ``rows`` is the capacity for them;
+        of the tokens given, packed by sequence: their positions one after another (a
+        draft of a tree stands at its sequence's first one plus its depth), and page *
+        page_size + place in the page; -1 behind the last.  ``rows`` is the capacity for them;
         without it a tensor's sum is fetched from the device.  Enqueued on the current
         stream; can be captured in a HIP graph."""
         if isinstance(new, numbers.Integral):
