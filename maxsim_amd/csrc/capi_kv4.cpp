@@ -185,7 +185,8 @@ extern "C" int msim_kv4_attend_ex_async(const msim_kv4_pool* pool, const int32_t
     a.sinks = a.window == INT_MAX ? 0 : (int32_t)std::min<int64_t>(sinks, INT_MAX);
     a.parents = parents;
     a.scale_log2 = scale_log2;
-    check_hip(launch_kv4_attend(p, b, a, t, workspace, workspace_bytes, cus, as_stream(stream)), "launch cache attention kernels");
+    check_hip(launch_kv4_attend(p, b, a, t, workspace, workspace_bytes, cus, as_stream(stream)),
+              "launch cache attention kernels");
   });
 }
 

@@ -757,7 +757,8 @@ Split split_for(const Kv4Pool& pool, const Kv4Batch& batch, int heads, Kv4Type t
     // Of these calls, whose keys a window may count, items stay whole where there are many for
     // their length. A tree's keys are the table's, so the rules hold where tables are as wide as
     // the sequences; behind wider ones trees go the way of longer contexts (8 x 8 drafts behind 1,400
-    // keys, table for 131,072 tokens, 23.4 us, trimmed 19.3). 32 heads of 128 on 8, one token of a sequence, by the window:
+    // keys, table for 131,072 tokens, 23.4 us, trimmed 19.3). 32 heads of 128 on 8, one token of a
+    // sequence, by the window:
     //   up to 512 keys always: of 4 sequences 11.6 us against 12.8 split, of 64 14.4 against 21;
     //   a workgroup for each CU, with all the waves it holds, from 7 items for each granule of one,
     //   and 10 where the longest sequence alone bounds them, others being shorter:
@@ -824,15 +825,21 @@ hipError_t launch_join(const Kv4Pool& pool, const Kv4Batch& batch, const Kv4Atte
   // with 32, up to 128 items, 2.5 us; 256 with 32 each of 256, up to 128 items, 5. It saves none
   // where there may be a piece for each (4 x 400 tokens behind 2,100, 32 heads of 128: 141 us, counted
   // 151), and under a window, where fewer items than workers are short and all of them split, few
-  // (32 x 5 tokens, window 300: 28.3, counted 29.8). The workgroups of a single long item
-  // would all be on one XCD (8 heads of 256 on 1, single precision, 30,000 keys: 31.3, counted 20.0).
+  // (32 x 5 tokens, window 300: 28.3, counted 29.8). The workgroups of an item are all on one XCD,
+  // so few items of a megabyte and more are counted too (8 heads of 256 on 1, single precision, 30,000
+  // keys, 2 MB: 31.3, counted 20.0; 12 heads of 64 on 2, 360 kB: 16.5 against 17.2).
   const uint32_t y = std::min(32u, rows);
   const uint64_t groups = (uint64_t)split.workers * y;
   const uint64_t items = (((uint64_t)batch.rows * split.share >> split.tile_shift) + batch.batch) * pool.kv_heads;
   const uint64_t pieces = std::min<uint64_t>(items, split.workers) * ((rows + kJoinWaves - 1) / kJoinWaves);
-  const dim3 block(kJoinWaves * kWave);
+  const int64_t longest = (int64_t)batch.max_pages << pool.page_shift;
+  const int64_t keys = args.causal && args.parents == nullptr ? std::min<int64_t>(longest, args.window) : longest;
+  const uint64_t parts =
+      std::min<uint64_t>((keys >> split.granule_shift) + 1, split.workers / std::max<uint64_t>(items, 1));
   const bool all_split = args.window != INT_MAX && items < split.workers;
-  if ((groups > 6144 && pieces < (all_split ? groups / 12 : groups)) || items < 4)
+  const dim3 block(kJoinWaves * kWave);
+  if ((groups > 6144 && pieces < (all_split ? groups / 12 : groups)) ||
+      (items < 8 && parts * rows * kDim * sizeof(float) >= 1 << 20))
     kv4_join_kernel<T, kDim, true><<<dim3(num_cus * 4), block, 0, stream>>>(args, split, rows, partial);
   else
     kv4_join_kernel<T, kDim, false><<<dim3(split.workers, y), block, 0, stream>>>(args, split, rows, partial);
